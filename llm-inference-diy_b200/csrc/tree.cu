@@ -1,0 +1,440 @@
+// tree.cu — the speculative-decoding operators around the tree attention (include/llmdiy_tree.h):
+// bias + rotary positions of a tree's rows, verification of the drafts, and the commit of the
+// accepted K/V rows.  No counterpart in the reference, which decodes one token per step.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "llmdiy_tree.h"
+
+using namespace llmdiy;
+
+namespace {
+
+constexpr int kDim = 128;  // head dimension
+constexpr int kMaxNodes = LLMDIY_TREE_MAX_NODES;
+
+inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
+    return tree_len ? min(max(tree_len[b], 0), N) : N;
+}
+
+// ---------------------------------------------------------------- bias + RoPE
+// One CTA per node.  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
+// to [-pi, pi] in 64 bits (a position of 10^5 leaves fp32 angles only 2 digits after the point), its sine
+// and cosine are then taken in fp32 (absolute error < 2^-21, against 2^-11 of the fp16 outputs).
+__global__ void __launch_bounds__(256)
+    tree_rope_k(const half* __restrict__ qkv, const half* __restrict__ bias, const int* __restrict__ depth,
+                const int* __restrict__ len, const int* __restrict__ tree_len, int N, int H, int KV, double log2_base,
+                half* __restrict__ Q, half* __restrict__ TK, half* __restrict__ TV) {
+    __shared__ float cs[kDim / 2], sn[kDim / 2];
+    const int b = blockIdx.y, i = blockIdx.x, tid = threadIdx.x;
+    if (i >= nodes_of(tree_len, b, N)) return;
+    const size_t row = (size_t)b * N + i;
+    if (tid < kDim / 2) {
+        const double pos = (double)len[b] + depth[row];
+        const double a = pos * exp2(-log2_base * tid / (kDim / 2));
+        constexpr double kTurn = 6.283185307179586476925;
+        const float r = (float)(a - kTurn * rint(a * (1.0 / kTurn)));
+        sincosf(r, &sn[tid], &cs[tid]);
+    }
+    __syncthreads();
+    const half* src = qkv + row * (H + 2 * KV) * kDim;
+    // rotated heads: 8 threads per head, each 8 pairs (two 16-byte loads); then the value rows
+    for (int u = tid; u < (H + KV) * 8; u += blockDim.x) {
+        const int h = u >> 3, t0 = (u & 7) * 8;
+        float x1[8], x2[8], r1[8], r2[8];
+        unpack8(*reinterpret_cast<const uint4*>(src + h * kDim + t0), x1);
+        unpack8(*reinterpret_cast<const uint4*>(src + h * kDim + t0 + 64), x2);
+        if (bias) {
+            float b1[8], b2[8];
+            unpack8(*reinterpret_cast<const uint4*>(bias + h * kDim + t0), b1);
+            unpack8(*reinterpret_cast<const uint4*>(bias + h * kDim + t0 + 64), b2);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { x1[e] += b1[e]; x2[e] += b2[e]; }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float c = cs[t0 + e], s = sn[t0 + e];
+            r1[e] = x1[e] * c - x2[e] * s;
+            r2[e] = x2[e] * c + x1[e] * s;
+        }
+        half* dst = h < H ? Q + (row * H + h) * kDim : TK + (row * KV + (h - H)) * kDim;
+        *reinterpret_cast<uint4*>(dst + t0) = pack8(r1);
+        *reinterpret_cast<uint4*>(dst + t0 + 64) = pack8(r2);
+    }
+    for (int u = tid; u < KV * 16; u += blockDim.x) {
+        float x[8];
+        unpack8(*reinterpret_cast<const uint4*>(src + (H + KV) * kDim + u * 8), x);
+        if (bias) {
+            float bb[8];
+            unpack8(*reinterpret_cast<const uint4*>(bias + (H + KV) * kDim + u * 8), bb);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += bb[e];
+        }
+        *reinterpret_cast<uint4*>(TV + row * KV * kDim + u * 8) = pack8(x);
+    }
+}
+
+// ---------------------------------------------------------------- verification
+// A cluster of C CTAs per sequence.  Every thread walks the tree from shared memory (the tested
+// entries p(x_i), q(x_i) of all nodes are fetched at the start, in one round trip); a refused
+// child needs the sum of max(0, p - T q) over the row, and the end of the walk its running sum.  The row is cut
+// into blocks of 128 entries, dealt contiguously to the cluster's warps (warp k of K: blocks
+// [k U / K, (k + 1) U / K)), so the warps' totals in order are a running sum over the row.
+constexpr int kVerThreads = 512;
+constexpr int kVerWarps = kVerThreads / 32;
+constexpr int kVerMaxCluster = 16;
+
+struct VerRow {
+    const float* p;
+    const float* q;  // NULL: no draft distribution
+    double T;        // weight of entry v: max(0, p - T q)
+    int V;
+    bool vec;  // rows are 16-byte aligned: four entries a load
+};
+
+LLMDIY_DEV double positive(double x) { return x > 0.0 ? x : 0.0; }  // NaN counts as 0
+
+// Weights of the four entries v0 .. v0 + 3 (0 past V).
+LLMDIY_DEV void ver_weights(const VerRow& r, int v0, double* w) {
+    float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool use_q = r.q != nullptr && r.T != 0.0;
+    if (r.vec && v0 + 3 < r.V) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(r.p + v0));
+        p[0] = a.x; p[1] = a.y; p[2] = a.z; p[3] = a.w;
+        if (use_q) {
+            const float4 c = __ldg(reinterpret_cast<const float4*>(r.q + v0));
+            q[0] = c.x; q[1] = c.y; q[2] = c.z; q[3] = c.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (v0 + e < r.V) {
+                p[e] = __ldg(r.p + v0 + e);
+                if (use_q) q[e] = __ldg(r.q + v0 + e);
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const double pe = positive(p[e]);
+        w[e] = use_q ? positive(pe - r.T * positive(q[e])) : pe;
+    }
+}
+
+LLMDIY_DEV double warp_sum(double x) {
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+    return x;
+}
+
+struct VerSmem {
+    int parent[kMaxNodes], token[kMaxNodes], child[kMaxNodes], sibling[kMaxNodes];
+    double p[kMaxNodes], q[kMaxNodes], u[kMaxNodes];
+    double part[2][kVerMaxCluster * kVerWarps];  // the cluster's warp totals, in order (two rounds)
+    int dead[kMaxNodes];                         // refused tokens of the current node (no draft distribution)
+};
+
+__global__ void __launch_bounds__(kVerThreads)
+    tree_verify_k(const float* __restrict__ target, int ldt, const float* __restrict__ draft, int ldd,
+                  const int* __restrict__ token, const int* __restrict__ parent, const int* __restrict__ tree_len,
+                  const float* __restrict__ uniform, int N, int V, int vec, int* __restrict__ path,
+                  int* __restrict__ accepted, int* __restrict__ next) {
+    namespace cg = cooperative_groups;
+    __shared__ VerSmem s;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n = nodes_of(tree_len, b, N);
+    const size_t row0 = (size_t)b * N;
+    if (rank == 0)
+        for (int i = tid; i < N; i += kVerThreads) path[row0 + i] = -1;
+    if (n == 0) {
+        if (rank == 0 && tid == 0) { accepted[b] = -1; next[b] = -1; }
+        return;  // the whole cluster
+    }
+    if (tid < n) {
+        const int par = tid ? parent[row0 + tid] : -1;
+        const int tok = tid ? token[row0 + tid] : 0;
+        const bool ok = par >= 0 && par < tid && tok >= 0 && tok < V;
+        s.parent[tid] = ok ? par : -1;
+        s.token[tid] = tok;
+        s.u[tid] = uniform[row0 + tid];
+        s.p[tid] = ok ? positive(target[(row0 + par) * ldt + tok]) : 0.0;
+        s.q[tid] = ok ? (draft ? positive(draft[(row0 + par) * ldd + tok]) : 1.0) : 0.0;
+    }
+    __syncthreads();
+    if (tid < n) {  // first child and next sibling in index order
+        int child = -1, sib = -1;
+        for (int j = n - 1; j > tid; --j) {
+            if (s.parent[j] == tid) child = j;
+            if (s.parent[j] == s.parent[tid]) sib = j;
+        }
+        s.child[tid] = child;
+        s.sibling[tid] = s.parent[tid] >= 0 ? sib : -1;
+    }
+    cluster.sync();  // every CTA of the cluster runs: its shared memory may be written
+
+    const int U = (V + 127) / 128, K = C * kVerWarps, k = rank * kVerWarps + warp;
+    const int u0 = (int)((long long)U * k / K), u1 = (int)((long long)U * (k + 1) / K);
+    VerRow r;
+    r.V = V;
+    r.vec = vec;
+    int round = 0, dead0 = 0, ndead = 0;  // the current node's refused tokens: s.dead[dead0 .. dead0 + ndead)
+    // weights of this lane's four entries of a block, without the refused tokens
+    auto weights = [&](int u, double* w) {
+        const int v0 = u * 128 + lane * 4;
+        ver_weights(r, v0, w);
+        for (int j = 0; j < ndead; ++j) {
+            const int x = s.dead[dead0 + j] - v0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = x == e ? 0.0 : w[e];
+        }
+    };
+    // this warp's total goes into every CTA's table; returns the table once it is complete.  Two tables
+    // take turns: a CTA writes table r & 1 again only after the barrier of round r + 1, which every CTA
+    // reaches after it has read round r's.
+    auto totals = [&]() -> const double* {
+        double t = 0.0;
+        for (int u = u0; u < u1; ++u) {
+            double w[4];
+            weights(u, w);
+            t += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        t = warp_sum(t);
+        double* mine = s.part[round++ & 1];
+        if (lane < C) cluster.map_shared_rank(mine, lane)[k] = t;
+        cluster.sync();
+        return mine;
+    };
+    // lane l's share of the table: entries [l K / 32, (l + 1) K / 32)
+    const int j0 = K * lane / 32, j1 = K * (lane + 1) / 32;
+    auto lane_sum = [&](const double* tab) {
+        double t = 0.0;
+        for (int j = j0; j < j1; ++j) t += tab[j];
+        return t;
+    };
+
+    int cur = 0, cand = s.child[0], count = 0;
+    double Sj = 1.0;
+    auto at_node = [&](int c) {
+        cur = c;
+        cand = s.child[c];
+        r.p = target + (row0 + c) * ldt;
+        r.q = draft ? draft + (row0 + c) * ldd : nullptr;
+        r.T = 0.0;
+        Sj = 1.0;
+        dead0 += ndead;  // every node is refused once at most: the list never overflows
+        ndead = 0;
+    };
+    at_node(0);
+    while (cand >= 0) {  // every thread of the cluster takes the same steps
+        double w = positive(s.p[cand] - r.T * s.q[cand]);
+        for (int j = 0; j < ndead; ++j)
+            if (s.dead[dead0 + j] == s.token[cand]) w = 0.0;
+        if (s.u[cand] * Sj * s.q[cand] < w) {
+            if (rank == 0 && tid == 0) path[row0 + count] = cand;
+            ++count;
+            at_node(cand);
+            continue;
+        }
+        if (!draft) {
+            s.dead[dead0 + ndead] = s.token[cand];  // (the same value from every thread)
+            ++ndead;
+            Sj -= w;
+        } else {
+            r.T += Sj;
+            if (s.sibling[cand] >= 0) Sj = warp_sum(lane_sum(totals()));
+        }
+        cand = s.sibling[cand];
+    }
+
+    // the last token: first entry whose running sum of weights exceeds u_0 * their sum
+    const double* tab;
+    double t, inc, total;
+    for (int attempt = 0;; ++attempt) {
+        tab = totals();
+        t = lane_sum(tab);
+        inc = t;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const double o = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += o;
+        }
+        total = __shfl_sync(0xffffffffu, inc, 31);
+        if (total > 0.0 || attempt) break;
+        r.T = 0.0;  // nothing left: from the target's row itself
+        ndead = 0;
+    }
+    if (rank == 0 && tid == 0) {
+        accepted[b] = count;
+        if (!(total > 0.0)) next[b] = -1;
+    }
+    if (!(total > 0.0)) return;
+    const double goal = s.u[0] * total;
+    // The lane, then its table entry, then the lane of a block and its entry: at each level the first
+    // one with a positive weight whose running sum exceeds the goal, or, where the levels' sums differ in
+    // their last bits so that none does, the last one with a positive weight.
+    auto pick_lane = [&](double running, double own) -> int {
+        const unsigned any = __ballot_sync(0xffffffffu, own > 0.0);
+        const unsigned hit = __ballot_sync(0xffffffffu, own > 0.0 && running > goal);
+        return hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : -1;
+    };
+    const int f = pick_lane(inc, t);
+    double base = __shfl_up_sync(0xffffffffu, inc, 1);
+    if (lane == 0) base = 0.0;
+    int mine = -1;
+    double mine_base = 0.0;
+    for (int j = j0; j < j1; ++j) {
+        if (tab[j] > 0.0) {
+            mine = j;
+            mine_base = base;
+            if (base + tab[j] > goal) break;
+        }
+        base += tab[j];
+    }
+    const int chosen = __shfl_sync(0xffffffffu, mine, f);
+    base = __shfl_sync(0xffffffffu, mine_base, f);
+    if (chosen != k) return;
+    int answer = -1;
+    for (int u = u0; u < u1; ++u) {
+        double w[4];
+        weights(u, w);
+        const double own = (w[0] + w[1]) + (w[2] + w[3]);
+        double run = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const double o = __shfl_up_sync(0xffffffffu, run, d);
+            if (lane >= d) run += o;
+        }
+        const double block = __shfl_sync(0xffffffffu, run, 31);
+        const int l = pick_lane(base + run, own);
+        if (l >= 0) {
+            double before = __shfl_up_sync(0xffffffffu, run, 1);
+            if (lane == 0) before = 0.0;
+            before += base;
+            int at = -1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool open = at < 0 || !(before > goal);  // not past the goal yet
+                if (open && w[e] > 0.0) at = u * 128 + lane * 4 + e;
+                if (open) before += w[e];
+            }
+            answer = __shfl_sync(0xffffffffu, at, l);
+        }
+        if (base + block > goal && answer >= 0) break;
+        base += block;
+    }
+    if (lane == 0) next[b] = answer;
+}
+
+// ---------------------------------------------------------------- commit
+// One CTA per (layer, sequence); a thread copies 16 bytes of K or V of one row at a time.
+__global__ void __launch_bounds__(256)
+    tree_commit_k(const half* __restrict__ TK, const half* __restrict__ TV, size_t tree_layer_stride, half* K, half* V,
+                  size_t layer_stride, int stride, int slot_rows, int num_slots, const int* __restrict__ slot,
+                  const int* __restrict__ len, const int* __restrict__ path, const int* __restrict__ accepted, int N,
+                  int cols, int* __restrict__ len_out) {
+    const int b = blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
+    const int at = slot ? slot[b] : b, m = len[b], acc = accepted[b];
+    const bool ok = at >= 0 && at < num_slots && m >= 0 && m <= slot_rows && acc >= 0;
+    const int rows = ok ? min(1 + min(acc, N - 1), slot_rows - m) : 0;
+    if (l == 0 && tid == 0 && len_out) len_out[b] = m + rows;
+    const half* tk = TK + (size_t)l * tree_layer_stride + (size_t)b * N * cols;
+    const half* tv = TV + (size_t)l * tree_layer_stride + (size_t)b * N * cols;
+    const size_t base = (size_t)l * layer_stride + ((size_t)(ok ? at : 0) * slot_rows + m) * stride;
+    const int per = cols / 8;  // 16-byte pieces of a row
+    for (int x = tid; x < rows * 2 * per; x += blockDim.x) {
+        const int row = x / (2 * per), c = x - row * 2 * per;
+        const int node = row ? path[(size_t)b * N + row - 1] : 0;
+        if (node < 0 || node >= N) continue;
+        const bool v = c >= per;
+        const int e = (v ? c - per : c) * 8;
+        const uint4 y = *reinterpret_cast<const uint4*>((v ? tv : tk) + (size_t)node * cols + e);
+        *reinterpret_cast<uint4*>((v ? V : K) + base + (size_t)row * stride + e) = y;
+    }
+}
+
+// Grid limits and products of sizes that index in 32 bits.
+bool sizes_ok(int B, int N, int H, int KV) {
+    return B > 0 && B <= 65535 && N > 0 && N <= kMaxNodes && KV > 0 && H >= KV && H % KV == 0 && H <= 1024;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmdiy_tree_layout(const int* parent, int n, int* depth, uint64_t* mask, int mask_words) {
+    if (!parent || !depth || !mask || n < 1 || n > kMaxNodes || mask_words < (n + 63) / 64 || parent[0] != -1)
+        return -1;
+    for (int i = 1; i < n; ++i)
+        if (parent[i] < 0 || parent[i] >= i) return -1;
+    for (int i = 0; i < n; ++i) {
+        const int p = parent[i];
+        uint64_t* m = mask + (size_t)i * mask_words;
+        for (int w = 0; w < mask_words; ++w) m[w] = p < 0 ? 0 : mask[(size_t)p * mask_words + w];
+        m[i / 64] |= 1ull << (i % 64);
+        depth[i] = p < 0 ? 0 : depth[p] + 1;
+    }
+    return 0;
+}
+
+int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth, const int* len,
+                     const int* tree_len, int B, int N, int num_heads, int num_kv_heads, float rope_base,
+                     uint16_t* Q, uint16_t* TK, uint16_t* TV, void* stream) {
+    if (!sizes_ok(B, N, num_heads, num_kv_heads) || !qkv || !depth || !len || !Q || !TK || !TV || !aligned16(qkv) ||
+        !aligned16(bias) || !aligned16(Q) || !aligned16(TK) || !aligned16(TV) || !(rope_base > 0.f) ||
+        !(rope_base < INFINITY))
+        return (int)cudaErrorInvalidValue;
+    tree_rope_k<<<dim3(N, B), 256, 0, S(stream)>>>(
+        reinterpret_cast<const half*>(qkv), reinterpret_cast<const half*>(bias), depth, len, tree_len, N, num_heads,
+        num_kv_heads, log2((double)rope_base), reinterpret_cast<half*>(Q), reinterpret_cast<half*>(TK),
+        reinterpret_cast<half*>(TV));
+    return (int)cudaGetLastError();
+}
+
+int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd, const int* token,
+                       const int* parent, const int* tree_len, const float* uniform, int B, int N, int V, int* path,
+                       int* accepted, int* next, void* stream) {
+    if (B <= 0 || B > 65535 || N <= 0 || N > kMaxNodes || V <= 0 || !target || ldt < V || (draft && ldd < V) || !token ||
+        !parent || !uniform || !path || !accepted || !next || !aligned4(target) || !aligned4(draft))
+        return (int)cudaErrorInvalidValue;
+    const int vec = aligned16(target) && ldt % 4 == 0 && (!draft || (aligned16(draft) && ldd % 4 == 0));
+    constexpr int C = 1;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(B * C);
+    lc.blockDim = dim3(kVerThreads);
+    lc.stream = S(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&lc, tree_verify_k, target, ldt, draft, ldd, token, parent, tree_len, uniform, N, V,
+                                   vec, path, accepted, next);
+}
+
+int llmdiy_tree_commit(const uint16_t* TK, const uint16_t* TV, size_t tree_layer_stride, uint16_t* K, uint16_t* V,
+                       size_t layer_stride, int stride, int slot_rows, int num_slots, const int* slot,
+                       const int* len, const int* path, const int* accepted, int B, int N, int num_kv_heads,
+                       int layers, int* len_out, void* stream) {
+    const int cols = num_kv_heads * kDim;
+    if (!sizes_ok(B, N, num_kv_heads, num_kv_heads) || !TK || !TV || !K || !V || !len || !path || !accepted ||
+        layers <= 0 || layers > 65535 || slot_rows <= 0 || num_slots <= 0 || stride < cols || (stride & 7) ||
+        (layer_stride & 7) || (tree_layer_stride & 7) || len_out == len ||
+        (layers > 1 && (layer_stride < ((size_t)num_slots * slot_rows - 1) * stride + cols ||
+                        tree_layer_stride < (size_t)B * N * cols)) ||
+        !aligned16(TK) || !aligned16(TV) || !aligned16(K) || !aligned16(V))
+        return (int)cudaErrorInvalidValue;
+    tree_commit_k<<<dim3(B, layers), 256, 0, S(stream)>>>(
+        reinterpret_cast<const half*>(TK), reinterpret_cast<const half*>(TV), tree_layer_stride,
+        reinterpret_cast<half*>(K), reinterpret_cast<half*>(V), layer_stride, stride, slot_rows, num_slots, slot, len,
+        path, accepted, N, cols, len_out);
+    return (int)cudaGetLastError();
+}
+
+}  // extern "C"

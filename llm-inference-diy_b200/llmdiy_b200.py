@@ -1,4 +1,5 @@
-"""ctypes binding of libllmdiy_b200.so (include/llmdiy_kernels.h, include/llmdiy_engine.h).
+"""ctypes binding of libllmdiy_b200.so (include/llmdiy_kernels.h, include/llmdiy_engine.h,
+include/llmdiy_batch.h, include/llmdiy_tree.h).
 
 Host-side mirror of the reference's interfaces for Python callers: the
 `Engine` class follows QwenEngine (framework_src/qwen_infer.cu:69-738) --
@@ -95,6 +96,13 @@ def lib() -> ctypes.CDLL:
         "llmdiy_scatter_interleaved": [P, P, I, I, I, P],
         "llmdiy_transpose_weight": [P, P, I, I, P],
         "llmdiy_transpose_weight_gpu": [ctypes.POINTER(ctypes.c_void_p), I, I],
+        "llmdiy_tree_layout": [IP, I, IP, ctypes.POINTER(U64), I],
+        "llmdiy_tree_rope": [P, P, P, P, P, I, I, I, I, F, P, P, P, P],
+        "llmdiy_tree_attn": [P, I, P, P, I, I, I, P, P, I, P, P, P, P, I, I, I, I, P, I, P, SZ, P],
+        "llmdiy_tree_attn_status": [P],
+        "llmdiy_softmax_rows": [P, I, P, I, I, P, I, P],
+        "llmdiy_tree_verify": [P, I, P, I, P, P, P, P, I, I, I, P, P, P, P],
+        "llmdiy_tree_commit": [P, P, SZ, P, P, SZ, I, I, I, P, P, P, P, I, I, I, I, P, P],
         "llmdiy_qwdf_read_config": [ctypes.c_char_p, ctypes.POINTER(Config)],
         "llmdiy_qwdf_validate": [ctypes.c_char_p, ctypes.POINTER(Config), ctypes.POINTER(U64), ctypes.c_char_p, SZ],
         "llmdiy_qwdf_write_random": [ctypes.c_char_p, ctypes.POINTER(Config), U64, F, I],
@@ -141,6 +149,8 @@ def lib() -> ctypes.CDLL:
     L.llmdiy_batch_destroy.restype = None
     L.llmdiy_batch_last_error.argtypes = [P]
     L.llmdiy_batch_last_error.restype = ctypes.c_char_p
+    L.llmdiy_tree_attn_work_bytes.argtypes = [I, I, I, I, I]
+    L.llmdiy_tree_attn_work_bytes.restype = SZ
     L.llmdiy_fd_mh_work_bytes.argtypes = [I, I]
     L.llmdiy_fd_mh_work_bytes.restype = SZ
     _lib = L
@@ -313,6 +323,61 @@ def scatter_interleaved(src, dst, N, num_heads, dst_cols, stream=None):
 
 def transpose_weight(out, inp, rows, cols, stream=None):
     _check(lib().llmdiy_transpose_weight(_p(out), _p(inp), rows, cols, _p(stream)), "transpose_weight")
+
+
+# ------------------------------------------- speculative decoding (llmdiy_tree.h)
+def tree_layout(parent):
+    """Host helper: (depth [n] int32, mask [n][ceil(n/64)] uint64) of one tree from its parents
+    (parent[0] = -1, parent[i] < i).  Raises LlmdiyError for anything else or more than 256 nodes."""
+    import numpy as np
+    n = len(parent)
+    words = max(1, (n + 63) // 64)
+    depth, mask = np.zeros(n, np.int32), np.zeros((n, words), np.uint64)
+    _check(lib().llmdiy_tree_layout(_ints(parent), n, depth.ctypes.data_as(ctypes.POINTER(ctypes.c_int)),
+                                    mask.ctypes.data_as(ctypes.POINTER(ctypes.c_uint64)), words), "tree_layout")
+    return depth, mask
+
+
+def tree_rope(qkv, bias, depth, lens, tree_len, B, N, num_heads, num_kv_heads, rope_base, Q, TK, TV, stream=None):
+    """Bias and rotary positions (len + depth) of a tree's rows: qkv -> Q and the tree's K/V rows TK, TV."""
+    _check(lib().llmdiy_tree_rope(_p(qkv), _p(bias), _p(depth), _p(lens), _p(tree_len), B, N, num_heads, num_kv_heads,
+                                  rope_base, _p(Q), _p(TK), _p(TV), _p(stream)), "tree_rope")
+
+
+def tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len):
+    return int(lib().llmdiy_tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len))
+
+
+def tree_attn(Q, ldq, K, V, stride, slot_rows, num_slots, slot, lens, max_len, TK, TV, mask, tree_len, B, N,
+              num_heads, num_kv_heads, O, ldo, work, work_bytes, stream=None):
+    """Attention of the tree's nodes over their sequences' cache rows and the tree rows their mask names."""
+    _check(lib().llmdiy_tree_attn(_p(Q), ldq, _p(K), _p(V), stride, slot_rows, num_slots, _p(slot), _p(lens), max_len,
+                                  _p(TK), _p(TV), _p(mask), _p(tree_len), B, N, num_heads, num_kv_heads, _p(O), ldo,
+                                  _p(work), work_bytes, _p(stream)), "tree_attn")
+
+
+def tree_attn_status(work):
+    return lib().llmdiy_tree_attn_status(_p(work))
+
+
+def softmax_rows(logits, ldl, temp, R, V, probs, ldp, stream=None):
+    """probs[r] = softmax(logits[r] / temp[r]) in fp32 (temp None: 1; 0: equal shares of the largest entries)."""
+    _check(lib().llmdiy_softmax_rows(_p(logits), ldl, _p(temp), R, V, _p(probs), ldp, _p(stream)), "softmax_rows")
+
+
+def tree_verify(target, ldt, draft, ldd, token, parent, tree_len, uniform, B, N, V, path, accepted, next_token,
+                stream=None):
+    """Accepted path, its length and the next token of each sequence's tree (draft None: deterministic drafts)."""
+    _check(lib().llmdiy_tree_verify(_p(target), ldt, _p(draft), ldd, _p(token), _p(parent), _p(tree_len), _p(uniform),
+                                    B, N, V, _p(path), _p(accepted), _p(next_token), _p(stream)), "tree_verify")
+
+
+def tree_commit(TK, TV, tree_layer_stride, K, V, layer_stride, stride, slot_rows, num_slots, slot, lens, path,
+                accepted, B, N, num_kv_heads, layers, len_out, stream=None):
+    """The root's and the accepted nodes' K/V rows of every layer into cache rows len, len + 1, ..."""
+    _check(lib().llmdiy_tree_commit(_p(TK), _p(TV), tree_layer_stride, _p(K), _p(V), layer_stride, stride, slot_rows,
+                                    num_slots, _p(slot), _p(lens), _p(path), _p(accepted), B, N, num_kv_heads, layers,
+                                    _p(len_out), _p(stream)), "tree_commit")
 
 
 # ----------------------------------------------------------------- QWDF files
