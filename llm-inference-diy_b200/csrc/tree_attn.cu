@@ -1,78 +1,682 @@
-// tree_attn.cu — attention of a tree of drafted tokens over the cache (include/llmdiy_tree.h).
-// No counterpart in the reference, which attends one query token per step.
+// tree_attn.cu — attention of a tree of drafted tokens over the cache (include/llmdiy_tree.h), on the
+// tcgen05 tensor cores.  No counterpart in the reference, which attends one query token per step.
+//
+// Work.  A unit is (sequence, kv head, M tile): the query rows m = node * G + g of the G heads that share the kv
+// head, at most 128 rows (the MMA's M) of whole nodes.  A unit's keys are 64-row tiles: the cache
+// rows [0, len), then the tree's own rows.  All units' tiles in a row are dealt to a grid of two CTAs per
+// SM in equal contiguous ranges, cut anywhere (CTA w of W: tiles [total w / W, total (w + 1) / W)), whatever
+// the sequences' lengths: ragged batches and single sequences alike keep every SM busy to the end.
+// A range holds at most one unit's end, some whole units and one unit's beginning; whole units write
+// their output, cut ones an fp32 partial (o unnormalised, m, l), which tree_merge_k joins by
+// log-sum-exp in order (a fixed order: the same bits every time).
+//
+// CTA.  Warp 4 streams Q (once per unit) and the K and V tiles by TMA through rings that run on
+// across units; warp 5 issues the MMAs:
+//   S(j)  = Q K(j)^T          128 x 64,  K = 128 dims  -> TMEM (two S buffers)
+//   O    += P(j) V(j)         128 x 128, K = 64 keys   -> TMEM (P from TMEM, over its S)
+// with S(j+1) issued before PV(j).  Warps 0-3 own the rows (thread = row = TMEM lane): mask, online
+// softmax in base 2, P as fp16; O is rescaled only when a row's maximum grows by more than 2^8 (P stays
+// within fp16, and O / l does not depend on the reference point).  fp16 P costs 2^-11 of each
+// probability, as the fp16 output does; l sums the unrounded fp32 values.
+//
+// What a row does not see must not reach it even as NaN * 0: masked scores are replaced by -inf
+// (K may hold anything there), and V rows past the end, as well as tree rows with an Inf or NaN, are zeroed in
+// shared memory before PV; the few rows that do see such a tree row add p * v themselves at the end.
+//
+// Every wait is bounded; on expiry the CTA records an error in *err, waits (bounded) for its copies and
+// MMAs in flight, frees its TMEM and returns.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "gemm_tc_host.h"
 #include "llmdiy_tree.h"
 #include "ops.cuh"
+#include "tc.cuh"
 
 using namespace llmdiy;
 
 namespace {
 
 constexpr int kTaDim = 128;
-constexpr int kTaThreads = 128;
+constexpr int kTaKeys = 64;      // keys per tile
+constexpr int kTaRows = 128;     // query rows of a unit at most (MMA M)
+constexpr int kTaThreads = 192;  // warps 0-3: rows; warp 4: TMA; warp 5: MMA issue
+constexpr int kTaCtasPerSm = 2;
+constexpr int kTaTileBytes = kTaKeys * kTaDim * 2;  // one K or V tile
+constexpr uint32_t kTaCols = 256;                   // TMEM: S0 | S1 | O (128 columns)
+constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
 
-// One CTA per (head, node, sequence): half-warp q takes keys q, q + 8, ... of the cache rows and then of the
-// tree's, each lane holding 8 of the 128 dims, with an online softmax per half-warp.
-__global__ void __launch_bounds__(kTaThreads)
-    tree_attn_k(const half* __restrict__ Q, int ldq, const half* __restrict__ K, const half* __restrict__ V, int stride,
-                int slot_rows, int num_slots, const int* __restrict__ slot, const int* __restrict__ len, int max_len,
-                const half* __restrict__ TK, const half* __restrict__ TV, const uint64_t* __restrict__ mask,
-                const int* __restrict__ tree_len, int N, int H, int KV, half* __restrict__ O, int ldo) {
-    __shared__ float so[4][kTaDim], sm[4], sl[4];
-    const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-    const int n = tree_len ? min(max(tree_len[b], 0), N) : N;
-    if (i >= n) return;
-    const int warp = tid >> 5, lane = tid & 31, hw = lane >> 4, dl = (lane & 15) * 8, hq = warp * 2 + hw;
-    const int kvh = h / (H / KV);
-    const int at = slot ? slot[b] : b;
-    const int L = at >= 0 && at < num_slots ? min(max(len[b], 0), max_len) : 0;
-    const size_t row = (size_t)b * N + i;
-    const uint64_t* mw = mask + row * ((N + 63) / 64);
-    const half* Kb = K + (size_t)max(at, 0) * slot_rows * stride + kvh * kTaDim + dl;
-    const half* Vb = V + (size_t)max(at, 0) * slot_rows * stride + kvh * kTaDim + dl;
-    const half* Tk = TK + ((size_t)b * N * KV + kvh) * kTaDim + dl;
-    const half* Tv = TV + ((size_t)b * N * KV + kvh) * kTaDim + dl;
-    float q8[8], o8[8], m = -INFINITY, l = 0.f;
-    unpack8(*reinterpret_cast<const uint4*>(Q + row * ldq + h * kTaDim + dl), q8);
+// Two layouts of the same kernel: units of up to 64 rows need only 16 KB for Q and get a third K
+// stage; the MMA still reads 128 rows, so rows 64-127 of its A operand are whatever lies behind
+// (rows do not mix, and nothing is read out of those).
+template <int QR, int KS, int VS>
+struct TaSmem {
+    half q[2][QR * 64];           // dims 0-63 | 64-127: K-major, 128-byte swizzle
+    half k[KS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, K-major (8 KB each)
+    half v[VS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, MN-major (8 KB each)
+    uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
+    uint64_t s_full[2], p_full[2], o_done[2], drain;
+    // tree rows with a non-finite V, by tree tile and quarter (a warp's 16 rows); two units' worth
+    alignas(8) uint16_t bad[2][4][4];
+    uint32_t tmem_base;
+    int fail;
+};
+
+struct TaArgs {
+    const int* slot;
+    const int* len;
+    const int* tree_len;
+    const uint64_t* mask;
+    const half *Q, *TK, *TV;  // for the rare rows that see a non-finite V
+    half* O;
+    float* part;  // [W][2][rows][128] fp32, then [W][2][rows][2]
+    int B, N, H, KV, ldq, ldo, slot_rows, num_slots, max_len;
+    int rows;  // rows of a partial: G * nodes_per_tile
+    int npt;   // nodes per M tile
+    int W;     // most CTAs that share the tiles
+    int evict_first;
+};
+
+LLMDIY_DEV int ta_nodes(const TaArgs& a, int b) {
+    return a.tree_len ? min(max(a.tree_len[b], 0), a.N) : a.N;
+}
+LLMDIY_DEV int ta_slot(const TaArgs& a, int b) { return a.slot ? a.slot[b] : b; }
+LLMDIY_DEV int ta_len(const TaArgs& a, int b) {
+    const int s = ta_slot(a, b);
+    return s >= 0 && s < a.num_slots ? min(max(a.len[b], 0), a.max_len) : 0;
+}
+// Tiles of a unit of sequence b, and its units.
+LLMDIY_DEV void ta_shape(const TaArgs& a, int b, int& n, int& L, int& tiles, int& units) {
+    n = ta_nodes(a, b);
+    L = n ? ta_len(a, b) : 0;
+    tiles = (L + kTaKeys - 1) / kTaKeys + (n + kTaKeys - 1) / kTaKeys;
+    units = a.KV * ((n + a.npt - 1) / a.npt);
+}
+
+// Tiles of all sequences before b (b = B: all).  A whole warp calls it together.
+LLMDIY_DEV long long ta_tiles_before(const TaArgs& a, int b, int lane) {
+    long long t = 0;
+    for (int i = lane; i < b; i += 32) {
+        int n, L, tiles, units;
+        ta_shape(a, i, n, L, tiles, units);
+        t += (long long)tiles * units;
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o8[e] = 0.f;
-    const float scale = 0.08838834764831845f;
-    for (int k0 = 0; k0 < L + n; k0 += 8) {  // the same bound for every lane: the sums shuffle
-        const int k = k0 + hq, j = k - L;
-        const bool seen = k < L || (j < n && ((mw[j >> 6] >> (j & 63)) & 1));
-        const half* kp = k < L ? Kb + (size_t)k * stride : Tk + (size_t)j * KV * kTaDim;
-        const half* vp = k < L ? Vb + (size_t)k * stride : Tv + (size_t)j * KV * kTaDim;
-        float kf[8], vf[8], d = 0.f;
-        if (seen) {
-            unpack8(*reinterpret_cast<const uint4*>(kp), kf);
-            unpack8(*reinterpret_cast<const uint4*>(vp), vf);
+    for (int m = 16; m >= 1; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+    return t;
+}
+
+// A position in the row of all tiles, advanced unit by unit.
+struct TaCursor {
+    int b, n, L, tiles, units;  // sequence and its shape
+    int unit;                   // within the sequence: kv head * M tiles + M tile
+    int tile;                   // next tile of the unit
+    long long left;             // tiles left of this CTA's range
+    LLMDIY_DEV int seg() const { return (int)min((long long)(tiles - tile), left); }  // tiles of this unit to do
+    LLMDIY_DEV void next(const TaArgs& a, int done) {  // past `done` tiles of this unit
+        left -= done;
+        tile += done;
+        if (tile < tiles || left <= 0) return;
+        tile = 0;
+        if (++unit < units) return;
+        unit = 0;
+        do {
+            if (++b >= a.B) {  // (not reached while left > 0, unless the lengths change under the kernel)
+                left = 0;
+                return;
+            }
+            ta_shape(a, b, n, L, tiles, units);
+        } while (units == 0);
+    }
+};
+
+LLMDIY_DEV long long ta_range_start(long long total, int w, int W) { return total * w / W; }
+LLMDIY_DEV int ta_ctas(long long total, int W) { return (int)min((long long)W, total); }
+
+// The cursor of CTA w's range [first, end) (a whole warp calls it together).
+LLMDIY_DEV void ta_start(const TaArgs& a, int w, int lane, TaCursor& c) {
+    const long long total = ta_tiles_before(a, a.B, lane);
+    c.left = 0;
+    const int W = ta_ctas(total, a.W);
+    if (w >= W) return;
+    const long long first = ta_range_start(total, w, W);
+    c.left = ta_range_start(total, w + 1, W) - first;
+    // the sequence that holds tile `first`: 32 sequences at a time, inclusive sums
+    long long before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        int n, L, tiles = 0, units = 0;
+        if (b0 + lane < a.B) ta_shape(a, b0 + lane, n, L, tiles, units);
+        const long long own = (long long)tiles * units;
+        long long inc = own;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d = __fmaf_rn(q8[e], kf[e], d);
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += o;
         }
-#pragma unroll
-        for (int mk = 8; mk >= 1; mk >>= 1) d += __shfl_xor_sync(0xffffffffu, d, mk);
-        if (!seen) continue;
-        const float s = d * scale, mx = fmaxf(m, s);
-        if (mx == -INFINITY) continue;
-        const float corr = __expf(m - mx), p = __expf(s - mx);
-        l = l * corr + p;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o8[e] = __fmaf_rn(p, vf[e], o8[e] * corr);
-        m = mx;
+        const unsigned hit = __ballot_sync(0xffffffffu, before + inc > first);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            c.b = b0 + l;
+            const long long rest = first - before - __shfl_sync(0xffffffffu, inc - own, l);
+            ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
+            c.unit = (int)(rest / c.tiles);
+            c.tile = (int)(rest - (long long)c.unit * c.tiles);
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, inc, 31);
     }
-    combine_halfwarps(m, l, o8);
-    if (lane < 16)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) so[warp][dl + e] = o8[e];
-    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+    c.left = 0;  // (not reached: the tile lies in some sequence)
+}
+
+LLMDIY_DEV void tma_load_3d(void* dst, const void* tmap, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+LLMDIY_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+LLMDIY_DEV uint32_t ta_pack(float lo, float hi) {
+    const half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+LLMDIY_DEV float ta_ex2(float x) {  // 2^x (2^-inf = 0)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kTaScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
+
+template <int QR, int KS, int VS>
+__global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
+    tree_attn_k(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap ttk,
+                const __grid_constant__ CUtensorMap ttv, const __grid_constant__ TaArgs a, int* err) {
+    using Smem = TaSmem<QR, KS, VS>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = a.H / a.KV;
+    if (tid == 0) {
+        mbar_init(&s.q_full, 1);
+        mbar_init(&s.q_empty, 1);
+        for (int i = 0; i < KS; ++i) {
+            mbar_init(&s.k_full[i], 1);
+            mbar_init(&s.k_empty[i], 1);
+        }
+        for (int i = 0; i < VS; ++i) {
+            mbar_init(&s.v_full[i], 1);
+            mbar_init(&s.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.s_full[i], 1);
+            mbar_init(&s.p_full[i], 4);
+            mbar_init(&s.o_done[i], 1);
+        }
+        mbar_init(&s.drain, 1);
+        s.fail = 0;
+        mbar_fence_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(&s.tmem_base, kTaCols);
+        tmem_relinquish();
+    }
+    TaCursor c;
+    ta_start(a, blockIdx.x, lane, c);
+    tc_fence_before();
     __syncthreads();
-    float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), Ls = 0.f, acc = 0.f;
-    for (int w = 0; w < 4; ++w) {
-        if (sm[w] == -INFINITY) continue;
-        const float f = __expf(sm[w] - M);
-        Ls += sl[w] * f;
-        acc = __fmaf_rn(f, so[w][tid], acc);
+    tc_fence_after();
+    pdl_launch_dependents();  // the merge may be scheduled; it waits for this grid before it reads a partial
+    const uint32_t tmem = s.tmem_base, tO = tmem + 128;  // S(j) lives at tmem + 64 * (j & 1)
+    const bool work = c.left > 0;
+
+    if (warp == 4 && work) {
+        if (lane == 0) {
+            // ---------------- producer: tile j's K into stage j % KS, its V into stage j % VS
+            const uint64_t pol = l2_policy_evict_first();
+            uint32_t kn = 0, vn = 0, unit_no = 0;  // K tiles, V tiles and units' queries issued
+            bool ok = true;
+            auto load = [&](half (*dst)[kTaKeys * 64], const CUtensorMap* cache, const CUtensorMap* tree, int kvh, int t,
+                            int tc, uint64_t* bar) {
+                mbar_arrive_expect_tx(bar, kTaTileBytes);
+                if (t < tc) {
+                    const int y = ta_slot(a, c.b) * a.slot_rows + t * kTaKeys;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (a.evict_first) tma_load_2d_hint(dst[x], cache, kvh * kTaDim + 64 * x, y, bar, pol);
+                        else tma_load_2d(dst[x], cache, kvh * kTaDim + 64 * x, y, bar);
+                    }
+                } else {
+                    const int y = c.b * a.N + (t - tc) * kTaKeys;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) tma_load_2d(dst[x], tree, kvh * kTaDim + 64 * x, y, bar);
+                }
+            };
+            while (ok && c.left > 0) {
+                const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+                const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg();
+                auto load_q = [&]() -> bool {
+                    if (unit_no && !mbar_wait(&s.q_empty, (unit_no - 1) & 1, &s.fail)) return false;
+                    mbar_arrive_expect_tx(&s.q_full, (uint32_t)(a.rows * kTaDim * 2));
+                    tma_load_3d(s.q[0], &tq, 0, kvh * G, c.b * a.N + m0, &s.q_full);
+                    tma_load_3d(s.q[1], &tq, 64, kvh * G, c.b * a.N + m0, &s.q_full);
+                    ++unit_no;
+                    return true;
+                };
+                const bool first_unit = unit_no == 0;
+                if (first_unit) (void)load_q();
+                for (int t = c.tile; t < c.tile + cnt; ++t) {
+                    if (kn >= KS && !mbar_wait(&s.k_empty[kn % KS], (kn / KS - 1) & 1, &s.fail)) { ok = false; break; }
+                    load(s.k[kn % KS], &tk, &ttk, kvh, t, tc, &s.k_full[kn % KS]);
+                    ++kn;
+                    if (vn >= VS && !mbar_wait(&s.v_empty[vn % VS], (vn / VS - 1) & 1, &s.fail)) { ok = false; break; }
+                    load(s.v[vn % VS], &tv, &ttv, kvh, t, tc, &s.v_full[vn % VS]);
+                    ++vn;
+                    // a later unit's queries take the place of the last one's when its S are done: its first
+                    // tile is under way by then
+                    if (t == c.tile && !first_unit && !load_q()) { ok = false; break; }
+                }
+                if (ok) c.next(a, cnt);
+            }
+            // the last copies land in this CTA's shared memory: they have before it exits, whatever happens
+            for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i) (void)mbar_wait(&s.k_full[i % KS], (i / KS) & 1);
+            for (uint32_t i = vn > VS ? vn - VS : 0; i < vn; ++i) (void)mbar_wait(&s.v_full[i % VS], (i / VS) & 1);
+            if (unit_no) (void)mbar_wait(&s.q_full, (unit_no - 1) & 1);
+            if (!ok) s.fail = 1;
+        }
+        __syncwarp();
+    } else if (warp == 5 && work) {
+        if (lane == 0) {
+            // ---------------- MMA issuer
+            constexpr uint32_t idS = umma_idesc_f16_f32(kTaRows, kTaKeys, false);
+            constexpr uint32_t idO = umma_idesc_f16_f32(kTaRows, kTaDim, true);
+            const uint32_t qa = smem_u32(s.q[0]);
+            const uint32_t total = (uint32_t)c.left;
+            uint32_t unit_no = 0;
+            int in_unit = c.seg();  // tiles of the current unit whose S is not issued yet
+            // S(j) = Q K(j)^T into TMEM buffer j & 1, then release K(j)'s stage (and Q after a unit's last tile)
+            auto qk = [&](uint32_t j, bool first) -> bool {
+                if (first && !mbar_wait(&s.q_full, unit_no++ & 1, &s.fail)) return false;
+                if (!mbar_wait(&s.k_full[j % KS], (j / KS) & 1, &s.fail)) return false;
+                tc_fence_after();
+                const uint32_t kb = smem_u32(s.k[j % KS][0]);
+#pragma unroll
+                for (int kk = 0; kk < kTaDim / 16; ++kk)
+                    umma_f16(tmem + 64u * (j & 1), umma_desc_sw128(qa + (kk >> 2) * (QR * 128) + 32 * (kk & 3)),
+                             umma_desc_sw128(kb + (kk >> 2) * 8192 + 32 * (kk & 3)), idS, kk != 0 ? 1u : 0u);
+                umma_commit(&s.s_full[j & 1]);
+                umma_commit(&s.k_empty[j % KS]);
+                return true;
+            };
+            auto pv = [&](uint32_t j, bool first) -> bool {  // O (+)= P(j) V(j), then release V(j)'s stage
+                if (!mbar_wait(&s.p_full[j & 1], (j >> 1) & 1, &s.fail)) return false;
+                if (!mbar_wait(&s.v_full[j % VS], (j / VS) & 1, &s.fail)) return false;
+                tc_fence_after();
+                const uint32_t pa = tmem + 64u * (j & 1), vb = smem_u32(s.v[j % VS][0]);
+#pragma unroll
+                for (int kk = 0; kk < kTaKeys / 16; ++kk)
+                    umma_f16_tmem_a(tO, pa + 8 * kk, umma_desc_sw128_mn(vb + 2048 * kk, 8192, 1024), idO,
+                                    first && kk == 0 ? 0u : 1u);
+                umma_commit(&s.v_empty[j % VS]);
+                umma_commit(&s.o_done[j & 1]);  // last: the rows end the CTA when they have seen it
+                return true;
+            };
+            bool first_pv = true;
+            auto advance = [&]() {  // one more S issued; true: the next tile begins a unit
+                if (--in_unit) return false;
+                umma_commit(&s.q_empty);
+                c.next(a, c.seg());
+                in_unit = c.left > 0 ? c.seg() : 0;
+                return true;
+            };
+            bool ok = qk(0, true);
+            bool next_first = ok && advance();
+            for (uint32_t j = 0; ok && j < total; ++j) {
+                const bool cut = next_first;  // tile j + 1 begins a unit
+                if (j + 1 < total) {
+                    // S(j+1) takes the buffer that held P(j-1): PV(j-1) must be complete
+                    if (j >= 1 && !mbar_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, &s.fail)) { ok = false; break; }
+                    if (!cut) {
+                        if (!qk(j + 1, false)) { ok = false; break; }
+                        next_first = advance();
+                    }
+                }
+                if (!pv(j, first_pv)) { ok = false; break; }
+                first_pv = cut;
+                if (cut && j + 1 < total) {
+                    // a new unit's Q arrives after the old unit's last S: issue PV first, then wait for Q
+                    if (!qk(j + 1, true)) { ok = false; break; }
+                    next_first = advance();
+                }
+            }
+            if (!ok) {
+                s.fail = 1;
+                umma_commit(&s.drain);  // every MMA issued so far completes before the CTA exits
+                (void)mbar_wait(&s.drain, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4 && work) {
+        // ---------------- rows
+        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        const int r = tid, words = (a.N + 63) / 64;
+        uint32_t j = 0;
+        int slot_no = 0, tree_units = 0;
+        bool ok = true;
+        auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {  // one answer for the warp
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, &s.fail));
+        };
+        while (ok && c.left > 0) {
+            const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+            const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(), t0 = c.tile;
+            const int node = m0 + r / G, g = r - (r / G) * G;
+            const bool live = r < a.rows && node < c.n;
+            const bool warp_live = warp * 32 < min(a.rows, (c.n - m0) * G);
+            const uint64_t* mrow = a.mask + ((size_t)c.b * a.N + (live ? node : 0)) * words;
+            const int tt0 = max(t0 - tc, 0);  // first tree tile of this segment, if any
+            uint64_t word = live && t0 + cnt > tc ? mrow[tt0] : 0;
+            float m = -INFINITY, l = 0.f;
+            for (int t = t0; t < t0 + cnt; ++t, ++j) {
+                const bool tree = t >= tc;
+                const int tt = t - tc;
+                const int nv = tree ? min(kTaKeys, c.n - tt * kTaKeys) : min(kTaKeys, c.L - t * kTaKeys);
+                uint64_t seen = nv == 64 ? ~0ull : (1ull << nv) - 1;
+                if (tree) {
+                    seen &= word;
+                    if (live && t + 1 < t0 + cnt) word = mrow[tt + 1];
+                }
+                if (tree || nv < kTaKeys) {
+                    // V rows that must not enter the product: past the end, or (tree) not finite
+                    if (!warp_wait(&s.v_full[j % VS], (j / VS) & 1)) { ok = false; break; }
+                    // (this warp's 16 rows; a row is two runs of eight 16-byte pieces)
+                    uint32_t bad16 = 0;
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int row = warp * 16 + it * 2 + (lane >> 4);
+                        uint4* piece = reinterpret_cast<uint4*>(s.v[j % VS][(lane >> 3) & 1]) + row * 8 + (lane & 7);
+                        const uint4 y = *piece;
+                        auto odd = [](uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; };
+                        const bool out = row >= nv;
+                        const unsigned hit = __ballot_sync(
+                            0xffffffffu, tree && !out && (odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w)));
+                        const bool mine = hit & (lane < 16 ? 0xffffu : 0xffff0000u);
+                        if (out || mine) *piece = make_uint4(0u, 0u, 0u, 0u);
+                        bad16 |= (uint32_t)((hit & 0xffffu) != 0) << (2 * it) | (uint32_t)((hit >> 16) != 0) << (2 * it + 1);
+                    }
+                    if (tree && lane == 0) s.bad[tree_units & 1][tt][warp] = (uint16_t)bad16;
+                    fence_async_smem();
+                }
+                if (!warp_wait(&s.s_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
+                if (warp_live) {
+                    tc_fence_after();
+                    float x[kTaKeys];
+#pragma unroll
+                    for (int q = 0; q < kTaKeys; q += 16)
+                        tmem_ld16(tmem + 64u * (j & 1) + lane_off + q, reinterpret_cast<uint32_t*>(x + q));
+                    tmem_ld_wait();
+                    if (tree || nv < kTaKeys) {
+                        const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+#pragma unroll
+                        for (int q = 0; q < kTaKeys; ++q)
+                            x[q] = ((q < 32 ? lo : hi) & (1u << (q & 31))) ? x[q] : -INFINITY;
+                    }
+                    float mx[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx[e] = x[e];
+#pragma unroll
+                    for (int q = 8; q < kTaKeys; ++q) mx[q & 7] = fmaxf(mx[q & 7], x[q]);
+                    const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                            fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * kTaScaleLog2;
+                    const bool grow = live && top > m + (t == t0 ? 0.f : 8.f);  // (a NaN maximum leaves m)
+                    if (t != t0 && __any_sync(0xffffffffu, grow)) {
+                        // rescale O, complete through PV(j-1) (the whole warp: TMEM moves 32 rows at a time)
+                        if (!warp_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) { ok = false; break; }
+                        tc_fence_after();
+                        const float f = grow ? exp2f(m - top) : 1.f;  // m = -inf: 0
+#pragma unroll 1
+                        for (int q = 0; q < kTaDim; q += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tO + lane_off + q, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(tO + lane_off + q, o);
+                        }
+                        tmem_st_wait();
+                        l *= f;
+                    }
+                    if (grow) m = top;
+                    const float nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every p is 2^-inf = 0
+                    float ls[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ls[e] = 0.f;
+                    uint32_t pk[kTaKeys / 2];
+#pragma unroll
+                    for (int q = 0; q < kTaKeys; q += 2) {
+                        const float p0 = ta_ex2(__fmaf_rn(x[q], kTaScaleLog2, nm));
+                        const float p1 = ta_ex2(__fmaf_rn(x[q + 1], kTaScaleLog2, nm));
+                        ls[q & 7] += p0;
+                        ls[(q + 1) & 7] += p1;
+                        pk[q / 2] = ta_pack(p0, p1);
+                    }
+                    l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+#pragma unroll
+                    for (int q = 0; q < kTaKeys / 2; q += 16) tmem_st16(tmem + 64u * (j & 1) + lane_off + q, pk + q);
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.p_full[j & 1]);
+            }
+            if (!ok) break;
+            // ---------------- the unit's (or its part's) output
+            if (!warp_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) { ok = false; break; }
+            tc_fence_after();
+            const bool whole = cnt == c.tiles;
+            const bool any_tree = t0 + cnt > tc;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const size_t at = (size_t)(blockIdx.x * 2 + slot_no) * a.rows + r;
+            half* dst = a.O + ((size_t)c.b * a.N + node) * a.ldo + (kvh * G + g) * kTaDim;
+            float* pdst = a.part + at * kTaDim;
+            if (warp_live) {
+#pragma unroll 1
+                for (int q = 0; q < kTaDim; q += 16) {
+                    uint32_t o[16];
+                    __syncwarp();
+                    tmem_ld16(tO + lane_off + q, o);
+                    tmem_ld_wait();
+                    float v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(o[e]);
+                    if (any_tree && live) {
+                        // tree rows with a non-finite V that this row sees: their p * v, left out of PV
+                        for (int tt = tt0; tt < t0 + cnt - tc; ++tt) {
+                            uint64_t hit = *reinterpret_cast<volatile uint64_t*>(s.bad[tree_units & 1][tt]);
+                            if (!hit) continue;
+                            hit &= mrow[tt];
+                            for (; hit; hit &= hit - 1) {
+                                const int kn = tt * 64 + __ffsll((long long)hit) - 1;
+                                const half* kr = a.TK + (((size_t)c.b * a.N + kn) * a.KV + kvh) * kTaDim;
+                                const half* vr = a.TV + (((size_t)c.b * a.N + kn) * a.KV + kvh) * kTaDim;
+                                const half* qr = a.Q + ((size_t)c.b * a.N + node) * a.ldq + (kvh * G + g) * kTaDim;
+                                float d = 0.f;
+                                for (int e = 0; e < kTaDim; ++e) d = __fmaf_rn(h2f(qr[e]), h2f(kr[e]), d);
+                                const float p = ta_ex2(__fmaf_rn(d, kTaScaleLog2, m == -INFINITY ? 0.f : -m));
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v[e] = __fmaf_rn(p, h2f(vr[q + e]), v[e]);
+                            }
+                        }
+                    }
+                    if (!live) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] *= inv;
+                        *reinterpret_cast<uint4*>(dst + q) = pack8(v);
+                        *reinterpret_cast<uint4*>(dst + q + 8) = pack8(v + 8);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<float4*>(pdst + q + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
+                }
+                if (live && !whole)
+                    *reinterpret_cast<float2*>(a.part + (size_t)a.W * 2 * a.rows * kTaDim + at * 2) = make_float2(m, l);
+            }
+            tc_fence_before();  // O has been read: the next unit's first PV may overwrite it
+            if (any_tree) ++tree_units;
+            slot_no = 1;
+            c.next(a, cnt);
+        }
+        if (!ok) s.fail = 1;
     }
-    O[row * ldo + h * kTaDim + tid] = f2h(Ls == 0.f ? 0.f : acc / Ls);
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && s.fail) atomicExch(err, 1);
+    if (warp == 0) tmem_dealloc(tmem, kTaCols);
+}
+
+// Joins the partials of the units that were cut: one warp per output row (sequence, node, head), which
+// finds the CTAs that share its unit from the same arithmetic.  Lane s weighs partial s, then
+// each lane sums 4 dims over the partials in order.
+constexpr int kTaMergeWarps = 8;
+
+__global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_constant__ TaArgs a) {
+    const int lane = threadIdx.x & 31, h = blockIdx.x * kTaMergeWarps + (threadIdx.x >> 5);
+    const int b = blockIdx.z, i = blockIdx.y;
+    int n, L, tiles, units;
+    ta_shape(a, b, n, L, tiles, units);
+    const long long total = ta_tiles_before(a, a.B, lane), before = ta_tiles_before(a, b, lane);
+    // every thread waits for the attention kernel, also where there is nothing to join: this grid
+    // must not be over before that one is
+    pdl_wait();
+    if (h >= a.H || i >= n) return;
+    const int G = a.H / a.KV, mt = units / a.KV, kvh = h / G, r = (i % a.npt) * G + h % G;
+    const int W = ta_ctas(total, a.W);
+    const long long f0 = before + (long long)(kvh * mt + i / a.npt) * tiles;
+    const int w0 = (int)(((f0 + 1) * W - 1) / total), w1 = (int)(((f0 + tiles) * W - 1) / total);
+    if (w0 == w1) return;  // whole: already written
+    // the first CTA's part of this unit is its first segment only when its range starts here
+    const int first = w0 * 2 + (ta_range_start(total, w0, W) == f0 ? 0 : 1);
+    const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.W * 2 * a.rows * kTaDim);
+    float M = -INFINITY;
+    for (int w = w0 + lane; w <= w1; w += 32)
+        M = fmaxf(M, __ldcg(ml + (size_t)(w == w0 ? first : w * 2) * a.rows + r).x);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float Ls = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = w0; c0 <= w1; c0 += 32) {
+        float f = 0.f, lw = 0.f;
+        if (c0 + lane <= w1) {
+            const int w = c0 + lane;
+            const float2 y = __ldcg(ml + (size_t)(w == w0 ? first : w * 2) * a.rows + r);
+            f = y.x == -INFINITY ? 0.f : exp2f(y.x - M);
+            lw = y.x == -INFINITY ? y.y : y.y * f;  // nothing seen: l = 0 (or NaN, which stays)
+            if (y.y != y.y) f = 1.f;
+        }
+        Ls += lw;
+        const int cnt = min(32, w1 - c0 + 1);
+#pragma unroll 4
+        for (int k = 0; k < cnt; ++k) {
+            const int w = c0 + k;
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(
+                a.part + ((size_t)(w == w0 ? first : w * 2) * a.rows + r) * kTaDim) + lane);
+            acc.x = __fmaf_rn(fk, y.x, acc.x);
+            acc.y = __fmaf_rn(fk, y.y, acc.y);
+            acc.z = __fmaf_rn(fk, y.z, acc.z);
+            acc.w = __fmaf_rn(fk, y.w, acc.w);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+    const half2 y0 = __floats2half2_rn(acc.x * inv, acc.y * inv), y1 = __floats2half2_rn(acc.z * inv, acc.w * inv);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t*>(&y0);
+    u.y = *reinterpret_cast<const uint32_t*>(&y1);
+    *reinterpret_cast<uint2*>(a.O + ((size_t)b * a.N + i) * a.ldo + h * kTaDim + lane * 4) = u;
+}
+
+// ------------------------------------------------------------------ host
+int ta_sms() {
+    static int sms[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!sms[dev]) {
+        int n = 0;
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        sms[dev] = n > 0 ? n : 148;
+    }
+    return sms[dev];
+}
+
+struct TaPlan {
+    int G, npt, rows, W;
+    bool ok;
+    size_t floats;  // of the partials
+};
+
+// The grid and the partials' size: never smaller for a larger B, N or max_len (same heads), so a
+// workspace sized for the largest call serves the others.
+TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
+    TaPlan p = {};
+    p.ok = B > 0 && B <= 65535 && N > 0 && N <= LLMDIY_TREE_MAX_NODES && KV > 0 && H >= KV && H <= 1024 && H % KV == 0 &&
+           H / KV <= kTaMaxGroup && max_len >= 0;
+    if (!p.ok) return p;
+    p.G = H / KV;
+    p.npt = std::min(kTaRows / p.G, N);
+    p.rows = p.G * p.npt;
+    const long long tiles = ((long long)max_len + kTaKeys - 1) / kTaKeys + (N + kTaKeys - 1) / kTaKeys;
+    const long long units = (long long)B * KV * ((N + p.npt - 1) / p.npt);
+    p.W = (int)std::min<long long>(kTaCtasPerSm * ta_sms(), units * tiles);
+    p.floats = (size_t)p.W * 2 * p.rows * (kTaDim + 2);
+    return p;
+}
+
+// Query rows as [B * N][H][128] (pitch ldq): box of 64 dims x G heads x npt nodes, 128-byte swizzle.
+bool make_query_map(CUtensorMap* m, const void* base, int nodes, int H, int ldq, int G, int npt) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<Encode>(p);
+    });
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)kTaDim, (cuuint64_t)H, (cuuint64_t)nodes};
+    cuuint64_t strides[2] = {(cuuint64_t)kTaDim * 2, (cuuint64_t)ldq * 2};
+    cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)npt};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr size_t kTaCtl = 4;  // floats before the partials: word 0 is the error word
+
+template <int QR, int KS, int VS>
+int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, cudaStream_t st) {
+    auto kern = tree_attn_k<QR, KS, VS>;
+    constexpr int bytes = (int)sizeof(TaSmem<QR, KS, VS>);
+    static_assert(bytes <= 115712, "two CTAs share an SM");
+    static std::atomic<bool> set[64];  // per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !set[dev])) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) set[dev] = true;
+    }
+    if (e != cudaSuccess) return (int)e;
+    kern<<<a.W, kTaThreads, bytes, st>>>(m[0], m[1], m[2], m[3], m[4], a, err);
+    return (int)cudaGetLastError();
 }
 
 }  // namespace
@@ -80,10 +684,8 @@ __global__ void __launch_bounds__(kTaThreads)
 extern "C" {
 
 size_t llmdiy_tree_attn_work_bytes(int B, int N, int num_heads, int num_kv_heads, int max_len) {
-    if (B <= 0 || N <= 0 || N > LLMDIY_TREE_MAX_NODES || num_kv_heads <= 0 || num_heads <= 0 ||
-        num_heads % num_kv_heads || max_len < 0)
-        return 0;
-    return 16;
+    const TaPlan p = ta_plan(B, N, num_heads, num_kv_heads, max_len);
+    return p.ok ? (kTaCtl + p.floats) * sizeof(float) : 0;
 }
 
 int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16_t* V, int stride, int slot_rows,
@@ -91,17 +693,57 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
                      const uint16_t* TV, const uint64_t* mask, const int* tree_len, int B, int N, int num_heads,
                      int num_kv_heads, uint16_t* O, int ldo, float* work, size_t work_bytes, void* stream) {
     auto a16 = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    const size_t need = llmdiy_tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len);
-    if (!need || B > 65535 || !a16(Q) || !a16(K) || !a16(V) || !a16(TK) || !a16(TV) || !a16(O) || !len || !mask ||
-        num_heads > 1024 || ldq < num_heads * kTaDim || (ldq & 7) || ldo < num_heads * kTaDim || (ldo & 7) ||
-        stride < num_kv_heads * kTaDim || (stride & 7) || slot_rows <= 0 || num_slots <= 0 || max_len > slot_rows ||
-        (long long)num_slots * slot_rows > 0x7fffffffLL || !a16(work) || work_bytes < need)
+    const TaPlan p = ta_plan(B, N, num_heads, num_kv_heads, max_len);
+    if (!p.ok || !a16(Q) || !a16(K) || !a16(V) || !a16(TK) || !a16(TV) || !a16(O) || !len || !mask ||
+        (reinterpret_cast<uintptr_t>(mask) & 7) || ldq < num_heads * kTaDim || (ldq & 7) || ldo < num_heads * kTaDim ||
+        (ldo & 7) || stride < num_kv_heads * kTaDim || (stride & 7) || slot_rows <= 0 || num_slots <= 0 ||
+        max_len > slot_rows || (long long)num_slots * slot_rows > 0x7fffffffLL || !a16(work) ||
+        work_bytes < (kTaCtl + p.floats) * sizeof(float))
         return (int)cudaErrorInvalidValue;
-    tree_attn_k<<<dim3(num_heads, N, B), kTaThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-        reinterpret_cast<const half*>(Q), ldq, reinterpret_cast<const half*>(K), reinterpret_cast<const half*>(V), stride,
-        slot_rows, num_slots, slot, len, max_len, reinterpret_cast<const half*>(TK), reinterpret_cast<const half*>(TV),
-        mask, tree_len, N, num_heads, num_kv_heads, reinterpret_cast<half*>(O), ldo);
-    return (int)cudaGetLastError();
+    CUtensorMap m[5];
+    const int cols = num_kv_heads * kTaDim;
+    if (!make_query_map(&m[0], Q, B * N, num_heads, ldq, p.G, p.npt) ||
+        !make_kmajor_map(&m[1], K, num_slots * slot_rows, cols, stride, kTaKeys) ||
+        !make_kmajor_map(&m[2], V, num_slots * slot_rows, cols, stride, kTaKeys) ||
+        !make_kmajor_map(&m[3], TK, B * N, cols, cols, kTaKeys) || !make_kmajor_map(&m[4], TV, B * N, cols, cols, kTaKeys))
+        return (int)cudaErrorInvalidValue;
+    TaArgs a = {};
+    a.slot = slot;
+    a.len = len;
+    a.tree_len = tree_len;
+    a.mask = mask;
+    a.Q = reinterpret_cast<const half*>(Q);
+    a.TK = reinterpret_cast<const half*>(TK);
+    a.TV = reinterpret_cast<const half*>(TV);
+    a.O = reinterpret_cast<half*>(O);
+    a.part = work + kTaCtl;
+    a.B = B;
+    a.N = N;
+    a.H = num_heads;
+    a.KV = num_kv_heads;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.slot_rows = slot_rows;
+    a.num_slots = num_slots;
+    a.max_len = max_len;
+    a.rows = p.rows;
+    a.npt = p.npt;
+    a.W = p.W;
+    a.evict_first = p.npt >= N;  // one M tile: every K/V row is read once
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    int* err = reinterpret_cast<int*>(work);
+    int rc = p.rows <= 64 ? ta_launch<64, 3, 3>(m, a, err, st) : ta_launch<128, 3, 2>(m, a, err, st);
+    if (rc) return rc;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((num_heads + kTaMergeWarps - 1) / kTaMergeWarps, N, B);
+    lc.blockDim = dim3(kTaMergeWarps * 32);
+    lc.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&lc, tree_merge_k, a);
 }
 
 int llmdiy_tree_attn_status(const float* work) {
@@ -110,7 +752,7 @@ int llmdiy_tree_attn_status(const float* work) {
     int* word = reinterpret_cast<int*>(const_cast<float*>(work));
     cudaError_t e = cudaMemcpy(&h, word, sizeof(int), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return (int)e;
-    if (h) cudaMemset(word, 0, sizeof(int));
+    if (h) cudaMemset(word, 0, sizeof(int));  // the kernels only ever set it
     return h ? -5 : 0;
 }
 
