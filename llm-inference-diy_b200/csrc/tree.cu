@@ -148,8 +148,13 @@ __global__ void __launch_bounds__(kVerThreads)
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n = nodes_of(tree_len, b, N);
     const size_t row0 = (size_t)b * N;
+    int par = -1, tok = -1;
+    if (tid > 0 && tid < N) {  // (in flight together with the tree's size)
+        par = parent[row0 + tid];
+        tok = token[row0 + tid];
+    }
+    const int n = nodes_of(tree_len, b, N);
     if (rank == 0)
         for (int i = tid; i < N; i += kVerThreads) path[row0 + i] = -1;
     if (n == 0) {
@@ -157,8 +162,6 @@ __global__ void __launch_bounds__(kVerThreads)
         return;  // the whole cluster
     }
     if (tid < n) {
-        const int par = tid ? parent[row0 + tid] : -1;
-        const int tok = tid ? token[row0 + tid] : 0;
         const bool ok = par >= 0 && par < tid && tok >= 0 && tok < V;
         s.parent[tid] = ok ? par : -1;
         s.token[tid] = tok;
@@ -199,6 +202,7 @@ __global__ void __launch_bounds__(kVerThreads)
     // reaches after it has read round r's.
     auto totals = [&]() -> const double* {
         double t = 0.0;
+#pragma unroll 4
         for (int u = u0; u < u1; ++u) {
             double w[4];
             weights(u, w);
@@ -403,7 +407,7 @@ int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd
         !parent || !uniform || !path || !accepted || !next || !aligned4(target) || !aligned4(draft))
         return (int)cudaErrorInvalidValue;
     const int vec = aligned16(target) && ldt % 4 == 0 && (!draft || (aligned16(draft) && ldd % 4 == 0));
-    constexpr int C = 1;
+    const int C = 8;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(B * C);
     lc.blockDim = dim3(kVerThreads);
