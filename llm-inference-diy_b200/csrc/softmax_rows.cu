@@ -1,16 +1,19 @@
 // softmax_rows.cu — probabilities of rows of fp16 logits, with a temperature per row
 // (include/llmdiy_tree.h).  No counterpart in the reference, whose engine takes the argmax only.
 //
-// One pass over memory: a cluster of C CTAs holds a row in registers (as fp16), slice c of it in CTA c.
-// Each CTA finds its slice's maximum and its sum of exponentials relative to that maximum; one
-// exchange of the C pairs through distributed shared memory gives the row's maximum M and sum
-// S = sum_c s_c 2^{(m_c - M) k}, k = log2(e) / t, and every thread writes 2^{(x - M) k} / S from its
-// registers.  x - M is exact in fp32 for fp16 x (but for far smaller x, whose share is 0), so the exponent carries
-// two roundings (k and the product).  Reading 2 and writing 4 bytes an entry is the bound: the exponentials
-// are taken twice (the second time for M) rather than kept, which would double the registers.
+// One pass over memory, by persistent clusters of C CTAs: cluster c takes rows c, c + clusters, ..., slice k of
+// a row in CTA k.  Bulk copies bring the next two rows' slices into shared memory while a row is
+// worked on; its entries go to registers, which frees their stage for the copy after next.  Each CTA finds
+// its slice's maximum m_c and its sum s_c of exponentials relative to it (kept in registers as
+// fp32); one exchange of the C pairs through distributed shared memory (asynchronous stores that complete on the
+// receiver's mbarrier: a cluster barrier would also wait for the last row's output to be written) gives
+// the row's maximum M and sum S = sum_c s_c 2^{(m_c - M) k}, k = log2(e) / t, and every thread writes its share times
+// 2^{(m_c - M) k} / S.  x - m is exact in fp32 for fp16 x (but for far smaller x, whose share is 0), so the
+// exponent carries two roundings (k and the product).  Reading 2 and writing 4 bytes an entry is the bound.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "llmdiy_tree.h"
@@ -19,10 +22,14 @@ using namespace llmdiy;
 
 namespace {
 
-constexpr int kSmThreads = 256;
-constexpr int kSmVecs = 10;                              // eight entries each, per thread
-constexpr int kSmSlice = kSmThreads * kSmVecs * 8;       // entries a CTA holds
+constexpr int kSmThreads = 512;
+constexpr int kSmPairs = 20;                                  // pairs of entries a thread holds
+constexpr int kSmSlice = kSmThreads * kSmPairs * 2 - 8;       // entries a CTA holds (pairs may start one entry early)
+constexpr int kSmStages = 2;
+// A stage: eight entries before the slice's first granule, the granules, and room for every thread's pairs
+constexpr int kSmStageBytes = (16 + (kSmThreads * kSmPairs * 2 + 16) * 2 + 127) / 128 * 128;
 constexpr int kSmMaxCluster = 8;
+constexpr int kSmCtasPerSm = 2;
 
 LLMDIY_DEV float sm_ex2(float x) {  // 2^x (2^-inf = 0)
     float y;
@@ -30,139 +37,199 @@ LLMDIY_DEV float sm_ex2(float x) {  // 2^x (2^-inf = 0)
     return y;
 }
 LLMDIY_DEV uint32_t sm_pair(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
+// Eight bytes into the shared memory of CTA `rank` of the cluster, counted by the mbarrier there.
+LLMDIY_DEV void sm_send(float2* dst, uint64_t* bar, uint32_t rank, float a, float b) {
+    uint32_t d, m;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(dst)), "r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(smem_u32(bar)), "r"(rank));
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(d),
+                 "f"(a), "f"(b), "r"(m)
+                 : "memory");
+}
 LLMDIY_DEV float2 sm_floats(uint32_t w) { return __half22float2(*reinterpret_cast<const half2*>(&w)); }
 
-// VEC: rows of logits and probabilities are 16-byte aligned; a thread's entries are runs of eight (16-byte
-// loads, two 16-byte stores).  Otherwise entry e of vector i is at (8 i + e) * threads + thread of
-// the slice, so that a warp's 2-byte loads and 4-byte stores are consecutive.
-template <bool VEC>
-__global__ void __launch_bounds__(kSmThreads, 3)
-    softmax_rows_k(const half* __restrict__ logits, int ldl, const float* __restrict__ temp, int V, int slice,
+// The 16-byte granules around entries [v0, v0 + n) of a row, cut at the ends of the whole buffer
+// [first, last): what a bulk copy brings.  `lead`: where entry v0 lies in a stage, in entries.
+struct SmWindow {
+    uintptr_t from, to;
+    int lead;
+};
+LLMDIY_DEV SmWindow sm_window(const uint16_t* x, int n, uintptr_t first, uintptr_t last) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = a + 2 * (uintptr_t)n;
+    SmWindow w;
+    w.lead = (int)(a & 15) / 2;
+    w.from = a & ~(uintptr_t)15;
+    w.to = (b + 15) & ~(uintptr_t)15;
+    if (w.from < first) w.from += 16;
+    if (w.to > last) w.to -= 16;
+    if (w.to < w.from) w.to = w.from;
+    return w;
+}
+
+__global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
+    softmax_rows_k(const half* __restrict__ logits, int ldl, const float* __restrict__ temp, int R, int V, int slice,
                    float* __restrict__ probs, int ldp) {
     namespace cg = cooperative_groups;
-    constexpr uint32_t kNone = 0xFC00FC00u;  // a pair of -inf
+    extern __shared__ __align__(128) uint8_t stage[];  // [kSmStages][kSmStageBytes]
     __shared__ float red_m[kSmThreads / 32], red_s[kSmThreads / 32];
-    __shared__ float2 part[kSmMaxCluster];
+    __shared__ float2 part[2][kSmMaxCluster];  // (m_c, s_c) of the cluster's CTAs: odd and even rows
+    __shared__ uint64_t full[kSmStages], got[2];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const size_t r = blockIdx.x / C;
-    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // "this CTA runs"
-    const int v0 = min(V, rank * slice), n = min(V, v0 + slice) - v0;  // this CTA's entries
-    const uint16_t* x = reinterpret_cast<const uint16_t*>(logits) + r * ldl + v0;
-    float* y = probs + r * ldp + v0;
-    const float t = temp ? temp[r] : 1.f;
-    // entries past the registers' kSmSlice (rows of more than 8 x kSmSlice entries) are read again each time
-    const int held = min(n, kSmSlice);
-    uint32_t w[kSmVecs][4];
-#pragma unroll
-    for (int i = 0; i < kSmVecs; ++i) {
-        if (VEC) {
-            const int at = (i * kSmThreads + tid) * 8;
-            if (at + 8 <= held) {
-                const uint4 u = ld_stream_u4(x + at);
-                w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[i][e] = sm_pair(at + 2 * e < held ? x[at + 2 * e] : 0xFC00, at + 2 * e + 1 < held ? x[at + 2 * e + 1] : 0xFC00);
-            }
-        } else {
-            if (i * 8 * kSmThreads >= held) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[i][e] = kNone;
-                continue;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int a0 = (i * 8 + 2 * e) * kSmThreads + tid, a1 = a0 + kSmThreads;
-                w[i][e] = sm_pair(a0 < held ? __ldg(x + a0) : 0xFC00, a1 < held ? __ldg(x + a1) : 0xFC00);
-            }
-        }
-    }
-    // maximum of the slice (NaN is passed over here; it reaches the sum)
-    half2 h = __half2half2(__ushort_as_half(0xFC00));
-#pragma unroll
-    for (int i = 0; i < kSmVecs; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h = __hmax2(h, *reinterpret_cast<const half2*>(&w[i][e]));
-    float m = fmaxf(__low2float(h), __high2float(h));
-    for (int a = kSmSlice + tid; a < n; a += kSmThreads) m = fmaxf(m, h2f(__ushort_as_half(x[a])));
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) red_m[warp] = m;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSmThreads / 32; ++k) m = fmaxf(m, red_m[k]);
-    // greedy (t <= 0 or NaN): the exponent is 0 at the maximum and -inf elsewhere.  k is bounded so that
-    // 0 * k is 0 at any t > 0.
-    const bool greedy = !(t > 0.f);
-    const float k = greedy ? 0.f : fminf(1.4426950408889634f / t, 1e30f);
-    auto weight = [&](float v, float top) {
-        return greedy ? (v == top ? 1.f : v != v ? v : 0.f) : sm_ex2((v - top) * k);
+    const int r0 = blockIdx.x / C, step = gridDim.x / C;
+    const int v0 = min(V, rank * slice), n = min(V, v0 + slice) - v0;  // this CTA's entries of every row
+    const int held = min(n, kSmSlice);  // those past the registers (rows of more than 8 kSmSlice) are read again
+    const uint16_t* base = reinterpret_cast<const uint16_t*>(logits);
+    const uintptr_t first = reinterpret_cast<uintptr_t>(base), last = first + 2 * ((uintptr_t)(R - 1) * ldl + V);
+    const uint64_t pol = l2_policy_evict_first();
+    auto copy = [&](int r, int st) {  // (one thread)
+        const SmWindow w = sm_window(base + (size_t)r * ldl + v0, held, first, last);
+        const uint32_t bytes = (uint32_t)(w.to - w.from);
+        mbar_arrive_expect_tx(&full[st], bytes);
+        // (a stage begins with the granule that holds the slice's first entry)
+        const uintptr_t g0 = reinterpret_cast<uintptr_t>(base + (size_t)r * ldl + v0) & ~(uintptr_t)15;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // after the plain stores to this stage
+        if (bytes)
+            bulk_g2s(stage + st * kSmStageBytes + 16 + (w.from - g0), reinterpret_cast<const void*>(w.from), bytes, &full[st],
+                     pol);
     };
-    const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: every weight 0
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSmVecs; ++i) {
-        float a = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = sm_floats(w[i][e]);
-            a += weight(f.x, ref) + weight(f.y, ref);
-        }
-        s += a;
+    if (tid == 0) {
+        for (int i = 0; i < kSmStages; ++i) mbar_init(&full[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&got[i], 1);
+        mbar_fence_init();
     }
-    for (int a = kSmSlice + tid; a < n; a += kSmThreads) s += weight(h2f(__ushort_as_half(x[a])), ref);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) red_s[warp] = s;
+    // what no copy writes is -inf for every row
+    for (int i = tid; i < kSmStages * kSmStageBytes / 4; i += kSmThreads) reinterpret_cast<uint32_t*>(stage)[i] = 0xFC00FC00u;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    float M = m, total = 0.f;
-#pragma unroll
-    for (int j = 0; j < kSmThreads / 32; ++j) total += red_s[j];
-    if (C > 1) {
-        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        if (tid < C) *cluster.map_shared_rank(&part[rank], tid) = make_float2(m, total);
-        cluster.sync();
-        for (int c = 0; c < C; ++c) M = fmaxf(M, part[c].x);
-        total = 0.f;
-        for (int c = 0; c < C; ++c) {
-            const float2 q = part[c];
-            const float f = q.x == -INFINITY ? 1.f : q.x == M ? 1.f : greedy ? 0.f : sm_ex2((q.x - M) * k);
-            total += q.y * f;  // (q.x = -inf: a sum of 0, or NaN)
+    if (tid == 0)
+        for (int i = 0; i < kSmStages; ++i)
+            if (r0 + (long long)i * step < R) copy(r0 + i * step, i);
+    if (C > 1) cluster.sync();  // every CTA of the cluster runs: its shared memory may be written
+    int it = 0;
+    for (long long row = r0; row < R; row += step, ++it) {
+        const size_t r = (size_t)row;
+        const uint16_t* x = base + r * ldl + v0;
+        float* y = probs + r * ldp + v0;
+        const int st = it % kSmStages;
+        const float t = temp ? temp[r] : 1.f;
+        const SmWindow win = sm_window(x, held, first, last);
+        uint16_t* sx = reinterpret_cast<uint16_t*>(stage + st * kSmStageBytes + 16) + win.lead;
+        const bool ok = mbar_wait(&full[st], (it / kSmStages) & 1);
+        // The copy's first and last granules hold up to seven entries of the rows beside this slice, and the
+        // last row in this stage may have ended up to fourteen entries further on: -inf for those; and
+        // where the whole buffer ends inside a granule, its entries come from global memory.
+        if (tid < 40) {
+            const uintptr_t xa = reinterpret_cast<uintptr_t>(x);
+            const int c0 = win.from > xa ? (int)(win.from - xa) / 2 : 0;
+            const int c1 = win.to > xa ? min(held, (int)((win.to - xa) / 2)) : 0;
+            const int a = tid < 16 ? tid - 8 : max(held - 8, 8) + tid - 16;  // -8 .. 7 and held - 8 .. held + 15
+            const bool in = a >= 0 && a < held;
+            if (!in) sx[a] = 0xFC00;
+            else if (a < c0 || a >= c1) sx[a] = x[a];
         }
+        __syncthreads();
+        // pairs begin where 8-byte stores of the output do
+        const int odd = (int)(reinterpret_cast<uintptr_t>(y) >> 2) & 1;
+        const uint16_t* mine = sx - odd + 2 * tid;
+        uint32_t w[kSmPairs];
+        if (((win.lead - odd) & 1) == 0) {
+#pragma unroll
+            for (int i = 0; i < kSmPairs; ++i) w[i] = *reinterpret_cast<const uint32_t*>(mine + 2 * i * kSmThreads);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSmPairs; ++i)
+                w[i] = sm_pair(mine[2 * i * kSmThreads], mine[2 * i * kSmThreads + 1]);
+        }
+        half2 h = __half2half2(__ushort_as_half(0xFC00));
+#pragma unroll
+        for (int i = 0; i < kSmPairs; ++i) h = __hmax2(h, *reinterpret_cast<const half2*>(&w[i]));  // (NaN reaches the sum)
+        float m = fmaxf(__low2float(h), __high2float(h));
+        for (int a = kSmSlice + tid; a < n; a += kSmThreads) m = fmaxf(m, h2f(__ushort_as_half(x[a])));
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) red_m[warp] = m;
+        __syncthreads();  // the stage has been read
+        if (tid == 0 && row + (long long)kSmStages * step < R) copy((int)row + kSmStages * step, st);
+        m = red_m[lane & (kSmThreads / 32 - 1)];
+#pragma unroll
+        for (int o = kSmThreads / 64; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // k is bounded so that 0 * k is 0 at any t > 0; greedy (t <= 0 or NaN) takes that bound, where the
+        // smallest difference of two fp16 values gives 2^-inf
+        const float k = t > 0.f ? fminf(1.4426950408889634f / t, 1e30f) : 1e30f;
+        auto weight = [&](float v, float top) { return sm_ex2((v - top) * k); };
+        const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: every weight 0
+        float s = 0.f, ex[2 * kSmPairs];
+#pragma unroll
+        for (int i = 0; i < kSmPairs; ++i) {
+            const float2 f = sm_floats(w[i]);
+            ex[2 * i] = weight(f.x, ref);
+            ex[2 * i + 1] = weight(f.y, ref);
+            s += ex[2 * i] + ex[2 * i + 1];
+        }
+        for (int a = kSmSlice + tid; a < n; a += kSmThreads) s += weight(h2f(__ushort_as_half(x[a])), ref);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) red_s[warp] = s;
+        __syncthreads();
+        float M = m, total = red_s[lane & (kSmThreads / 32 - 1)];
+#pragma unroll
+        for (int o = kSmThreads / 64; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (!ok) total = NAN;  // a copy that never landed shows in its row
+        if (C > 1) {
+            // Two tables take turns: a CTA sends row i + 2's pair only after every CTA's pair of row i + 1 has come,
+            // which each sends after it has read row i's table.
+            float2* tab = part[it & 1];
+            if (tid == 0) mbar_arrive_expect_tx(&got[it & 1], C * 8);
+            if (tid < C) sm_send(&tab[rank], &got[it & 1], tid, m, total);
+            const bool all = mbar_wait(&got[it & 1], (it >> 1) & 1);
+            const float2 q = tab[lane & (C - 1)];
+            M = q.x;
+            for (int o = C / 2; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            total = q.y * (q.x == -INFINITY ? 1.f : weight(q.x, M));  // (q.x = -inf: a sum of 0, or NaN)
+            for (int o = C / 2; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            if (!all) total = NAN;
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const float top = M == -INFINITY ? 0.f : M;
+        const float scale = inv * (m == -INFINITY ? 1.f : weight(m, top));
+        float2* out = reinterpret_cast<float2*>(y - odd) + tid;
+        const int room = held + odd - 2 * tid;  // entries from this thread's first on
+#pragma unroll
+        for (int i = 0; i < kSmPairs; ++i) {
+            const float2 o = make_float2(ex[2 * i] * scale, ex[2 * i + 1] * scale);
+            const bool head = i == 0 && odd && tid == 0;  // the pair that begins one entry early
+            if (2 * i * kSmThreads + 1 < room && !head) out[i * kSmThreads] = o;
+            if (2 * i * kSmThreads + 1 == room && !head) out[i * kSmThreads].x = o.x;
+            if (head && held > 0) y[0] = o.y;
+        }
+        for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    const float top = M == -INFINITY ? 0.f : M;
-#pragma unroll
-    for (int i = 0; i < kSmVecs; ++i) {
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = sm_floats(w[i][e]);
-            o[2 * e] = weight(f.x, top) * inv;
-            o[2 * e + 1] = weight(f.y, top) * inv;
-        }
-        if (VEC) {
-            const int at = (i * kSmThreads + tid) * 8;
-            if (at + 8 <= held) {
-                *reinterpret_cast<float4*>(y + at) = make_float4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<float4*>(y + at + 4) = make_float4(o[4], o[5], o[6], o[7]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (at + e < held) y[at + e] = o[e];
-            }
-        } else if (i * 8 * kSmThreads < held) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int at = (i * 8 + e) * kSmThreads + tid;
-                if (at < held) y[at] = o[e];
-            }
-        }
-    }
-    for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
+}
+
+// Clusters of C CTAs that run at once on the current device.
+int sm_clusters(int C) {
+    static std::atomic<int> known[64][4];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+    const int slot = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
+    int n = known[dev][slot];
+    if (n) return n;
+    cudaFuncSetAttribute(softmax_rows_k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmStages * kSmStageBytes);
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(C);
+    lc.blockDim = dim3(kSmThreads);
+    lc.dynamicSmemBytes = kSmStages * kSmStageBytes;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, softmax_rows_k, &lc) != cudaSuccess || n < 1) n = 1;
+    known[dev][slot] = n;
+    return n;
 }
 
 }  // namespace
@@ -172,16 +239,14 @@ extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float*
     if (!logits || !probs || R <= 0 || V <= 0 || ldl < V || ldp < V || (reinterpret_cast<uintptr_t>(logits) & 1) ||
         (reinterpret_cast<uintptr_t>(probs) & 3))
         return (int)cudaErrorInvalidValue;
-    const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (reinterpret_cast<uintptr_t>(probs) & 15) == 0 &&
-                     ldl % 8 == 0 && ldp % 4 == 0;
     // CTAs per row: enough to hold it, and more while they leave SMs idle and a slice stays above 4096 entries
     int C = 1;
     while (C < kSmMaxCluster && ((V + C - 1) / C > kSmSlice || ((long long)R * C < 74 && V / C >= 8192))) C *= 2;
-    if ((long long)R * C > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     const int slice = (((V + C - 1) / C) + 7) / 8 * 8;
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3(R * C);
+    lc.gridDim = dim3(std::min(R, sm_clusters(C)) * C);
     lc.blockDim = dim3(kSmThreads);
+    lc.dynamicSmemBytes = kSmStages * kSmStageBytes;
     lc.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -189,6 +254,6 @@ extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float*
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     lc.attrs = at;
     lc.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&lc, vec ? softmax_rows_k<true> : softmax_rows_k<false>,
-                                   reinterpret_cast<const half*>(logits), ldl, temp, V, slice, probs, ldp);
+    return (int)cudaLaunchKernelEx(&lc, softmax_rows_k, reinterpret_cast<const half*>(logits), ldl, temp, R, V, slice,
+                                   probs, ldp);
 }

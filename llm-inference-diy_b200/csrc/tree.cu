@@ -88,40 +88,32 @@ __global__ void __launch_bounds__(256)
 constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerMaxCluster = 16;
-
-struct VerRow {
-    const float* p;
-    const float* q;  // NULL: no draft distribution
-    double T;        // weight of entry v: max(0, p - T q)
-    int V;
-    bool vec;  // rows are 16-byte aligned: four entries a load
-};
+constexpr int kVerHeld = 5;  // blocks of a warp's share kept in registers: 16 CTAs hold rows of 163840 entries
 
 LLMDIY_DEV double positive(double x) { return x > 0.0 ? x : 0.0; }  // NaN counts as 0
 
-// Weights of the four entries v0 .. v0 + 3 (0 past V).
-LLMDIY_DEV void ver_weights(const VerRow& r, int v0, double* w) {
-    float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool use_q = r.q != nullptr && r.T != 0.0;
-    if (r.vec && v0 + 3 < r.V) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(r.p + v0));
-        p[0] = a.x; p[1] = a.y; p[2] = a.z; p[3] = a.w;
-        if (use_q) {
-            const float4 c = __ldg(reinterpret_cast<const float4*>(r.q + v0));
-            q[0] = c.x; q[1] = c.y; q[2] = c.z; q[3] = c.w;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (v0 + e < r.V) {
-                p[e] = __ldg(r.p + v0 + e);
-                if (use_q) q[e] = __ldg(r.q + v0 + e);
-            }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const double pe = positive(p[e]);
-        w[e] = use_q ? positive(pe - r.T * positive(q[e])) : pe;
+// Entries v0 .. v0 + 3 of a row (0 past V); vec: the rows are 16-byte aligned.
+LLMDIY_DEV float4 ver_load(const float* row, int v0, int V, bool vec) {
+    if (vec && v0 + 3 < V) return __ldg(reinterpret_cast<const float4*>(row + v0));
+    float4 a;
+    a.x = v0 < V ? __ldg(row + v0) : 0.f;
+    a.y = v0 + 1 < V ? __ldg(row + v0 + 1) : 0.f;
+    a.z = v0 + 2 < V ? __ldg(row + v0 + 2) : 0.f;
+    a.w = v0 + 3 < V ? __ldg(row + v0 + 3) : 0.f;
+    return a;
+}
+
+// max(0, p - T q) of four entries (T = 0: p, whatever q holds)
+LLMDIY_DEV void ver_weights(const float4& p, const float4& q, double T, double* w) {
+    w[0] = positive(p.x);
+    w[1] = positive(p.y);
+    w[2] = positive(p.z);
+    w[3] = positive(p.w);
+    if (T != 0.0) {
+        w[0] = positive(w[0] - T * positive(q.x));
+        w[1] = positive(w[1] - T * positive(q.y));
+        w[2] = positive(w[2] - T * positive(q.z));
+        w[3] = positive(w[3] - T * positive(q.w));
     }
 }
 
@@ -183,29 +175,52 @@ __global__ void __launch_bounds__(kVerThreads)
 
     const int U = (V + 127) / 128, K = C * kVerWarps, k = rank * kVerWarps + warp;
     const int u0 = (int)((long long)U * k / K), u1 = (int)((long long)U * (k + 1) / K);
-    VerRow r;
-    r.V = V;
-    r.vec = vec;
+    const float *prow = target, *qrow = draft;  // the current node's rows
+    double T = 0.0;                             // weight of entry v: max(0, p - T q)
     int round = 0, dead0 = 0, ndead = 0;  // the current node's refused tokens: s.dead[dead0 .. dead0 + ndead)
-    // weights of this lane's four entries of a block, without the refused tokens
-    auto weights = [&](int u, double* w) {
+    // The first kVerHeld blocks of the warp's share stay in registers while the walk is at a node; rows
+    // too long for that read the others again in every round.
+    float4 hp[kVerHeld], hq[kVerHeld];
+    int held_node = -1;
+    int cur = 0, cand = -1, count = 0;
+    double Sj = 1.0;
+    // this lane's four entries of a block
+    auto weigh = [&](int u, const float4& p, const float4& q, double* w) {
+        ver_weights(p, q, T, w);
         const int v0 = u * 128 + lane * 4;
-        ver_weights(r, v0, w);
-        for (int j = 0; j < ndead; ++j) {
+        for (int j = 0; j < ndead; ++j) {  // without the refused tokens
             const int x = s.dead[dead0 + j] - v0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = x == e ? 0.0 : w[e];
         }
     };
+    auto fetch = [&](int u, float4& p, float4& q) {
+        const int v0 = u * 128 + lane * 4;
+        p = ver_load(prow, v0, V, vec);
+        q = draft && T != 0.0 ? ver_load(qrow, v0, V, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
     // this warp's total goes into every CTA's table; returns the table once it is complete.  Two tables
     // take turns: a CTA writes table r & 1 again only after the barrier of round r + 1, which every CTA
     // reaches after it has read round r's.
     auto totals = [&]() -> const double* {
+        if (held_node != cur) {
+            held_node = cur;
+#pragma unroll
+            for (int i = 0; i < kVerHeld; ++i) fetch(u0 + i < u1 ? u0 + i : U, hp[i], hq[i]);  // block U: past V, zeros
+        }
         double t = 0.0;
-#pragma unroll 4
-        for (int u = u0; u < u1; ++u) {
+#pragma unroll
+        for (int i = 0; i < kVerHeld; ++i) {
             double w[4];
-            weights(u, w);
+            weigh(u0 + i, hp[i], hq[i], w);
+            t += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+#pragma unroll 2
+        for (int u = u0 + kVerHeld; u < u1; ++u) {
+            float4 p, q;
+            double w[4];
+            fetch(u, p, q);
+            weigh(u, p, q, w);
             t += (w[0] + w[1]) + (w[2] + w[3]);
         }
         t = warp_sum(t);
@@ -222,21 +237,19 @@ __global__ void __launch_bounds__(kVerThreads)
         return t;
     };
 
-    int cur = 0, cand = s.child[0], count = 0;
-    double Sj = 1.0;
     auto at_node = [&](int c) {
         cur = c;
         cand = s.child[c];
-        r.p = target + (row0 + c) * ldt;
-        r.q = draft ? draft + (row0 + c) * ldd : nullptr;
-        r.T = 0.0;
+        prow = target + (row0 + c) * ldt;
+        qrow = draft + (draft ? (row0 + c) * ldd : 0);
+        T = 0.0;
         Sj = 1.0;
         dead0 += ndead;  // every node is refused once at most: the list never overflows
         ndead = 0;
     };
     at_node(0);
     while (cand >= 0) {  // every thread of the cluster takes the same steps
-        double w = positive(s.p[cand] - r.T * s.q[cand]);
+        double w = positive(s.p[cand] - T * s.q[cand]);
         for (int j = 0; j < ndead; ++j)
             if (s.dead[dead0 + j] == s.token[cand]) w = 0.0;
         if (s.u[cand] * Sj * s.q[cand] < w) {
@@ -250,7 +263,7 @@ __global__ void __launch_bounds__(kVerThreads)
             ++ndead;
             Sj -= w;
         } else {
-            r.T += Sj;
+            T += Sj;
             if (s.sibling[cand] >= 0) Sj = warp_sum(lane_sum(totals()));
         }
         cand = s.sibling[cand];
@@ -270,7 +283,7 @@ __global__ void __launch_bounds__(kVerThreads)
         }
         total = __shfl_sync(0xffffffffu, inc, 31);
         if (total > 0.0 || attempt) break;
-        r.T = 0.0;  // nothing left: from the target's row itself
+        T = 0.0;  // nothing left: from the target's row itself
         ndead = 0;
     }
     if (rank == 0 && tid == 0) {
@@ -304,9 +317,8 @@ __global__ void __launch_bounds__(kVerThreads)
     base = __shfl_sync(0xffffffffu, mine_base, f);
     if (chosen != k) return;
     int answer = -1;
-    for (int u = u0; u < u1; ++u) {
-        double w[4];
-        weights(u, w);
+    bool done = false;
+    auto search = [&](int u, const double* w) {
         const double own = (w[0] + w[1]) + (w[2] + w[3]);
         double run = own;
 #pragma unroll
@@ -315,22 +327,33 @@ __global__ void __launch_bounds__(kVerThreads)
             if (lane >= d) run += o;
         }
         const double block = __shfl_sync(0xffffffffu, run, 31);
+        double before = __shfl_up_sync(0xffffffffu, run, 1);
         const int l = pick_lane(base + run, own);
-        if (l >= 0) {
-            double before = __shfl_up_sync(0xffffffffu, run, 1);
-            if (lane == 0) before = 0.0;
-            before += base;
-            int at = -1;
+        if (done || l < 0) return;
+        before = base + (lane == 0 ? 0.0 : before);
+        int at = -1;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool open = at < 0 || !(before > goal);  // not past the goal yet
-                if (open && w[e] > 0.0) at = u * 128 + lane * 4 + e;
-                if (open) before += w[e];
-            }
-            answer = __shfl_sync(0xffffffffu, at, l);
+        for (int e = 0; e < 4; ++e) {
+            const bool open = at < 0 || !(before > goal);  // not past the goal yet
+            if (open && w[e] > 0.0) at = u * 128 + lane * 4 + e;
+            if (open) before += w[e];
         }
-        if (base + block > goal && answer >= 0) break;
+        answer = __shfl_sync(0xffffffffu, at, l);
+        done = base + block > goal;
         base += block;
+    };
+#pragma unroll
+    for (int i = 0; i < kVerHeld; ++i) {
+        double w[4];
+        weigh(u0 + i, hp[i], hq[i], w);
+        search(u0 + i, w);
+    }
+    for (int u = u0 + kVerHeld; u < u1 && !done; ++u) {
+        float4 p, q;
+        double w[4];
+        fetch(u, p, q);
+        weigh(u, p, q, w);
+        search(u, w);
     }
     if (lane == 0) next[b] = answer;
 }
