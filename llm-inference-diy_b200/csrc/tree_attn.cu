@@ -3,18 +3,24 @@
 //
 // Work.  A unit is (sequence, kv head, M tile): the query rows m = node * G + g of the G heads that share the kv
 // head, at most 128 rows (the MMA's M) of whole nodes.  A unit's keys are 64-row tiles: the cache
-// rows [0, len), then the tree's own rows.  All units' tiles in a row are dealt to a grid of two CTAs per
-// SM in equal contiguous ranges, cut anywhere (CTA w of W: tiles [total w / W, total (w + 1) / W)), whatever
-// the sequences' lengths: ragged batches and single sequences alike keep every SM busy to the end.
-// A range holds at most one unit's end, some whole units and one unit's beginning; whole units write
-// their output, cut ones an fp32 partial (o unnormalised, m, l), which tree_merge_k joins by
-// log-sum-exp in order (a fixed order: the same bits every time).
+// rows [0, len), then the tree's own rows.  Two ways to share them out (ta_plan):
+//
+// Direct: a cluster of C CTAs per unit, its tiles in C equal runs; the CTAs' parts (o unnormalised, m, l) are
+// joined through distributed shared memory, each CTA finishing a share of the rows.  One launch, no global
+// scratch.
+//
+// Flat: all units' tiles in a row, each unit with kTaUnitCost tiles more for its beginning and end, dealt to a
+// grid of two CTAs per SM in equal contiguous ranges cut anywhere, so that ragged batches keep every SM
+// busy to the end.  Whole units write their output, cut ones an fp32 partial, which tree_merge_k joins
+// in order (both ways join in a fixed order: the same bits every time).
 //
 // CTA.  Warp 4 streams Q (once per unit) and the K and V tiles by TMA through rings that run on
 // across units; warp 5 issues the MMAs:
-//   S(j)  = Q K(j)^T          128 x 64,  K = 128 dims  -> TMEM (two S buffers)
-//   O    += P(j) V(j)         128 x 128, K = 64 keys   -> TMEM (P from TMEM, over its S)
-// with S(j+1) issued before PV(j).  Warps 0-3 own the rows (thread = row = TMEM lane): mask, online
+//   S(j)  = Q K(j)^T          128 x 64,  K = 128 dims  -> TMEM
+//   O    += P(j) V(j)         128 x 128, K = 64 keys   -> TMEM (P from TMEM, two buffers)
+// S(j+1) follows as soon as the rows have S(j) in registers, so that neither the softmax nor PV(j) keeps the
+// next scores waiting (with P written over S and two S buffers, S(j+2) waited for PV(j) to complete,
+// and a tile took 1.2 us however few rows there were).  Warps 0-3 own the rows (thread = row = TMEM lane): mask, online
 // softmax in base 2, P as fp16; O is rescaled only when a row's maximum grows by more than 2^8 (P stays
 // within fp16, and O / l does not depend on the reference point).  fp16 P costs 2^-11 of each
 // probability, as the fp16 output does; l sums the unrounded fp32 values.
@@ -29,6 +35,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 #include <mutex>
 
 #include "gemm_tc_host.h"
@@ -46,10 +53,12 @@ constexpr int kTaRows = 128;     // query rows of a unit at most (MMA M)
 constexpr int kTaThreads = 192;  // warps 0-3: rows; warp 4: TMA; warp 5: MMA issue
 constexpr int kTaCtasPerSm = 2;
 constexpr int kTaTileBytes = kTaKeys * kTaDim * 2;  // one K or V tile
-constexpr uint32_t kTaCols = 256;                   // TMEM: S0 | S1 | O (128 columns)
+constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0 | P1 (32 each) | O (128)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
+constexpr int kTaMaxCluster = 8;  // (clusters of 16 do not all run at once: 16 x 16 CTAs took 24.6 us, 16 x 8 13.7)
+constexpr int kTaUnitCost = 4;  // a unit's beginning and end take about as long as four tiles
 
-// Two layouts of the same kernel: units of up to 64 rows need only 16 KB for Q and get a third K
+// Two layouts of the same kernel: units of up to 64 rows need only 16 KB for Q and get a third V
 // stage; the MMA still reads 128 rows, so rows 64-127 of its A operand are whatever lies behind
 // (rows do not mix, and nothing is read out of those).
 template <int QR, int KS, int VS>
@@ -58,7 +67,7 @@ struct TaSmem {
     half k[KS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, K-major (8 KB each)
     half v[VS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, MN-major (8 KB each)
     uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
-    uint64_t s_full[2], p_full[2], o_done[2], drain;
+    uint64_t s_full, s_free, p_full[2], o_done[2], drain;
     // tree rows with a non-finite V, by tree tile and quarter (a warp's 16 rows); two units' worth
     alignas(8) uint16_t bad[2][4][4];
     uint32_t tmem_base;
@@ -76,7 +85,8 @@ struct TaArgs {
     int B, N, H, KV, ldq, ldo, slot_rows, num_slots, max_len;
     int rows;  // rows of a partial: G * nodes_per_tile
     int npt;   // nodes per M tile
-    int W;     // most CTAs that share the tiles
+    int W;     // flat: most CTAs that share the tiles
+    int direct;
     int evict_first;
 };
 
@@ -96,31 +106,40 @@ LLMDIY_DEV void ta_shape(const TaArgs& a, int b, int& n, int& L, int& tiles, int
     units = a.KV * ((n + a.npt - 1) / a.npt);
 }
 
-// Tiles of all sequences before b (b = B: all).  A whole warp calls it together.
-LLMDIY_DEV long long ta_tiles_before(const TaArgs& a, int b, int lane) {
-    long long t = 0;
-    for (int i = lane; i < b; i += 32) {
-        int n, L, tiles, units;
-        ta_shape(a, i, n, L, tiles, units);
-        t += (long long)tiles * units;
+// Flat positions: a unit takes kTaUnitCost + tiles of them, the first kTaUnitCost without a tile.  W CTAs:
+// CTA w has [ta_start_of(w), ta_start_of(w + 1)).
+struct TaDeal {
+    int total, W, base, rem;
+    LLMDIY_DEV TaDeal(int total_, int most) : total(total_), W(min(most, total_)) {
+        base = W ? total / W : 0;
+        rem = total - base * W;
     }
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
-    return t;
-}
+    LLMDIY_DEV int start(int w) const { return base * w + min(w, rem); }
+    LLMDIY_DEV int owner(int f) const {
+        const int big = (base + 1) * rem;  // the first rem CTAs have one position more
+        return f < big ? f / (base + 1) : rem + (f - big) / base;
+    }
+};
 
-// A position in the row of all tiles, advanced unit by unit.
+// A unit, and what is left of a CTA's range from position `at` of it on.
 struct TaCursor {
     int b, n, L, tiles, units;  // sequence and its shape
     int unit;                   // within the sequence: kv head * M tiles + M tile
-    int tile;                   // next tile of the unit
-    long long left;             // tiles left of this CTA's range
-    LLMDIY_DEV int seg() const { return (int)min((long long)(tiles - tile), left); }  // tiles of this unit to do
-    LLMDIY_DEV void next(const TaArgs& a, int done) {  // past `done` tiles of this unit
-        left -= done;
-        tile += done;
-        if (tile < tiles || left <= 0) return;
-        tile = 0;
+    int at;                     // flat position within the unit
+    int left;                   // positions left of this CTA's range
+    int row0;                   // first cache row of the sequence's slot (set by the producer)
+    // the range's tiles of this unit: [t0, t0 + result)
+    LLMDIY_DEV int seg(int& t0) const {
+        t0 = max(at - kTaUnitCost, 0);
+        return max(min(at + left, tiles + kTaUnitCost) - kTaUnitCost, 0) - t0;
+    }
+    LLMDIY_DEV void next(const TaArgs& a) {  // to the next unit
+        left -= tiles + kTaUnitCost - at;
+        at = 0;
+        if (left <= 0) {
+            left = 0;
+            return;
+        }
         if (++unit < units) return;
         unit = 0;
         do {
@@ -133,49 +152,83 @@ struct TaCursor {
     }
 };
 
-LLMDIY_DEV long long ta_range_start(long long total, int w, int W) { return total * w / W; }
-LLMDIY_DEV int ta_ctas(long long total, int W) { return (int)min((long long)W, total); }
-
-// The cursor of CTA w's range [first, end) (a whole warp calls it together).
-LLMDIY_DEV void ta_start(const TaArgs& a, int w, int lane, TaCursor& c) {
-    const long long total = ta_tiles_before(a, a.B, lane);
-    c.left = 0;
-    const int W = ta_ctas(total, a.W);
-    if (w >= W) return;
-    const long long first = ta_range_start(total, w, W);
-    c.left = ta_range_start(total, w + 1, W) - first;
-    // the sequence that holds tile `first`: 32 sequences at a time, inclusive sums
-    long long before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        int n, L, tiles = 0, units = 0;
+// The unit at position f of the flat order, c.at = f within it; returns that unit's first position
+// (f < total; a whole warp calls it together).
+LLMDIY_DEV int ta_locate(const TaArgs& a, int f, int lane, TaCursor& c) {
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {  // 32 sequences at a time, inclusive sums
+        int n = 0, L = 0, tiles = 0, units = 0;
         if (b0 + lane < a.B) ta_shape(a, b0 + lane, n, L, tiles, units);
-        const long long own = (long long)tiles * units;
-        long long inc = own;
+        const int own = (tiles + kTaUnitCost) * units;
+        int inc = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+            const int o = __shfl_up_sync(0xffffffffu, inc, d);
             if (lane >= d) inc += o;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + inc > first);
+        const unsigned hit = __ballot_sync(0xffffffffu, before + inc > f);
         if (hit) {
             const int l = __ffs(hit) - 1;
             c.b = b0 + l;
-            const long long rest = first - before - __shfl_sync(0xffffffffu, inc - own, l);
-            ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
-            c.unit = (int)(rest / c.tiles);
-            c.tile = (int)(rest - (long long)c.unit * c.tiles);
-            return;
+            c.n = __shfl_sync(0xffffffffu, n, l);
+            c.L = __shfl_sync(0xffffffffu, L, l);
+            c.tiles = __shfl_sync(0xffffffffu, tiles, l);
+            c.units = __shfl_sync(0xffffffffu, units, l);
+            const int rest = f - before - __shfl_sync(0xffffffffu, inc - own, l);
+            c.unit = rest / (c.tiles + kTaUnitCost);
+            c.at = rest - c.unit * (c.tiles + kTaUnitCost);
+            return f - c.at;
         }
         before += __shfl_sync(0xffffffffu, inc, 31);
     }
-    c.left = 0;  // (not reached: the tile lies in some sequence)
+    c.left = 0;  // (not reached: the position lies in some sequence)
+    return 0;
+}
+LLMDIY_DEV int ta_total(const TaArgs& a, int lane) {
+    int t = 0;
+    for (int i = lane; i < a.B; i += 32) {
+        int n, L, tiles, units;
+        ta_shape(a, i, n, L, tiles, units);
+        t += (tiles + kTaUnitCost) * units;
+    }
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+    return t;
 }
 
+LLMDIY_DEV void named_bar_arrive(int id, int nthreads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 LLMDIY_DEV void tma_load_3d(void* dst, const void* tmap, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(smem_u32(dst)), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
+}
+// Loads from the shared memory of CTA `rank` of the cluster (addr: the same variable's address here).
+LLMDIY_DEV float2 ta_peer_f2(uint32_t addr, uint32_t rank) {
+    float2 v;
+    asm volatile("{\n .reg .b32 p;\n mapa.shared::cluster.u32 p, %2, %3;\n ld.shared::cluster.v2.f32 {%0, %1}, [p];\n}"
+                 : "=f"(v.x), "=f"(v.y)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
+}
+LLMDIY_DEV float4 ta_peer_f4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile(
+        "{\n .reg .b32 p;\n mapa.shared::cluster.u32 p, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
+LLMDIY_DEV void ta_store4(half* dst, const float4& v, float scale) {
+    const half2 y0 = __floats2half2_rn(v.x * scale, v.y * scale), y1 = __floats2half2_rn(v.z * scale, v.w * scale);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t*>(&y0);
+    u.y = *reinterpret_cast<const uint32_t*>(&y1);
+    *reinterpret_cast<uint2*>(dst) = u;
 }
 LLMDIY_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 LLMDIY_DEV uint32_t ta_pack(float lo, float hi) {
@@ -187,9 +240,39 @@ LLMDIY_DEV float ta_ex2(float x) {  // 2^x (2^-inf = 0)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The slow part of a wait, out of line: the loops that wait for every tile have to stay short, since each CTA's
+// few warps run their code straight through once a tile and instruction fetch sets their pace.
+__device__ __noinline__ bool ta_wait_slow(uint64_t* bar, uint32_t parity, const volatile int* fail) {
+    return mbar_wait(bar, parity, fail);
+}
+LLMDIY_DEV bool ta_wait(uint64_t* bar, uint32_t parity, const volatile int* fail) {
+    return mbar_try_wait(bar, parity) || ta_wait_slow(bar, parity, fail);
+}
+// Two fp32 values at once
+LLMDIY_DEV uint64_t ta_f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+LLMDIY_DEV void ta_split(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+LLMDIY_DEV uint64_t ta_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+LLMDIY_DEV uint64_t ta_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+LLMDIY_DEV float ta_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 constexpr float kTaScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
 
-template <int QR, int KS, int VS>
+template <int QR, int KS, int VS, bool DIRECT>
 __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     tree_attn_k(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap ttk,
@@ -199,7 +282,12 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     Smem& s = *reinterpret_cast<Smem*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.H / a.KV;
-    if (tid == 0) {
+    if (warp == 4 && lane == 0) {  // the thread that issues the copies: it need not wait for the others
+        prefetch_tmap(&tq);
+        prefetch_tmap(&tk);
+        prefetch_tmap(&tv);
+        prefetch_tmap(&ttk);
+        prefetch_tmap(&ttv);
         mbar_init(&s.q_full, 1);
         mbar_init(&s.q_empty, 1);
         for (int i = 0; i < KS; ++i) {
@@ -210,27 +298,52 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             mbar_init(&s.v_full[i], 1);
             mbar_init(&s.v_empty[i], 1);
         }
+        mbar_init(&s.s_full, 1);
+        mbar_init(&s.s_free, 4);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s.s_full[i], 1);
             mbar_init(&s.p_full[i], 4);
             mbar_init(&s.o_done[i], 1);
         }
         mbar_init(&s.drain, 1);
         s.fail = 0;
         mbar_fence_init();
+        fence_async_smem();
     }
     if (warp == 0) {
         tmem_alloc(&s.tmem_base, kTaCols);
         tmem_relinquish();
     }
     TaCursor c;
-    ta_start(a, blockIdx.x, lane, c);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    pdl_launch_dependents();  // the merge may be scheduled; it waits for this grid before it reads a partial
-    const uint32_t tmem = s.tmem_base, tO = tmem + 128;  // S(j) lives at tmem + 64 * (j & 1)
+    c.left = 0;
+    const int C = DIRECT ? (int)gridDim.x : 1, rank = DIRECT ? (int)blockIdx.x : 0;  // the unit's cluster
+    if (DIRECT) {
+        c.b = blockIdx.z;
+        c.unit = blockIdx.y;
+        ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
+        if (c.unit < c.units) {
+            const int t0 = c.tiles * rank / C, t1 = c.tiles * (rank + 1) / C;
+            c.at = kTaUnitCost + t0;
+            c.left = t1 - t0;
+        }
+    } else {
+        const TaDeal deal(ta_total(a, lane), a.W);
+        if ((int)blockIdx.x < deal.W) {
+            const int f = deal.start(blockIdx.x);
+            c.left = deal.start(blockIdx.x + 1) - f;
+            (void)ta_locate(a, f, lane, c);
+        }
+    }
     const bool work = c.left > 0;
+    if (warp != 4) {  // (the producer comes later)
+        tc_fence_before();
+        named_bar_sync(1, kTaThreads);
+        tc_fence_after();
+    } else {
+        __syncwarp();
+        named_bar_arrive(1, kTaThreads);
+    }
+    if (!DIRECT) pdl_launch_dependents();  // the merge may be scheduled; it waits for this grid before it reads
+    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;  // P(j) at tP + 32 * (j & 1)
 
     if (warp == 4 && work) {
         if (lane == 0) {
@@ -239,10 +352,10 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             uint32_t kn = 0, vn = 0, unit_no = 0;  // K tiles, V tiles and units' queries issued
             bool ok = true;
             auto load = [&](half (*dst)[kTaKeys * 64], const CUtensorMap* cache, const CUtensorMap* tree, int kvh, int t,
-                            int tc, uint64_t* bar) {
+                            int tc, int row0, uint64_t* bar) {
                 mbar_arrive_expect_tx(bar, kTaTileBytes);
                 if (t < tc) {
-                    const int y = ta_slot(a, c.b) * a.slot_rows + t * kTaKeys;
+                    const int y = row0 + t * kTaKeys;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         if (a.evict_first) tma_load_2d_hint(dst[x], cache, kvh * kTaDim + 64 * x, y, bar, pol);
@@ -256,9 +369,15 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             };
             while (ok && c.left > 0) {
                 const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
-                const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg();
+                int t0;
+                const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(t0);
+                if (cnt <= 0) {
+                    c.next(a);
+                    continue;
+                }
+                const int row0 = c.L ? ta_slot(a, c.b) * a.slot_rows : 0;
                 auto load_q = [&]() -> bool {
-                    if (unit_no && !mbar_wait(&s.q_empty, (unit_no - 1) & 1, &s.fail)) return false;
+                    if (unit_no && !ta_wait(&s.q_empty, (unit_no - 1) & 1, &s.fail)) return false;
                     mbar_arrive_expect_tx(&s.q_full, (uint32_t)(a.rows * kTaDim * 2));
                     tma_load_3d(s.q[0], &tq, 0, kvh * G, c.b * a.N + m0, &s.q_full);
                     tma_load_3d(s.q[1], &tq, 64, kvh * G, c.b * a.N + m0, &s.q_full);
@@ -267,18 +386,18 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                 };
                 const bool first_unit = unit_no == 0;
                 if (first_unit) (void)load_q();
-                for (int t = c.tile; t < c.tile + cnt; ++t) {
-                    if (kn >= KS && !mbar_wait(&s.k_empty[kn % KS], (kn / KS - 1) & 1, &s.fail)) { ok = false; break; }
-                    load(s.k[kn % KS], &tk, &ttk, kvh, t, tc, &s.k_full[kn % KS]);
+                for (int t = t0; t < t0 + cnt; ++t) {
+                    if (kn >= KS && !ta_wait(&s.k_empty[kn % KS], (kn / KS - 1) & 1, &s.fail)) { ok = false; break; }
+                    load(s.k[kn % KS], &tk, &ttk, kvh, t, tc, row0, &s.k_full[kn % KS]);
                     ++kn;
-                    if (vn >= VS && !mbar_wait(&s.v_empty[vn % VS], (vn / VS - 1) & 1, &s.fail)) { ok = false; break; }
-                    load(s.v[vn % VS], &tv, &ttv, kvh, t, tc, &s.v_full[vn % VS]);
+                    if (vn >= VS && !ta_wait(&s.v_empty[vn % VS], (vn / VS - 1) & 1, &s.fail)) { ok = false; break; }
+                    load(s.v[vn % VS], &tv, &ttv, kvh, t, tc, row0, &s.v_full[vn % VS]);
                     ++vn;
                     // a later unit's queries take the place of the last one's when its S are done: its first
                     // tile is under way by then
-                    if (t == c.tile && !first_unit && !load_q()) { ok = false; break; }
+                    if (t == t0 && !first_unit && !load_q()) { ok = false; break; }
                 }
-                if (ok) c.next(a, cnt);
+                if (ok) c.next(a);
             }
             // the last copies land in this CTA's shared memory: they have before it exits, whatever happens
             for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i) (void)mbar_wait(&s.k_full[i % KS], (i / KS) & 1);
@@ -292,63 +411,71 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             // ---------------- MMA issuer
             constexpr uint32_t idS = umma_idesc_f16_f32(kTaRows, kTaKeys, false);
             constexpr uint32_t idO = umma_idesc_f16_f32(kTaRows, kTaDim, true);
-            const uint32_t qa = smem_u32(s.q[0]);
-            const uint32_t total = (uint32_t)c.left;
+            // descriptors of the first stages; the start address field counts 16 bytes
+            const uint64_t qd = umma_desc_sw128(smem_u32(s.q[0])), kd = umma_desc_sw128(smem_u32(s.k[0][0])),
+                           vd = umma_desc_sw128_mn(smem_u32(s.v[0][0]), 8192, 1024);
             uint32_t unit_no = 0;
-            int in_unit = c.seg();  // tiles of the current unit whose S is not issued yet
-            // S(j) = Q K(j)^T into TMEM buffer j & 1, then release K(j)'s stage (and Q after a unit's last tile)
+            auto tiles_ahead = [&]() -> int {  // of the cursor's unit, or of the next one with any
+                int t0;
+                while (c.left > 0) {
+                    const int cnt = c.seg(t0);
+                    if (cnt > 0) return cnt;
+                    c.next(a);
+                }
+                return 0;
+            };
+            // S(j) = Q K(j)^T, then release K(j)'s stage
             auto qk = [&](uint32_t j, bool first) -> bool {
-                if (first && !mbar_wait(&s.q_full, unit_no++ & 1, &s.fail)) return false;
-                if (!mbar_wait(&s.k_full[j % KS], (j / KS) & 1, &s.fail)) return false;
+                if (first && !ta_wait(&s.q_full, unit_no++ & 1, &s.fail)) return false;
+                if (!ta_wait(&s.k_full[j % KS], (j / KS) & 1, &s.fail)) return false;
                 tc_fence_after();
-                const uint32_t kb = smem_u32(s.k[j % KS][0]);
+                const uint64_t kj = kd + (j % KS) * (kTaTileBytes / 16);
 #pragma unroll
                 for (int kk = 0; kk < kTaDim / 16; ++kk)
-                    umma_f16(tmem + 64u * (j & 1), umma_desc_sw128(qa + (kk >> 2) * (QR * 128) + 32 * (kk & 3)),
-                             umma_desc_sw128(kb + (kk >> 2) * 8192 + 32 * (kk & 3)), idS, kk != 0 ? 1u : 0u);
-                umma_commit(&s.s_full[j & 1]);
+                    umma_f16(tmem, qd + ((kk >> 2) * (QR * 128) + 32 * (kk & 3)) / 16,
+                             kj + ((kk >> 2) * 8192 + 32 * (kk & 3)) / 16, idS, kk != 0 ? 1u : 0u);
+                umma_commit(&s.s_full);
                 umma_commit(&s.k_empty[j % KS]);
                 return true;
             };
             auto pv = [&](uint32_t j, bool first) -> bool {  // O (+)= P(j) V(j), then release V(j)'s stage
-                if (!mbar_wait(&s.p_full[j & 1], (j >> 1) & 1, &s.fail)) return false;
-                if (!mbar_wait(&s.v_full[j % VS], (j / VS) & 1, &s.fail)) return false;
+                if (!ta_wait(&s.p_full[j & 1], (j >> 1) & 1, &s.fail)) return false;
+                if (!ta_wait(&s.v_full[j % VS], (j / VS) & 1, &s.fail)) return false;
                 tc_fence_after();
-                const uint32_t pa = tmem + 64u * (j & 1), vb = smem_u32(s.v[j % VS][0]);
+                const uint32_t pa = tP + 32u * (j & 1);
+                const uint64_t vj = vd + (j % VS) * (kTaTileBytes / 16);
 #pragma unroll
                 for (int kk = 0; kk < kTaKeys / 16; ++kk)
-                    umma_f16_tmem_a(tO, pa + 8 * kk, umma_desc_sw128_mn(vb + 2048 * kk, 8192, 1024), idO,
-                                    first && kk == 0 ? 0u : 1u);
+                    umma_f16_tmem_a(tO, pa + 8 * kk, vj + 2048 * kk / 16, idO, first && kk == 0 ? 0u : 1u);
                 umma_commit(&s.v_empty[j % VS]);
                 umma_commit(&s.o_done[j & 1]);  // last: the rows end the CTA when they have seen it
                 return true;
             };
             bool first_pv = true;
-            auto advance = [&]() {  // one more S issued; true: the next tile begins a unit
-                if (--in_unit) return false;
-                umma_commit(&s.q_empty);
-                c.next(a, c.seg());
-                in_unit = c.left > 0 ? c.seg() : 0;
-                return true;
-            };
-            bool ok = qk(0, true);
-            bool next_first = ok && advance();
-            for (uint32_t j = 0; ok && j < total; ++j) {
-                const bool cut = next_first;  // tile j + 1 begins a unit
-                if (j + 1 < total) {
-                    // S(j+1) takes the buffer that held P(j-1): PV(j-1) must be complete
-                    if (j >= 1 && !mbar_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, &s.fail)) { ok = false; break; }
-                    if (!cut) {
-                        if (!qk(j + 1, false)) { ok = false; break; }
-                        next_first = advance();
-                    }
+            int ahead = tiles_ahead();  // of the unit: tiles whose S is not issued yet
+            const bool any = ahead > 0;  // (a short range may lie in a unit's beginning)
+            bool ok = !any || qk(0, true);
+            --ahead;
+            for (uint32_t j = 0; ok && any; ++j) {
+                const bool cut = ahead == 0;  // tile j ends its unit
+                if (cut) {
+                    umma_commit(&s.q_empty);  // (after its last S)
+                    c.next(a);
+                    ahead = tiles_ahead();
+                }
+                const bool more = ahead > 0;
+                // S(j+1) takes the place of S(j) as soon as the rows have it in registers
+                if (more && !ta_wait(&s.s_free, j & 1, &s.fail)) { ok = false; break; }
+                if (more && !cut) {
+                    if (!qk(j + 1, false)) { ok = false; break; }
+                    --ahead;
                 }
                 if (!pv(j, first_pv)) { ok = false; break; }
+                if (!more) break;
                 first_pv = cut;
-                if (cut && j + 1 < total) {
-                    // a new unit's Q arrives after the old unit's last S: issue PV first, then wait for Q
+                if (cut) {  // a new unit's Q arrives after the old unit's last S: its first S comes after PV
                     if (!qk(j + 1, true)) { ok = false; break; }
-                    next_first = advance();
+                    --ahead;
                 }
             }
             if (!ok) {
@@ -364,20 +491,28 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         const int r = tid, words = (a.N + 63) / 64;
         uint32_t j = 0;
         int slot_no = 0, tree_units = 0;
+        float m = -INFINITY, l = 0.f;
         bool ok = true;
         auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {  // one answer for the warp
-            return __all_sync(0xffffffffu, mbar_wait(bar, parity, &s.fail));
+            return __all_sync(0xffffffffu, ta_wait(bar, parity, &s.fail));
         };
         while (ok && c.left > 0) {
             const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
-            const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(), t0 = c.tile;
+            int t0;
+            const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(t0);
+            if (cnt <= 0) {
+                c.next(a);
+                slot_no = 1;
+                continue;
+            }
             const int node = m0 + r / G, g = r - (r / G) * G;
             const bool live = r < a.rows && node < c.n;
             const bool warp_live = warp * 32 < min(a.rows, (c.n - m0) * G);
             const uint64_t* mrow = a.mask + ((size_t)c.b * a.N + (live ? node : 0)) * words;
             const int tt0 = max(t0 - tc, 0);  // first tree tile of this segment, if any
             uint64_t word = live && t0 + cnt > tc ? mrow[tt0] : 0;
-            float m = -INFINITY, l = 0.f;
+            m = -INFINITY;
+            l = 0.f;
             for (int t = t0; t < t0 + cnt; ++t, ++j) {
                 const bool tree = t >= tc;
                 const int tt = t - tc;
@@ -408,27 +543,29 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     if (tree && lane == 0) s.bad[tree_units & 1][tt][warp] = (uint16_t)bad16;
                     fence_async_smem();
                 }
-                if (!warp_wait(&s.s_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
+                if (!warp_wait(&s.s_full, j & 1)) { ok = false; break; }
                 if (warp_live) {
                     tc_fence_after();
                     float x[kTaKeys];
 #pragma unroll
                     for (int q = 0; q < kTaKeys; q += 16)
-                        tmem_ld16(tmem + 64u * (j & 1) + lane_off + q, reinterpret_cast<uint32_t*>(x + q));
+                        tmem_ld16(tmem + lane_off + q, reinterpret_cast<uint32_t*>(x + q));
                     tmem_ld_wait();
+                    tc_fence_before();
+                    if (lane == 0) mbar_arrive(&s.s_free);
                     if (tree || nv < kTaKeys) {
                         const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
 #pragma unroll
                         for (int q = 0; q < kTaKeys; ++q)
                             x[q] = ((q < 32 ? lo : hi) & (1u << (q & 31))) ? x[q] : -INFINITY;
                     }
-                    float mx[8];
+                    float mx[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mx[e] = x[e];
+                    for (int e = 0; e < 4; ++e) mx[e] = ta_max3(x[3 * e], x[3 * e + 1], x[3 * e + 2]);
 #pragma unroll
-                    for (int q = 8; q < kTaKeys; ++q) mx[q & 7] = fmaxf(mx[q & 7], x[q]);
-                    const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                            fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * kTaScaleLog2;
+                    for (int q = 12; q < 60; q += 2) mx[(q >> 1) & 3] = ta_max3(mx[(q >> 1) & 3], x[q], x[q + 1]);
+                    const float top = ta_max3(ta_max3(mx[0], x[60], x[61]), ta_max3(mx[1], x[62], x[63]),
+                                              fmaxf(mx[2], mx[3])) * kTaScaleLog2;
                     const bool grow = live && top > m + (t == t0 ? 0.f : 8.f);  // (a NaN maximum leaves m)
                     if (t != t0 && __any_sync(0xffffffffu, grow)) {
                         // rescale O, complete through PV(j-1) (the whole warp: TMEM moves 32 rows at a time)
@@ -449,23 +586,29 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     }
                     if (grow) m = top;
                     const float nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every p is 2^-inf = 0
-                    float ls[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ls[e] = 0.f;
+                    const uint64_t scale2 = ta_f2(kTaScaleLog2, kTaScaleLog2), nm2 = ta_f2(nm, nm);
+                    uint64_t ls[2] = {0, 0};
                     uint32_t pk[kTaKeys / 2];
 #pragma unroll
                     for (int q = 0; q < kTaKeys; q += 2) {
-                        const float p0 = ta_ex2(__fmaf_rn(x[q], kTaScaleLog2, nm));
-                        const float p1 = ta_ex2(__fmaf_rn(x[q + 1], kTaScaleLog2, nm));
-                        ls[q & 7] += p0;
-                        ls[(q + 1) & 7] += p1;
+                        float p0, p1;
+                        ta_split(ta_fma2(ta_f2(x[q], x[q + 1]), scale2, nm2), p0, p1);
+                        p0 = ta_ex2(p0);
+                        p1 = ta_ex2(p1);
+                        ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(p0, p1));
                         pk[q / 2] = ta_pack(p0, p1);
                     }
-                    l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+                    float l0, l1;
+                    ta_split(ta_add2(ls[0], ls[1]), l0, l1);
+                    l += l0 + l1;
+                    // P, once PV(j-2) has read the buffer
+                    if (j >= 2 && !warp_wait(&s.o_done[j & 1], ((j >> 1) - 1) & 1)) { ok = false; break; }
 #pragma unroll
-                    for (int q = 0; q < kTaKeys / 2; q += 16) tmem_st16(tmem + 64u * (j & 1) + lane_off + q, pk + q);
+                    for (int q = 0; q < kTaKeys / 2; q += 16) tmem_st16(tP + 32u * (j & 1) + lane_off + q, pk + q);
                     tmem_st_wait();
                     tc_fence_before();
+                } else if (lane == 0) {
+                    mbar_arrive(&s.s_free);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.p_full[j & 1]);
@@ -474,27 +617,30 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             // ---------------- the unit's (or its part's) output
             if (!warp_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
-            const bool whole = cnt == c.tiles;
+            const bool whole = cnt == c.tiles && C == 1;
+            // a part of a unit goes to the workspace, or (direct) to shared memory: Q, K and V are done with
+            float* own = reinterpret_cast<float*>(s.k[0][0]) + tid * kTaDim;
             const bool any_tree = t0 + cnt > tc;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const size_t at = (size_t)(blockIdx.x * 2 + slot_no) * a.rows + r;
             half* dst = a.O + ((size_t)c.b * a.N + node) * a.ldo + (kvh * G + g) * kTaDim;
             float* pdst = a.part + at * kTaDim;
             if (warp_live) {
+                // non-finite V rows that this part's rows left out of PV (rare)
+                bool any_bad = false;
+                if (any_tree)
+                    for (int tt = tt0; tt < t0 + cnt - tc; ++tt)
+                        any_bad |= *reinterpret_cast<volatile uint64_t*>(s.bad[tree_units & 1][tt]) != 0;
 #pragma unroll 1
-                for (int q = 0; q < kTaDim; q += 16) {
-                    uint32_t o[16];
+                for (int q = 0; q < kTaDim; q += 32) {
+                    float v[32];
                     __syncwarp();
-                    tmem_ld16(tO + lane_off + q, o);
+                    tmem_ld16(tO + lane_off + q, reinterpret_cast<uint32_t*>(v));
+                    tmem_ld16(tO + lane_off + q + 16, reinterpret_cast<uint32_t*>(v + 16));
                     tmem_ld_wait();
-                    float v[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(o[e]);
-                    if (any_tree && live) {
-                        // tree rows with a non-finite V that this row sees: their p * v, left out of PV
+                    if (any_bad && live) {
                         for (int tt = tt0; tt < t0 + cnt - tc; ++tt) {
                             uint64_t hit = *reinterpret_cast<volatile uint64_t*>(s.bad[tree_units & 1][tt]);
-                            if (!hit) continue;
                             hit &= mrow[tt];
                             for (; hit; hit &= hit - 1) {
                                 const int kn = tt * 64 + __ffsll((long long)hit) - 1;
@@ -505,31 +651,74 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                                 for (int e = 0; e < kTaDim; ++e) d = __fmaf_rn(h2f(qr[e]), h2f(kr[e]), d);
                                 const float p = ta_ex2(__fmaf_rn(d, kTaScaleLog2, m == -INFINITY ? 0.f : -m));
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) v[e] = __fmaf_rn(p, h2f(vr[q + e]), v[e]);
+                                for (int e = 0; e < 32; ++e) v[e] = __fmaf_rn(p, h2f(vr[q + e]), v[e]);
                             }
                         }
                     }
                     if (!live) continue;
                     if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] *= inv;
-                        *reinterpret_cast<uint4*>(dst + q) = pack8(v);
-                        *reinterpret_cast<uint4*>(dst + q + 8) = pack8(v + 8);
+                        for (int e = 0; e < 32; ++e) v[e] *= inv;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) *reinterpret_cast<uint4*>(dst + q + e) = pack8(v + e);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4)
-                            *reinterpret_cast<float4*>(pdst + q + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        for (int e = 0; e < 32; e += 4) {
+                            // (16-byte pieces of a row turned by the row: 32 rows' stores meet different banks)
+                            float* to = DIRECT ? own + (((q + e) / 4) ^ lane) * 4 : pdst + q + e;
+                            *reinterpret_cast<float4*>(to) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        }
                     }
                 }
-                if (live && !whole)
+                if (live && !whole && !DIRECT)
                     *reinterpret_cast<float2*>(a.part + (size_t)a.W * 2 * a.rows * kTaDim + at * 2) = make_float2(m, l);
             }
             tc_fence_before();  // O has been read: the next unit's first PV may overwrite it
             if (any_tree) ++tree_units;
             slot_no = 1;
-            c.next(a, cnt);
+            c.next(a);
         }
         if (!ok) s.fail = 1;
+        if (DIRECT && C > 1) reinterpret_cast<float2*>(s.q[0])[tid] = make_float2(m, l);
+    } else if (warp < 4 && DIRECT && C > 1) {
+        reinterpret_cast<float2*>(s.q[0])[tid] = make_float2(-INFINITY, 0.f);  // no tile for this CTA
+    }
+    if (DIRECT && C > 1) {
+        // ---------------- the cluster's parts of the unit's rows row r by CTA r C / rows
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (c.unit < c.units) {
+            const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+            const int live = min(a.rows, (c.n - m0) * G), r1 = live * (rank + 1) / C;
+            const uint32_t ml = smem_u32(s.q[0]), oo = smem_u32(s.k[0][0]);
+            for (int r = live * rank / C + warp; r < r1; r += kTaThreads / 32) {
+                float2 w = make_float2(-INFINITY, 0.f);
+                if (lane < C) w = ta_peer_f2(ml + r * 8, lane);
+                float M = w.x;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                const unsigned parts = __ballot_sync(0xffffffffu, w.x != -INFINITY || w.y != w.y);
+                // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
+                const float f = w.x == -INFINITY ? (w.y == w.y ? 0.f : 1.f) : exp2f(w.x - M);
+                float L = w.y * f;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                for (int k = 0; k < C; ++k) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k);
+                    if (!((parts >> k) & 1)) continue;  // (a part that saw nothing has no o)
+                    const float4 y = ta_peer_f4(oo + r * (kTaDim * 4) + ((lane ^ (r & 31)) * 16), k);
+                    acc.x = __fmaf_rn(fk, y.x, acc.x);
+                    acc.y = __fmaf_rn(fk, y.y, acc.y);
+                    acc.z = __fmaf_rn(fk, y.z, acc.z);
+                    acc.w = __fmaf_rn(fk, y.w, acc.w);
+                }
+                const int node = m0 + r / G, h = kvh * G + r - (r / G) * G;
+                ta_store4(a.O + ((size_t)c.b * a.N + node) * a.ldo + h * kTaDim + lane * 4, acc, L == 0.f ? 0.f : 1.f / L);
+            }
+        }
+        // The peers have read this CTA's part (relaxed: nothing written has to be seen).
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -537,67 +726,64 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     if (warp == 0) tmem_dealloc(tmem, kTaCols);
 }
 
-// Joins the partials of the units that were cut: one warp per output row (sequence, node, head), which
-// finds the CTAs that share its unit from the same arithmetic.  Lane s weighs partial s, then
-// each lane sums 4 dims over the partials in order.
+// Flat: joins the partials of the units that were cut.  Block w - 1 looks at the cut before CTA w: if it
+// parts a unit's tiles, the blocks of that unit's cuts share its rows, a warp per row: lane s weighs partial
+// s, then each lane sums 4 dims over the partials in order.
 constexpr int kTaMergeWarps = 8;
 
 __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_constant__ TaArgs a) {
-    const int lane = threadIdx.x & 31, h = blockIdx.x * kTaMergeWarps + (threadIdx.x >> 5);
-    const int b = blockIdx.z, i = blockIdx.y;
-    int n, L, tiles, units;
-    ta_shape(a, b, n, L, tiles, units);
-    const long long total = ta_tiles_before(a, a.B, lane), before = ta_tiles_before(a, b, lane);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = blockIdx.x + 1;
+    const TaDeal deal(ta_total(a, lane), a.W);
+    TaCursor c;
+    int f0 = 0;
+    const bool cut = w < deal.W;
+    if (cut) f0 = ta_locate(a, deal.start(w), lane, c);
     // every thread waits for the attention kernel, also where there is nothing to join: this grid
     // must not be over before that one is
     pdl_wait();
-    if (h >= a.H || i >= n) return;
-    const int G = a.H / a.KV, mt = units / a.KV, kvh = h / G, r = (i % a.npt) * G + h % G;
-    const int W = ta_ctas(total, a.W);
-    const long long f0 = before + (long long)(kvh * mt + i / a.npt) * tiles;
-    const int w0 = (int)(((f0 + 1) * W - 1) / total), w1 = (int)(((f0 + tiles) * W - 1) / total);
-    if (w0 == w1) return;  // whole: already written
-    // the first CTA's part of this unit is its first segment only when its range starts here
-    const int first = w0 * 2 + (ta_range_start(total, w0, W) == f0 ? 0 : 1);
+    if (!cut || c.at <= kTaUnitCost) return;  // no tile of the unit before the cut
+    const int w0 = deal.owner(f0 + kTaUnitCost), w1 = deal.owner(f0 + kTaUnitCost + c.tiles - 1);
+    // the first CTA's part of this unit is its first segment only when its range does not start before the unit
+    const int first = w0 * 2 + (deal.start(w0) >= f0 ? 0 : 1);
+    const int G = a.H / a.KV, mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+    const int live = min(a.rows, (c.n - m0) * G), share = w - w0 - 1, shares = w1 - w0;
+    const int r1 = live * (share + 1) / shares;
     const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.W * 2 * a.rows * kTaDim);
-    float M = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 32)
-        M = fmaxf(M, __ldcg(ml + (size_t)(w == w0 ? first : w * 2) * a.rows + r).x);
+    for (int r = live * share / shares + warp; r < r1; r += kTaMergeWarps) {
+        float M = -INFINITY;
+        for (int k = w0 + lane; k <= w1; k += 32)
+            M = fmaxf(M, __ldcg(ml + (size_t)(k == w0 ? first : k * 2) * a.rows + r).x);
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float Ls = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = w0; c0 <= w1; c0 += 32) {
-        float f = 0.f, lw = 0.f;
-        if (c0 + lane <= w1) {
-            const int w = c0 + lane;
-            const float2 y = __ldcg(ml + (size_t)(w == w0 ? first : w * 2) * a.rows + r);
-            f = y.x == -INFINITY ? 0.f : exp2f(y.x - M);
-            lw = y.x == -INFINITY ? y.y : y.y * f;  // nothing seen: l = 0 (or NaN, which stays)
-            if (y.y != y.y) f = 1.f;
-        }
-        Ls += lw;
-        const int cnt = min(32, w1 - c0 + 1);
+        for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        float Ls = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c0 = w0; c0 <= w1; c0 += 32) {
+            float f = 0.f;
+            if (c0 + lane <= w1) {
+                const int k = c0 + lane;
+                const float2 y = __ldcg(ml + (size_t)(k == w0 ? first : k * 2) * a.rows + r);
+                // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
+                f = y.x == -INFINITY ? (y.y == y.y ? 0.f : 1.f) : exp2f(y.x - M);
+                Ls += y.y * f;
+            }
+            const int cnt = min(32, w1 - c0 + 1);
 #pragma unroll 4
-        for (int k = 0; k < cnt; ++k) {
-            const int w = c0 + k;
-            const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(
-                a.part + ((size_t)(w == w0 ? first : w * 2) * a.rows + r) * kTaDim) + lane);
-            acc.x = __fmaf_rn(fk, y.x, acc.x);
-            acc.y = __fmaf_rn(fk, y.y, acc.y);
-            acc.z = __fmaf_rn(fk, y.z, acc.z);
-            acc.w = __fmaf_rn(fk, y.w, acc.w);
+            for (int i = 0; i < cnt; ++i) {
+                const int k = c0 + i;
+                const float fk = __shfl_sync(0xffffffffu, f, i);
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(
+                    a.part + ((size_t)(k == w0 ? first : k * 2) * a.rows + r) * kTaDim) + lane);
+                acc.x = __fmaf_rn(fk, y.x, acc.x);
+                acc.y = __fmaf_rn(fk, y.y, acc.y);
+                acc.z = __fmaf_rn(fk, y.z, acc.z);
+                acc.w = __fmaf_rn(fk, y.w, acc.w);
+            }
         }
-    }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
-    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
-    const half2 y0 = __floats2half2_rn(acc.x * inv, acc.y * inv), y1 = __floats2half2_rn(acc.z * inv, acc.w * inv);
-    uint2 u;
-    u.x = *reinterpret_cast<const uint32_t*>(&y0);
-    u.y = *reinterpret_cast<const uint32_t*>(&y1);
-    *reinterpret_cast<uint2*>(a.O + ((size_t)b * a.N + i) * a.ldo + h * kTaDim + lane * 4) = u;
+        for (int o = 16; o >= 1; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
+        const int node = m0 + r / G, h = kvh * G + r - (r / G) * G;
+        ta_store4(a.O + ((size_t)c.b * a.N + node) * a.ldo + h * kTaDim + lane * 4, acc, Ls == 0.f ? 0.f : 1.f / Ls);
+    }
 }
 
 // ------------------------------------------------------------------ host
@@ -614,12 +800,13 @@ int ta_sms() {
 }
 
 struct TaPlan {
-    int G, npt, rows, W;
+    int G, npt, rows, mt, W;
+    int cluster;  // direct: CTAs per unit (0: flat)
     bool ok;
-    size_t floats;  // of the partials
+    size_t floats;  // of the flat partials
 };
 
-// The grid and the partials' size: never smaller for a larger B, N or max_len (same heads), so a
+// The grid and the partials' size; the latter is never smaller for a larger B, N or max_len (same heads), so a
 // workspace sized for the largest call serves the others.
 TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     TaPlan p = {};
@@ -629,10 +816,19 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     p.G = H / KV;
     p.npt = std::min(kTaRows / p.G, N);
     p.rows = p.G * p.npt;
+    p.mt = (N + p.npt - 1) / p.npt;
     const long long tiles = ((long long)max_len + kTaKeys - 1) / kTaKeys + (N + kTaKeys - 1) / kTaKeys;
-    const long long units = (long long)B * KV * ((N + p.npt - 1) / p.npt);
-    p.W = (int)std::min<long long>(kTaCtasPerSm * ta_sms(), units * tiles);
+    const long long units = (long long)B * KV * p.mt;
+    p.ok = units * (tiles + kTaUnitCost) <= 0x7fffffffLL;
+    const int slots = kTaCtasPerSm * ta_sms();
+    p.W = (int)std::min<long long>(slots, units * tiles);
     p.floats = (size_t)p.W * 2 * p.rows * (kTaDim + 2);
+    int c = 1;
+    while (c < kTaMaxCluster && 2 * c * units <= slots && 2 * c <= tiles) c *= 2;
+    const char* env = getenv("TD");
+    const int lim = env ? atoi(env) : 8;
+    if (getenv("TC")) c = std::min(c, atoi(getenv("TC")));
+    if ((tiles + c - 1) / c <= lim) p.cluster = c;
     return p;
 }
 
@@ -662,21 +858,33 @@ bool make_query_map(CUtensorMap* m, const void* base, int nodes, int H, int ldq,
 
 constexpr size_t kTaCtl = 4;  // floats before the partials: word 0 is the error word
 
-template <int QR, int KS, int VS>
-int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, cudaStream_t st) {
-    auto kern = tree_attn_k<QR, KS, VS>;
+template <int QR, int KS, int VS, bool DIRECT>
+int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cluster, cudaStream_t st) {
+    auto kern = tree_attn_k<QR, KS, VS, DIRECT>;
     constexpr int bytes = (int)sizeof(TaSmem<QR, KS, VS>);
     static_assert(bytes <= 115712, "two CTAs share an SM");
+    static_assert((KS + VS) * kTaTileBytes >= QR * kTaDim * 4, "a part's rows fit over K and V");
     static std::atomic<bool> set[64];  // per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= 64 || !set[dev])) {
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess && dev >= 0 && dev < 64) set[dev] = true;
     }
     if (e != cudaSuccess) return (int)e;
-    kern<<<a.W, kTaThreads, bytes, st>>>(m[0], m[1], m[2], m[3], m[4], a, err);
-    return (int)cudaGetLastError();
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid;
+    lc.blockDim = dim3(kTaThreads);
+    lc.dynamicSmemBytes = bytes;
+    lc.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&lc, kern, m[0], m[1], m[2], m[3], m[4], a, err);
 }
 
 }  // namespace
@@ -732,10 +940,16 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     a.evict_first = p.npt >= N;  // one M tile: every K/V row is read once
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int* err = reinterpret_cast<int*>(work);
-    int rc = p.rows <= 64 ? ta_launch<64, 3, 3>(m, a, err, st) : ta_launch<128, 3, 2>(m, a, err, st);
-    if (rc) return rc;
+    a.direct = p.cluster > 0;
+    const dim3 grid = a.direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W);
+    const int cluster = std::max(1, p.cluster);
+    int rc = p.rows <= 64 ? a.direct ? ta_launch<64, 3, 3, true>(m, a, err, grid, cluster, st)
+                                     : ta_launch<64, 3, 3, false>(m, a, err, grid, cluster, st)
+             : a.direct   ? ta_launch<128, 3, 2, true>(m, a, err, grid, cluster, st)
+                          : ta_launch<128, 3, 2, false>(m, a, err, grid, cluster, st);
+    if (rc || a.direct || p.W < 2) return rc;
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((num_heads + kTaMergeWarps - 1) / kTaMergeWarps, N, B);
+    lc.gridDim = dim3(p.W - 1);
     lc.blockDim = dim3(kTaMergeWarps * 32);
     lc.stream = st;
     cudaLaunchAttribute at[1];
