@@ -15,7 +15,7 @@
 // in order (both ways join in a fixed order: the same bits every time).
 //
 // CTA.  Warp 4 streams Q (once per unit) and the K and V tiles by TMA through rings that run on
-// across units; warp 5 issues the MMAs:
+// across units; warps 5 and 6 issue the MMAs:
 //   S(j)  = Q K(j)^T          128 x 64,  K = 128 dims  -> TMEM
 //   O    += P(j) V(j)         128 x 128, K = 64 keys   -> TMEM (P from TMEM, two buffers)
 // S(j+1) follows as soon as the rows have S(j) in registers, so that neither the softmax nor PV(j) keeps the
@@ -50,7 +50,7 @@ namespace {
 constexpr int kTaDim = 128;
 constexpr int kTaKeys = 64;      // keys per tile
 constexpr int kTaRows = 128;     // query rows of a unit at most (MMA M)
-constexpr int kTaThreads = 192;  // warps 0-3: rows; warp 4: TMA; warp 5: MMA issue
+constexpr int kTaThreads = 224;  // warps 0-3: rows; warp 4: TMA; warps 5 and 6: the MMAs of S and of O
 constexpr int kTaCtasPerSm = 2;
 constexpr int kTaTileBytes = kTaKeys * kTaDim * 2;  // one K or V tile
 constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0 | P1 (32 each) | O (128)
@@ -67,7 +67,7 @@ struct TaSmem {
     half k[KS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, K-major (8 KB each)
     half v[VS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, MN-major (8 KB each)
     uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
-    uint64_t s_full, s_free, p_full[2], o_done[2], drain;
+    uint64_t s_full, s_free, p_full[2], o_done[2], drain[2];
     // tree rows with a non-finite V, by tree tile and quarter (a warp's 16 rows); two units' worth
     alignas(8) uint16_t bad[2][4][4];
     uint32_t tmem_base;
@@ -230,6 +230,11 @@ LLMDIY_DEV void ta_store4(half* dst, const float4& v, float scale) {
     u.y = *reinterpret_cast<const uint32_t*>(&y1);
     *reinterpret_cast<uint2*>(dst) = u;
 }
+LLMDIY_DEV bool elect_one() {  // one lane of a converged warp
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+    return p != 0;
+}
 LLMDIY_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 LLMDIY_DEV uint32_t ta_pack(float lo, float hi) {
     const half2 h = __floats2half2_rn(lo, hi);
@@ -304,7 +309,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             mbar_init(&s.p_full[i], 4);
             mbar_init(&s.o_done[i], 1);
         }
-        mbar_init(&s.drain, 1);
+        mbar_init(&s.drain[0], 1);
+        mbar_init(&s.drain[1], 1);
         s.fail = 0;
         mbar_fence_init();
         fence_async_smem();
@@ -334,6 +340,9 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         }
     }
     const bool work = c.left > 0;
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {  // one answer for the warp
+        return __all_sync(0xffffffffu, ta_wait(bar, parity, &s.fail));
+    };
     if (warp != 4) {  // (the producer comes later)
         tc_fence_before();
         named_bar_sync(1, kTaThreads);
@@ -407,82 +416,81 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         }
         __syncwarp();
     } else if (warp == 5 && work) {
-        if (lane == 0) {
-            // ---------------- MMA issuer
-            constexpr uint32_t idS = umma_idesc_f16_f32(kTaRows, kTaKeys, false);
-            constexpr uint32_t idO = umma_idesc_f16_f32(kTaRows, kTaDim, true);
-            // descriptors of the first stages; the start address field counts 16 bytes
-            const uint64_t qd = umma_desc_sw128(smem_u32(s.q[0])), kd = umma_desc_sw128(smem_u32(s.k[0][0])),
-                           vd = umma_desc_sw128_mn(smem_u32(s.v[0][0]), 8192, 1024);
-            uint32_t unit_no = 0;
-            auto tiles_ahead = [&]() -> int {  // of the cursor's unit, or of the next one with any
-                int t0;
-                while (c.left > 0) {
-                    const int cnt = c.seg(t0);
-                    if (cnt > 0) return cnt;
-                    c.next(a);
-                }
-                return 0;
-            };
-            // S(j) = Q K(j)^T, then release K(j)'s stage
-            auto qk = [&](uint32_t j, bool first) -> bool {
-                if (first && !ta_wait(&s.q_full, unit_no++ & 1, &s.fail)) return false;
-                if (!ta_wait(&s.k_full[j % KS], (j / KS) & 1, &s.fail)) return false;
+        // ---------------- S(j) = Q K(j)^T, then release K(j)'s stage (and Q after a unit's last tile)
+        constexpr uint32_t idS = umma_idesc_f16_f32(kTaRows, kTaKeys, false);
+        // descriptors of the first stages; the start address field counts 16 bytes
+        const uint64_t qd = umma_desc_sw128(smem_u32(s.q[0])), kd = umma_desc_sw128(smem_u32(s.k[0][0]));
+        const bool lead = elect_one();
+        uint32_t j = 0, st = 0, ph = 0, unit_no = 0;
+        bool ok = true;
+        while (ok && c.left > 0) {
+            int t0;
+            const int cnt = c.seg(t0);
+            for (int i = 0; i < cnt; ++i, ++j) {
+                if (i == 0 && !warp_wait(&s.q_full, unit_no++ & 1)) { ok = false; break; }
+                // S(j) takes the place of S(j-1) as soon as the rows have that in registers
+                if (j && !warp_wait(&s.s_free, (j - 1) & 1)) { ok = false; break; }
+                if (!warp_wait(&s.k_full[st], ph)) { ok = false; break; }
                 tc_fence_after();
-                const uint64_t kj = kd + (j % KS) * (kTaTileBytes / 16);
+                const uint64_t kj = kd + st * (kTaTileBytes / 16);
+                if (lead) {
 #pragma unroll
-                for (int kk = 0; kk < kTaDim / 16; ++kk)
-                    umma_f16(tmem, qd + ((kk >> 2) * (QR * 128) + 32 * (kk & 3)) / 16,
-                             kj + ((kk >> 2) * 8192 + 32 * (kk & 3)) / 16, idS, kk != 0 ? 1u : 0u);
-                umma_commit(&s.s_full);
-                umma_commit(&s.k_empty[j % KS]);
-                return true;
-            };
-            auto pv = [&](uint32_t j, bool first) -> bool {  // O (+)= P(j) V(j), then release V(j)'s stage
-                if (!ta_wait(&s.p_full[j & 1], (j >> 1) & 1, &s.fail)) return false;
-                if (!ta_wait(&s.v_full[j % VS], (j / VS) & 1, &s.fail)) return false;
+                    for (int kk = 0; kk < kTaDim / 16; ++kk)
+                        umma_f16(tmem, qd + ((kk >> 2) * (QR * 128) + 32 * (kk & 3)) / 16,
+                                 kj + ((kk >> 2) * 8192 + 32 * (kk & 3)) / 16, idS, kk != 0 ? 1u : 0u);
+                    umma_commit(&s.s_full);
+                    umma_commit(&s.k_empty[st]);
+                    if (i + 1 == cnt) umma_commit(&s.q_empty);
+                }
+                __syncwarp();
+                if (++st == KS) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            }
+            c.next(a);
+        }
+        if (!ok) {
+            s.fail = 1;
+            if (lead) umma_commit(&s.drain[0]);  // every MMA issued so far completes before the CTA exits
+            (void)mbar_wait(&s.drain[0], 0);
+        }
+        __syncwarp();
+    } else if (warp == 6 && work) {
+        // ---------------- O (+)= P(j) V(j), then release V(j)'s stage
+        constexpr uint32_t idO = umma_idesc_f16_f32(kTaRows, kTaDim, true);
+        const uint64_t vd = umma_desc_sw128_mn(smem_u32(s.v[0][0]), 8192, 1024);
+        const bool lead = elect_one();
+        uint32_t j = 0, st = 0, ph = 0;
+        bool ok = true;
+        while (ok && c.left > 0) {
+            int t0;
+            const int cnt = c.seg(t0);
+            for (int i = 0; i < cnt; ++i, ++j) {
+                if (!warp_wait(&s.v_full[st], ph)) { ok = false; break; }
+                if (!warp_wait(&s.p_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t pa = tP + 32u * (j & 1);
-                const uint64_t vj = vd + (j % VS) * (kTaTileBytes / 16);
+                const uint64_t vj = vd + st * (kTaTileBytes / 16);
+                if (lead) {
 #pragma unroll
-                for (int kk = 0; kk < kTaKeys / 16; ++kk)
-                    umma_f16_tmem_a(tO, pa + 8 * kk, vj + 2048 * kk / 16, idO, first && kk == 0 ? 0u : 1u);
-                umma_commit(&s.v_empty[j % VS]);
-                umma_commit(&s.o_done[j & 1]);  // last: the rows end the CTA when they have seen it
-                return true;
-            };
-            bool first_pv = true;
-            int ahead = tiles_ahead();  // of the unit: tiles whose S is not issued yet
-            const bool any = ahead > 0;  // (a short range may lie in a unit's beginning)
-            bool ok = !any || qk(0, true);
-            --ahead;
-            for (uint32_t j = 0; ok && any; ++j) {
-                const bool cut = ahead == 0;  // tile j ends its unit
-                if (cut) {
-                    umma_commit(&s.q_empty);  // (after its last S)
-                    c.next(a);
-                    ahead = tiles_ahead();
+                    for (int kk = 0; kk < kTaKeys / 16; ++kk)
+                        umma_f16_tmem_a(tO, pa + 8 * kk, vj + 2048 * kk / 16, idO, i == 0 && kk == 0 ? 0u : 1u);
+                    umma_commit(&s.v_empty[st]);
+                    umma_commit(&s.o_done[j & 1]);  // last: the rows end the CTA when they have seen it
                 }
-                const bool more = ahead > 0;
-                // S(j+1) takes the place of S(j) as soon as the rows have it in registers
-                if (more && !ta_wait(&s.s_free, j & 1, &s.fail)) { ok = false; break; }
-                if (more && !cut) {
-                    if (!qk(j + 1, false)) { ok = false; break; }
-                    --ahead;
-                }
-                if (!pv(j, first_pv)) { ok = false; break; }
-                if (!more) break;
-                first_pv = cut;
-                if (cut) {  // a new unit's Q arrives after the old unit's last S: its first S comes after PV
-                    if (!qk(j + 1, true)) { ok = false; break; }
-                    --ahead;
+                __syncwarp();
+                if (++st == VS) {
+                    st = 0;
+                    ph ^= 1;
                 }
             }
-            if (!ok) {
-                s.fail = 1;
-                umma_commit(&s.drain);  // every MMA issued so far completes before the CTA exits
-                (void)mbar_wait(&s.drain, 0);
-            }
+            c.next(a);
+        }
+        if (!ok) {
+            s.fail = 1;
+            if (lead) umma_commit(&s.drain[1]);
+            (void)mbar_wait(&s.drain[1], 0);
         }
         __syncwarp();
     } else if (warp < 4 && work) {
@@ -493,9 +501,6 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         int slot_no = 0, tree_units = 0;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {  // one answer for the warp
-            return __all_sync(0xffffffffu, ta_wait(bar, parity, &s.fail));
-        };
         while (ok && c.left > 0) {
             const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
             int t0;
@@ -588,23 +593,25 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     const float nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every p is 2^-inf = 0
                     const uint64_t scale2 = ta_f2(kTaScaleLog2, kTaScaleLog2), nm2 = ta_f2(nm, nm);
                     uint64_t ls[2] = {0, 0};
-                    uint32_t pk[kTaKeys / 2];
+                    // P, once PV(j-2) has read the buffer
+                    if (j >= 2 && !warp_wait(&s.o_done[j & 1], ((j >> 1) - 1) & 1)) { ok = false; break; }
 #pragma unroll
-                    for (int q = 0; q < kTaKeys; q += 2) {
-                        float p0, p1;
-                        ta_split(ta_fma2(ta_f2(x[q], x[q + 1]), scale2, nm2), p0, p1);
-                        p0 = ta_ex2(p0);
-                        p1 = ta_ex2(p1);
-                        ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(p0, p1));
-                        pk[q / 2] = ta_pack(p0, p1);
+                    for (int q0 = 0; q0 < kTaKeys; q0 += 32) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int q = 0; q < 32; q += 2) {
+                            float p0, p1;
+                            ta_split(ta_fma2(ta_f2(x[q0 + q], x[q0 + q + 1]), scale2, nm2), p0, p1);
+                            p0 = ta_ex2(p0);
+                            p1 = ta_ex2(p1);
+                            ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(p0, p1));
+                            pk[q / 2] = ta_pack(p0, p1);
+                        }
+                        tmem_st16(tP + 32u * (j & 1) + lane_off + q0 / 2, pk);
                     }
                     float l0, l1;
                     ta_split(ta_add2(ls[0], ls[1]), l0, l1);
                     l += l0 + l1;
-                    // P, once PV(j-2) has read the buffer
-                    if (j >= 2 && !warp_wait(&s.o_done[j & 1], ((j >> 1) - 1) & 1)) { ok = false; break; }
-#pragma unroll
-                    for (int q = 0; q < kTaKeys / 2; q += 16) tmem_st16(tP + 32u * (j & 1) + lane_off + q, pk + q);
                     tmem_st_wait();
                     tc_fence_before();
                 } else if (lane == 0) {
