@@ -275,7 +275,27 @@ LLMDIY_DEV float ta_max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+LLMDIY_DEV float ta_ex2v(float x) {  // as ta_ex2, issued where it stands
+    float y;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 constexpr float kTaScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
+
+// add[e] += p v[dim0 + e] of the tree rows base + bit that `hit` names, for one query row (out of line: rare).
+__device__ __noinline__ void ta_add_bad(const TaArgs& a, uint64_t hit, int b, int node, int base, int kvh, int h,
+                                        int dim0, float nm, float* add) {
+    for (; hit; hit &= hit - 1) {
+        const int kn = base + __ffsll((long long)hit) - 1;
+        const half* kr = a.TK + (((size_t)b * a.N + kn) * a.KV + kvh) * kTaDim;
+        const half* vr = a.TV + (((size_t)b * a.N + kn) * a.KV + kvh) * kTaDim;
+        const half* qr = a.Q + ((size_t)b * a.N + node) * a.ldq + h * kTaDim;
+        float d = 0.f;
+        for (int e = 0; e < kTaDim; ++e) d = __fmaf_rn(h2f(qr[e]), h2f(kr[e]), d);
+        const float p = ta_ex2(__fmaf_rn(d, kTaScaleLog2, nm));
+        for (int e = 0; e < 32; ++e) add[e] = __fmaf_rn(p, h2f(vr[dim0 + e]), add[e]);
+    }
+}
 
 template <int QR, int KS, int VS, bool DIRECT>
 __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
@@ -380,7 +400,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                 const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
                 int t0;
                 const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(t0);
-                if (cnt <= 0) {
+                if (!DIRECT && cnt <= 0) {
                     c.next(a);
                     continue;
                 }
@@ -406,6 +426,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     // tile is under way by then
                     if (t == t0 && !first_unit && !load_q()) { ok = false; break; }
                 }
+                if (DIRECT) break;
                 if (ok) c.next(a);
             }
             // the last copies land in this CTA's shared memory: they have before it exits, whatever happens
@@ -448,6 +469,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     ph ^= 1;
                 }
             }
+            if (DIRECT) break;
             c.next(a);
         }
         if (!ok) {
@@ -485,6 +507,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     ph ^= 1;
                 }
             }
+            if (DIRECT) break;
             c.next(a);
         }
         if (!ok) {
@@ -505,7 +528,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
             int t0;
             const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(t0);
-            if (cnt <= 0) {
+            if (!DIRECT && cnt <= 0) {
                 c.next(a);
                 slot_no = 1;
                 continue;
@@ -515,19 +538,21 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             const bool warp_live = warp * 32 < min(a.rows, (c.n - m0) * G);
             const uint64_t* mrow = a.mask + ((size_t)c.b * a.N + (live ? node : 0)) * words;
             const int tt0 = max(t0 - tc, 0);  // first tree tile of this segment, if any
+            const int plain = c.L / kTaKeys;  // the tiles before this one are full cache tiles
             uint64_t word = live && t0 + cnt > tc ? mrow[tt0] : 0;
             m = -INFINITY;
             l = 0.f;
             for (int t = t0; t < t0 + cnt; ++t, ++j) {
-                const bool tree = t >= tc;
-                const int tt = t - tc;
-                const int nv = tree ? min(kTaKeys, c.n - tt * kTaKeys) : min(kTaKeys, c.L - t * kTaKeys);
-                uint64_t seen = nv == 64 ? ~0ull : (1ull << nv) - 1;
-                if (tree) {
-                    seen &= word;
-                    if (live && t + 1 < t0 + cnt) word = mrow[tt + 1];
-                }
-                if (tree || nv < kTaKeys) {
+                uint64_t seen = ~0ull;
+                if (__builtin_expect(t >= plain, 0)) {
+                    const bool tree = t >= tc;
+                    const int tt = t - tc;
+                    const int nv = tree ? min(kTaKeys, c.n - tt * kTaKeys) : min(kTaKeys, c.L - t * kTaKeys);
+                    if (nv < kTaKeys) seen = (1ull << nv) - 1;
+                    if (tree) {
+                        seen &= word;
+                        if (live && t + 1 < t0 + cnt) word = mrow[tt + 1];
+                    }
                     // V rows that must not enter the product: past the end, or (tree) not finite
                     if (!warp_wait(&s.v_full[j % VS], (j / VS) & 1)) { ok = false; break; }
                     // (this warp's 16 rows; a row is two runs of eight 16-byte pieces)
@@ -558,7 +583,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     tmem_ld_wait();
                     tc_fence_before();
                     if (lane == 0) mbar_arrive(&s.s_free);
-                    if (tree || nv < kTaKeys) {
+                    if (__builtin_expect(t >= plain, 0)) {
                         const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
 #pragma unroll
                         for (int q = 0; q < kTaKeys; ++q)
@@ -572,7 +597,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     const float top = ta_max3(ta_max3(mx[0], x[60], x[61]), ta_max3(mx[1], x[62], x[63]),
                                               fmaxf(mx[2], mx[3])) * kTaScaleLog2;
                     const bool grow = live && top > m + (t == t0 ? 0.f : 8.f);  // (a NaN maximum leaves m)
-                    if (t != t0 && __any_sync(0xffffffffu, grow)) {
+                    if (__builtin_expect(t != t0 && __any_sync(0xffffffffu, grow), 0)) {
                         // rescale O, complete through PV(j-1) (the whole warp: TMEM moves 32 rows at a time)
                         if (!warp_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) { ok = false; break; }
                         tc_fence_after();
@@ -595,20 +620,38 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     uint64_t ls[2] = {0, 0};
                     // P, once PV(j-2) has read the buffer
                     if (j >= 2 && !warp_wait(&s.o_done[j & 1], ((j >> 1) - 1) & 1)) { ok = false; break; }
+                    // Sixteen keys at a time, the exponentials of one group ahead of the sums and the rounding of the
+                    // last (in this order: a sum right behind its exponentials waits for them)
+                    float e[2][16];
+                    uint32_t pk[16];
+                    auto exps = [&](int q0) {
+                        float* to = e[(q0 >> 4) & 1];
 #pragma unroll
-                    for (int q0 = 0; q0 < kTaKeys; q0 += 32) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int q = 0; q < 32; q += 2) {
-                            float p0, p1;
-                            ta_split(ta_fma2(ta_f2(x[q0 + q], x[q0 + q + 1]), scale2, nm2), p0, p1);
-                            p0 = ta_ex2(p0);
-                            p1 = ta_ex2(p1);
-                            ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(p0, p1));
-                            pk[q / 2] = ta_pack(p0, p1);
+                        for (int q = 0; q < 16; q += 2) {
+                            float a0, a1;
+                            ta_split(ta_fma2(ta_f2(x[q0 + q], x[q0 + q + 1]), scale2, nm2), a0, a1);
+                            to[q] = ta_ex2v(a0);
+                            to[q + 1] = ta_ex2v(a1);
                         }
-                        tmem_st16(tP + 32u * (j & 1) + lane_off + q0 / 2, pk);
-                    }
+                    };
+                    auto take = [&](int q0) {
+                        const float* from = e[(q0 >> 4) & 1];
+#pragma unroll
+                        for (int q = 0; q < 16; q += 2) {
+                            ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(from[q], from[q + 1]));
+                            pk[((q0 & 16) + q) / 2] = ta_pack(from[q], from[q + 1]);
+                        }
+                    };
+                    exps(0);
+                    exps(16);
+                    take(0);
+                    exps(32);
+                    take(16);
+                    tmem_st16(tP + 32u * (j & 1) + lane_off, pk);
+                    exps(48);
+                    take(32);
+                    take(48);
+                    tmem_st16(tP + 32u * (j & 1) + lane_off + 16, pk);
                     float l0, l1;
                     ta_split(ta_add2(ls[0], ls[1]), l0, l1);
                     l += l0 + l1;
@@ -645,22 +688,13 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     tmem_ld16(tO + lane_off + q, reinterpret_cast<uint32_t*>(v));
                     tmem_ld16(tO + lane_off + q + 16, reinterpret_cast<uint32_t*>(v + 16));
                     tmem_ld_wait();
-                    if (any_bad && live) {
-                        for (int tt = tt0; tt < t0 + cnt - tc; ++tt) {
-                            uint64_t hit = *reinterpret_cast<volatile uint64_t*>(s.bad[tree_units & 1][tt]);
-                            hit &= mrow[tt];
-                            for (; hit; hit &= hit - 1) {
-                                const int kn = tt * 64 + __ffsll((long long)hit) - 1;
-                                const half* kr = a.TK + (((size_t)c.b * a.N + kn) * a.KV + kvh) * kTaDim;
-                                const half* vr = a.TV + (((size_t)c.b * a.N + kn) * a.KV + kvh) * kTaDim;
-                                const half* qr = a.Q + ((size_t)c.b * a.N + node) * a.ldq + (kvh * G + g) * kTaDim;
-                                float d = 0.f;
-                                for (int e = 0; e < kTaDim; ++e) d = __fmaf_rn(h2f(qr[e]), h2f(kr[e]), d);
-                                const float p = ta_ex2(__fmaf_rn(d, kTaScaleLog2, m == -INFINITY ? 0.f : -m));
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __fmaf_rn(p, h2f(vr[q + e]), v[e]);
-                            }
-                        }
+                    if (__builtin_expect(any_bad && live, 0)) {
+                        float add[32];
+                        for (int e = 0; e < 32; ++e) add[e] = 0.f;
+                        for (int tt = tt0; tt < t0 + cnt - tc; ++tt)
+                            ta_add_bad(a, *reinterpret_cast<volatile uint64_t*>(s.bad[tree_units & 1][tt]) & mrow[tt], c.b, node,
+                                       tt * 64, kvh, kvh * G + g, q, m == -INFINITY ? 0.f : -m, add);
+                        for (int e = 0; e < 32; ++e) v[e] += add[e];
                     }
                     if (!live) continue;
                     if (whole) {
@@ -683,6 +717,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             tc_fence_before();  // O has been read: the next unit's first PV may overwrite it
             if (any_tree) ++tree_units;
             slot_no = 1;
+            if (DIRECT) break;
             c.next(a);
         }
         if (!ok) s.fail = 1;
@@ -831,7 +866,8 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     p.W = (int)std::min<long long>(slots, units * tiles);
     p.floats = (size_t)p.W * 2 * p.rows * (kTaDim + 2);
     int c = 1;
-    while (c < kTaMaxCluster && 2 * c * units <= slots && 2 * c <= tiles) c *= 2;
+    const int tf = getenv("TF") ? atoi(getenv("TF")) : 1;
+    while (c < kTaMaxCluster && 2 * c * units <= (long long)slots * tf && 2 * c <= tiles) c *= 2;
     const char* env = getenv("TD");
     const int lim = env ? atoi(env) : 8;
     if (getenv("TC")) c = std::min(c, atoi(getenv("TC")));
