@@ -85,7 +85,8 @@ struct TaArgs {
     int B, N, H, KV, ldq, ldo, slot_rows, num_slots, max_len;
     int rows;  // rows of a partial: G * nodes_per_tile
     int npt;   // nodes per M tile
-    int W;     // flat: most CTAs that share the tiles
+    int mt;    // M tiles of a kv head (of the longest tree)
+    int W;     // flat: most CTAs that share the tiles of one M tile
     int direct;
     int evict_first;
 };
@@ -98,12 +99,12 @@ LLMDIY_DEV int ta_len(const TaArgs& a, int b) {
     const int s = ta_slot(a, b);
     return s >= 0 && s < a.num_slots ? min(max(a.len[b], 0), a.max_len) : 0;
 }
-// Tiles of a unit of sequence b, and its units.
+// Tiles of a unit of sequence b, and its units of one M tile (its kv heads).
 LLMDIY_DEV void ta_shape(const TaArgs& a, int b, int& n, int& L, int& tiles, int& units) {
     n = ta_nodes(a, b);
     L = n ? ta_len(a, b) : 0;
     tiles = (L + kTaKeys - 1) / kTaKeys + (n + kTaKeys - 1) / kTaKeys;
-    units = a.KV * ((n + a.npt - 1) / a.npt);
+    units = n ? a.KV : 0;
 }
 
 // Flat positions: a unit takes kTaUnitCost + tiles of them, the first kTaUnitCost without a tile.  W CTAs:
@@ -124,7 +125,7 @@ struct TaDeal {
 // A unit, and what is left of a CTA's range from position `at` of it on.
 struct TaCursor {
     int b, n, L, tiles, units;  // sequence and its shape
-    int unit;                   // within the sequence: kv head * M tiles + M tile
+    int unit;                   // within the sequence: kv head
     int at;                     // flat position within the unit
     int left;                   // positions left of this CTA's range
     int row0;                   // first cache row of the sequence's slot (set by the producer)
@@ -342,24 +343,29 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     TaCursor c;
     c.left = 0;
     const int C = DIRECT ? (int)gridDim.x : 1, rank = DIRECT ? (int)blockIdx.x : 0;  // the unit's cluster
+    // Flat: the M tiles of a kv head go to neighbouring CTAs at the same tiles, so that the second one to read a K/V
+    // tile finds it in L2.
+    const int mtile = DIRECT ? (int)blockIdx.y % a.mt : (int)blockIdx.x % a.mt, m0 = mtile * a.npt;
     if (DIRECT) {
         c.b = blockIdx.z;
-        c.unit = blockIdx.y;
+        c.unit = blockIdx.y / a.mt;
         ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
-        if (c.unit < c.units) {
+        if (m0 < c.n) {
             const int t0 = c.tiles * rank / C, t1 = c.tiles * (rank + 1) / C;
             c.at = kTaUnitCost + t0;
             c.left = t1 - t0;
         }
     } else {
         const TaDeal deal(ta_total(a, lane), a.W);
-        if ((int)blockIdx.x < deal.W) {
-            const int f = deal.start(blockIdx.x);
-            c.left = deal.start(blockIdx.x + 1) - f;
+        const int w = blockIdx.x / a.mt;
+        if (w < deal.W) {
+            const int f = deal.start(w);
+            c.left = deal.start(w + 1) - f;
             (void)ta_locate(a, f, lane, c);
         }
     }
     const bool work = c.left > 0;
+    auto seg = [&](int& t0) { return m0 < c.n ? c.seg(t0) : 0; };  // (a tree may end before this M tile)
     auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {  // one answer for the warp
         return __all_sync(0xffffffffu, ta_wait(bar, parity, &s.fail));
     };
@@ -397,9 +403,9 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                 }
             };
             while (ok && c.left > 0) {
-                const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+                const int kvh = c.unit;
                 int t0;
-                const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(t0);
+                const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = seg(t0);
                 if (!DIRECT && cnt <= 0) {
                     c.next(a);
                     continue;
@@ -446,7 +452,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         bool ok = true;
         while (ok && c.left > 0) {
             int t0;
-            const int cnt = c.seg(t0);
+            const int cnt = seg(t0);
             for (int i = 0; i < cnt; ++i, ++j) {
                 if (i == 0 && !warp_wait(&s.q_full, unit_no++ & 1)) { ok = false; break; }
                 // S(j) takes the place of S(j-1) as soon as the rows have that in registers
@@ -487,7 +493,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         bool ok = true;
         while (ok && c.left > 0) {
             int t0;
-            const int cnt = c.seg(t0);
+            const int cnt = seg(t0);
             for (int i = 0; i < cnt; ++i, ++j) {
                 if (!warp_wait(&s.v_full[st], ph)) { ok = false; break; }
                 if (!warp_wait(&s.p_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
@@ -525,9 +531,9 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         while (ok && c.left > 0) {
-            const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+            const int kvh = c.unit;
             int t0;
-            const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = c.seg(t0);
+            const int tc = (c.L + kTaKeys - 1) / kTaKeys, cnt = seg(t0);
             if (!DIRECT && cnt <= 0) {
                 c.next(a);
                 slot_no = 1;
@@ -712,7 +718,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     }
                 }
                 if (live && !whole && !DIRECT)
-                    *reinterpret_cast<float2*>(a.part + (size_t)a.W * 2 * a.rows * kTaDim + at * 2) = make_float2(m, l);
+                    *reinterpret_cast<float2*>(a.part + (size_t)a.W * a.mt * 2 * a.rows * kTaDim + at * 2) = make_float2(m, l);
             }
             tc_fence_before();  // O has been read: the next unit's first PV may overwrite it
             if (any_tree) ++tree_units;
@@ -728,8 +734,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     if (DIRECT && C > 1) {
         // ---------------- the cluster's parts of the unit's rows row r by CTA r C / rows
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (c.unit < c.units) {
-            const int mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+        if (m0 < c.n) {
+            const int kvh = c.unit;
             const int live = min(a.rows, (c.n - m0) * G), r1 = live * (rank + 1) / C;
             const uint32_t ml = smem_u32(s.q[0]), oo = smem_u32(s.k[0][0]);
             for (int r = live * rank / C + warp; r < r1; r += kTaThreads / 32) {
@@ -774,7 +780,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
 constexpr int kTaMergeWarps = 8;
 
 __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_constant__ TaArgs a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = blockIdx.x + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = blockIdx.x / a.mt + 1, m0 = blockIdx.x % a.mt * a.npt;
     const TaDeal deal(ta_total(a, lane), a.W);
     TaCursor c;
     int f0 = 0;
@@ -783,18 +789,21 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
     // every thread waits for the attention kernel, also where there is nothing to join: this grid
     // must not be over before that one is
     pdl_wait();
-    if (!cut || c.at <= kTaUnitCost) return;  // no tile of the unit before the cut
+    if (!cut || c.at <= kTaUnitCost || m0 >= c.n) return;  // no tile of the unit before the cut
     const int w0 = deal.owner(f0 + kTaUnitCost), w1 = deal.owner(f0 + kTaUnitCost + c.tiles - 1);
     // the first CTA's part of this unit is its first segment only when its range does not start before the unit
-    const int first = w0 * 2 + (deal.start(w0) >= f0 ? 0 : 1);
-    const int G = a.H / a.KV, mt = c.units / a.KV, kvh = c.unit / mt, m0 = (c.unit - kvh * mt) * a.npt;
+    const int mtile = blockIdx.x % a.mt;
+    auto part = [&](int k) {  // the part of CTA (k, mtile)
+        return (k * a.mt + mtile) * 2 + (k == w0 && deal.start(w0) < f0 ? 1 : 0);
+    };
+    const int G = a.H / a.KV, kvh = c.unit;
     const int live = min(a.rows, (c.n - m0) * G), share = w - w0 - 1, shares = w1 - w0;
     const int r1 = live * (share + 1) / shares;
-    const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.W * 2 * a.rows * kTaDim);
+    const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.W * a.mt * 2 * a.rows * kTaDim);
     for (int r = live * share / shares + warp; r < r1; r += kTaMergeWarps) {
         float M = -INFINITY;
         for (int k = w0 + lane; k <= w1; k += 32)
-            M = fmaxf(M, __ldcg(ml + (size_t)(k == w0 ? first : k * 2) * a.rows + r).x);
+            M = fmaxf(M, __ldcg(ml + (size_t)part(k) * a.rows + r).x);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         float Ls = 0.f;
@@ -803,7 +812,7 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
             float f = 0.f;
             if (c0 + lane <= w1) {
                 const int k = c0 + lane;
-                const float2 y = __ldcg(ml + (size_t)(k == w0 ? first : k * 2) * a.rows + r);
+                const float2 y = __ldcg(ml + (size_t)part(k) * a.rows + r);
                 // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
                 f = y.x == -INFINITY ? (y.y == y.y ? 0.f : 1.f) : exp2f(y.x - M);
                 Ls += y.y * f;
@@ -814,7 +823,7 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
                 const int k = c0 + i;
                 const float fk = __shfl_sync(0xffffffffu, f, i);
                 const float4 y = __ldcg(reinterpret_cast<const float4*>(
-                    a.part + ((size_t)(k == w0 ? first : k * 2) * a.rows + r) * kTaDim) + lane);
+                    a.part + ((size_t)part(k) * a.rows + r) * kTaDim) + lane);
                 acc.x = __fmaf_rn(fk, y.x, acc.x);
                 acc.y = __fmaf_rn(fk, y.y, acc.y);
                 acc.z = __fmaf_rn(fk, y.z, acc.z);
@@ -842,7 +851,7 @@ int ta_sms() {
 }
 
 struct TaPlan {
-    int G, npt, rows, mt, W;
+    int G, npt, rows, mt, W;  // W: flat CTAs per M tile
     int cluster;  // direct: CTAs per unit (0: flat)
     bool ok;
     size_t floats;  // of the flat partials
@@ -862,9 +871,9 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     const long long tiles = ((long long)max_len + kTaKeys - 1) / kTaKeys + (N + kTaKeys - 1) / kTaKeys;
     const long long units = (long long)B * KV * p.mt;
     p.ok = units * (tiles + kTaUnitCost) <= 0x7fffffffLL;
-    const int slots = kTaCtasPerSm * ta_sms();
-    p.W = (int)std::min<long long>(slots, units * tiles);
-    p.floats = (size_t)p.W * 2 * p.rows * (kTaDim + 2);
+    const int slots = std::max(kTaCtasPerSm * ta_sms(), p.mt);
+    p.W = (int)std::min<long long>(slots / p.mt, units / p.mt * tiles);
+    p.floats = (size_t)std::min<long long>(slots, units * tiles) * 2 * p.rows * (kTaDim + 2);
     int c = 1;
     const int tf = getenv("TF") ? atoi(getenv("TF")) : 1;
     while (c < kTaMaxCluster && 2 * c * units <= (long long)slots * tf && 2 * c <= tiles) c *= 2;
@@ -979,12 +988,13 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     a.max_len = max_len;
     a.rows = p.rows;
     a.npt = p.npt;
+    a.mt = p.mt;
     a.W = p.W;
     a.evict_first = p.npt >= N;  // one M tile: every K/V row is read once
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int* err = reinterpret_cast<int*>(work);
     a.direct = p.cluster > 0;
-    const dim3 grid = a.direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W);
+    const dim3 grid = a.direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W * p.mt);
     const int cluster = std::max(1, p.cluster);
     int rc = p.rows <= 64 ? a.direct ? ta_launch<64, 3, 3, true>(m, a, err, grid, cluster, st)
                                      : ta_launch<64, 3, 3, false>(m, a, err, grid, cluster, st)
@@ -992,7 +1002,7 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
                           : ta_launch<128, 3, 2, false>(m, a, err, grid, cluster, st);
     if (rc || a.direct || p.W < 2) return rc;
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3(p.W - 1);
+    lc.gridDim = dim3((p.W - 1) * p.mt);
     lc.blockDim = dim3(kTaMergeWarps * 32);
     lc.stream = st;
     cudaLaunchAttribute at[1];
