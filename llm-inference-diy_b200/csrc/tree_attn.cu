@@ -35,7 +35,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 #include <mutex>
 
 #include "gemm_tc_host.h"
@@ -54,6 +53,7 @@ constexpr int kTaThreads = 224;  // warps 0-3: rows; warp 4: TMA; warps 5 and 6:
 constexpr int kTaCtasPerSm = 2;
 constexpr int kTaTileBytes = kTaKeys * kTaDim * 2;  // one K or V tile
 constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0 | P1 (32 each) | O (128)
+constexpr int kTaDirectTiles = 48;  // (see ta_plan)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
 constexpr int kTaMaxCluster = 8;  // (clusters of 16 do not all run at once: 16 x 16 CTAs took 24.6 us, 16 x 8 13.7)
 constexpr int kTaUnitCost = 4;  // a unit's beginning and end take about as long as four tiles
@@ -775,9 +775,10 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
 }
 
 // Flat: joins the partials of the units that were cut.  Block w - 1 looks at the cut before CTA w: if it
-// parts a unit's tiles, the blocks of that unit's cuts share its rows, a warp per row: lane s weighs partial
-// s, then each lane sums 4 dims over the partials in order.
-constexpr int kTaMergeWarps = 8;
+// parts a unit's tiles, the blocks of that unit's cuts share its rows, two rows to a warp and eight partials' loads
+// in flight (with a warp per row, one row after the other, joining 64-row units took 20 us): of a row's sixteen
+// lanes, lane i weighs partials i, i + 16, .., then each sums 8 dims over the partials in order.
+constexpr int kTaMergeWarps = 16;
 
 __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_constant__ TaArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = blockIdx.x / a.mt + 1, m0 = blockIdx.x % a.mt * a.npt;
@@ -793,47 +794,53 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
     const int w0 = deal.owner(f0 + kTaUnitCost), w1 = deal.owner(f0 + kTaUnitCost + c.tiles - 1);
     // the first CTA's part of this unit is its first segment only when its range does not start before the unit
     const int mtile = blockIdx.x % a.mt;
-    auto part = [&](int k) {  // the part of CTA (k, mtile)
-        return (k * a.mt + mtile) * 2 + (k == w0 && deal.start(w0) < f0 ? 1 : 0);
-    };
+    const int later = deal.start(w0) < f0 ? 1 : 0;
+    auto part = [&](int k) { return (k * a.mt + mtile) * 2 + (k == w0 ? later : 0); };  // of CTA (k, mtile)
     const int G = a.H / a.KV, kvh = c.unit;
     const int live = min(a.rows, (c.n - m0) * G), share = w - w0 - 1, shares = w1 - w0;
     const int r1 = live * (share + 1) / shares;
     const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.W * a.mt * 2 * a.rows * kTaDim);
-    for (int r = live * share / shares + warp; r < r1; r += kTaMergeWarps) {
+    const int gl = lane & 15;
+    for (int q = live * share / shares + warp * 2; q < r1; q += kTaMergeWarps * 2) {
+        const int r = min(q + (lane >> 4), r1 - 1);  // (lanes past the share repeat its last row)
         float M = -INFINITY;
-        for (int k = w0 + lane; k <= w1; k += 32)
-            M = fmaxf(M, __ldcg(ml + (size_t)part(k) * a.rows + r).x);
+        for (int k = w0 + gl; k <= w1; k += 16) M = fmaxf(M, __ldcg(ml + (size_t)part(k) * a.rows + r).x);
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int o = 8; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         float Ls = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c0 = w0; c0 <= w1; c0 += 32) {
+        float4 acc[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c0 = w0; c0 <= w1; c0 += 16) {
             float f = 0.f;
-            if (c0 + lane <= w1) {
-                const int k = c0 + lane;
-                const float2 y = __ldcg(ml + (size_t)part(k) * a.rows + r);
+            if (c0 + gl <= w1) {
+                const float2 y = __ldcg(ml + (size_t)part(c0 + gl) * a.rows + r);
                 // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
                 f = y.x == -INFINITY ? (y.y == y.y ? 0.f : 1.f) : exp2f(y.x - M);
                 Ls += y.y * f;
             }
-            const int cnt = min(32, w1 - c0 + 1);
-#pragma unroll 4
+            const int cnt = min(16, w1 - c0 + 1);
+#pragma unroll 8
             for (int i = 0; i < cnt; ++i) {
-                const int k = c0 + i;
-                const float fk = __shfl_sync(0xffffffffu, f, i);
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(
-                    a.part + ((size_t)part(k) * a.rows + r) * kTaDim) + lane);
-                acc.x = __fmaf_rn(fk, y.x, acc.x);
-                acc.y = __fmaf_rn(fk, y.y, acc.y);
-                acc.z = __fmaf_rn(fk, y.z, acc.z);
-                acc.w = __fmaf_rn(fk, y.w, acc.w);
+                const float fk = __shfl_sync(0xffffffffu, f, i, 16);
+                const float4* src = reinterpret_cast<const float4*>(a.part + ((size_t)part(c0 + i) * a.rows + r) * kTaDim) + gl;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float4 y = __ldcg(src + 16 * e);
+                    acc[e].x = __fmaf_rn(fk, y.x, acc[e].x);
+                    acc[e].y = __fmaf_rn(fk, y.y, acc[e].y);
+                    acc[e].z = __fmaf_rn(fk, y.z, acc[e].z);
+                    acc[e].w = __fmaf_rn(fk, y.w, acc[e].w);
+                }
             }
         }
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
+        for (int o = 8; o >= 1; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
         const int node = m0 + r / G, h = kvh * G + r - (r / G) * G;
-        ta_store4(a.O + ((size_t)c.b * a.N + node) * a.ldo + h * kTaDim + lane * 4, acc, Ls == 0.f ? 0.f : 1.f / Ls);
+        half* dst = a.O + ((size_t)c.b * a.N + node) * a.ldo + h * kTaDim + gl * 4;
+        if (q + (lane >> 4) < r1)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) ta_store4(dst + 64 * e, acc[e], Ls == 0.f ? 0.f : 1.f / Ls);
     }
 }
 
@@ -872,15 +879,21 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     const long long units = (long long)B * KV * p.mt;
     p.ok = units * (tiles + kTaUnitCost) <= 0x7fffffffLL;
     const int slots = std::max(kTaCtasPerSm * ta_sms(), p.mt);
-    p.W = (int)std::min<long long>(slots / p.mt, units / p.mt * tiles);
+    // flat CTAs have four tiles or more
+    p.W = (int)std::max<long long>(1, std::min<long long>(slots / p.mt, units / p.mt * tiles / 4));
     p.floats = (size_t)std::min<long long>(slots, units * tiles) * 2 * p.rows * (kTaDim + 2);
-    int c = 1;
-    const int tf = getenv("TF") ? atoi(getenv("TF")) : 1;
-    while (c < kTaMaxCluster && 2 * c * units <= (long long)slots * tf && 2 * c <= tiles) c *= 2;
-    const char* env = getenv("TD");
-    const int lim = env ? atoi(env) : 8;
-    if (getenv("TC")) c = std::min(c, atoi(getenv("TC")));
-    if ((tiles + c - 1) / c <= lim) p.cluster = c;
+    // Direct or flat, by what both would take if every sequence were max_len long, in us.  A CTA that runs its chain of
+    // products undisturbed needs 0.75 a tile (1.0 with more than 32 rows), and all slots together 1.46 a tile and slot from
+    // HBM; a flat call pays for its second launch and for joining W / units partials a row.  Of sequences
+    // of different lengths direct waits for the longest, so several of them with more than
+    // kTaDirectTiles tiles a CTA go flat.  Measured (direct / flat): 16 units of 17 tiles 9.9 / 17.4, 16 of 2049 203 / 184,
+    // 16 of 514 (128 rows) 78 / 68, 2 of 126 20 / 59, 1024 of up to 33 103 / 122, 256 of up to 66 67 / 67.
+    const int c = (int)std::max<long long>(1, std::min<long long>({kTaMaxCluster, slots / units, tiles}));
+    const double t = (double)((tiles + c - 1) / c), chain = p.rows > 32 ? 1.0 : 0.75, hbm = 1.46 / slots;
+    const double flat_ctas = (double)p.W * p.mt;
+    const double direct_us = 9.0 + t * std::max(chain, hbm * std::min<double>(slots, units * c));
+    const double flat_us = 20.0 + units * tiles / flat_ctas * std::max(chain, hbm * flat_ctas) + 0.12 * flat_ctas / units;
+    if (direct_us < flat_us && (B == 1 || t <= kTaDirectTiles)) p.cluster = c;
     return p;
 }
 

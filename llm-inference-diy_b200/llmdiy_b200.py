@@ -326,6 +326,7 @@ def transpose_weight(out, inp, rows, cols, stream=None):
 
 
 # ------------------------------------------- speculative decoding (llmdiy_tree.h)
+# (addresses go to ctypes as they are, ints or None: a step makes several of these calls per layer)
 def tree_layout(parent):
     """Host helper: (depth [n] int32, mask [n][ceil(n/64)] uint64) of one tree from its parents
     (parent[0] = -1, parent[i] < i).  Raises LlmdiyError for anything else or more than 256 nodes."""
@@ -340,8 +341,8 @@ def tree_layout(parent):
 
 def tree_rope(qkv, bias, depth, lens, tree_len, B, N, num_heads, num_kv_heads, rope_base, Q, TK, TV, stream=None):
     """Bias and rotary positions (len + depth) of a tree's rows: qkv -> Q and the tree's K/V rows TK, TV."""
-    _check(lib().llmdiy_tree_rope(_p(qkv), _p(bias), _p(depth), _p(lens), _p(tree_len), B, N, num_heads, num_kv_heads,
-                                  rope_base, _p(Q), _p(TK), _p(TV), _p(stream)), "tree_rope")
+    _check(lib().llmdiy_tree_rope(qkv, bias, depth, lens, tree_len, B, N, num_heads, num_kv_heads,
+                                  rope_base, Q, TK, TV, stream), "tree_rope")
 
 
 def tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len):
@@ -351,33 +352,33 @@ def tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len):
 def tree_attn(Q, ldq, K, V, stride, slot_rows, num_slots, slot, lens, max_len, TK, TV, mask, tree_len, B, N,
               num_heads, num_kv_heads, O, ldo, work, work_bytes, stream=None):
     """Attention of the tree's nodes over their sequences' cache rows and the tree rows their mask names."""
-    _check(lib().llmdiy_tree_attn(_p(Q), ldq, _p(K), _p(V), stride, slot_rows, num_slots, _p(slot), _p(lens), max_len,
-                                  _p(TK), _p(TV), _p(mask), _p(tree_len), B, N, num_heads, num_kv_heads, _p(O), ldo,
-                                  _p(work), work_bytes, _p(stream)), "tree_attn")
+    _check(lib().llmdiy_tree_attn(Q, ldq, K, V, stride, slot_rows, num_slots, slot, lens, max_len,
+                                  TK, TV, mask, tree_len, B, N, num_heads, num_kv_heads, O, ldo,
+                                  work, work_bytes, stream), "tree_attn")
 
 
 def tree_attn_status(work):
-    return lib().llmdiy_tree_attn_status(_p(work))
+    return lib().llmdiy_tree_attn_status(work)
 
 
 def softmax_rows(logits, ldl, temp, R, V, probs, ldp, stream=None):
     """probs[r] = softmax(logits[r] / temp[r]) in fp32 (temp None: 1; 0: equal shares of the largest entries)."""
-    _check(lib().llmdiy_softmax_rows(_p(logits), ldl, _p(temp), R, V, _p(probs), ldp, _p(stream)), "softmax_rows")
+    _check(lib().llmdiy_softmax_rows(logits, ldl, temp, R, V, probs, ldp, stream), "softmax_rows")
 
 
 def tree_verify(target, ldt, draft, ldd, token, parent, tree_len, uniform, B, N, V, path, accepted, next_token,
                 stream=None):
     """Accepted path, its length and the next token of each sequence's tree (draft None: deterministic drafts)."""
-    _check(lib().llmdiy_tree_verify(_p(target), ldt, _p(draft), ldd, _p(token), _p(parent), _p(tree_len), _p(uniform),
-                                    B, N, V, _p(path), _p(accepted), _p(next_token), _p(stream)), "tree_verify")
+    _check(lib().llmdiy_tree_verify(target, ldt, draft, ldd, token, parent, tree_len, uniform,
+                                    B, N, V, path, accepted, next_token, stream), "tree_verify")
 
 
 def tree_commit(TK, TV, tree_layer_stride, K, V, layer_stride, stride, slot_rows, num_slots, slot, lens, path,
                 accepted, B, N, num_kv_heads, layers, len_out, stream=None):
     """The root's and the accepted nodes' K/V rows of every layer into cache rows len, len + 1, ..."""
-    _check(lib().llmdiy_tree_commit(_p(TK), _p(TV), tree_layer_stride, _p(K), _p(V), layer_stride, stride, slot_rows,
-                                    num_slots, _p(slot), _p(lens), _p(path), _p(accepted), B, N, num_kv_heads, layers,
-                                    _p(len_out), _p(stream)), "tree_commit")
+    _check(lib().llmdiy_tree_commit(TK, TV, tree_layer_stride, K, V, layer_stride, stride, slot_rows,
+                                    num_slots, slot, lens, path, accepted, B, N, num_kv_heads, layers,
+                                    len_out, stream), "tree_commit")
 
 
 # ----------------------------------------------------------------- QWDF files
