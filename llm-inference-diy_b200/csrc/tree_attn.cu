@@ -52,7 +52,12 @@ constexpr int kTaRows = 128;     // query rows of a unit at most (MMA M)
 constexpr int kTaThreads = 224;  // warps 0-3: rows; warp 4: TMA; warps 5 and 6: the MMAs of S and of O
 constexpr int kTaCtasPerSm = 2;
 constexpr int kTaTileBytes = kTaKeys * kTaDim * 2;  // one K or V tile
-constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0 | P1 (32 each) | O (128)
+constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0 | P1, or P's two terms (32 each) | O (128)
+// Calls of up to this many query rows in all (sequences x nodes x heads) take P in two fp16 terms (p = hi + lo): the
+// rounding of a few rows' few large probabilities does not average out.  Of 16 rows over 1023 keys one term put
+// up to 3.3e-4 of the output's norm, two terms leave the output's own rounding, 2.1e-4; over more rows one term keeps to
+// 2.9e-4.  Two terms take 10.6 us there against 10.0, and 194 against 185 over 131072 keys.
+constexpr int kTaTwoTermRows = 128;
 constexpr int kTaDirectTiles = 48;  // (see ta_plan)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
 constexpr int kTaMaxCluster = 8;  // (clusters of 16 do not all run at once: 16 x 16 CTAs took 24.6 us, 16 x 8 13.7)
@@ -298,7 +303,7 @@ __device__ __noinline__ void ta_add_bad(const TaArgs& a, uint64_t hit, int b, in
     }
 }
 
-template <int QR, int KS, int VS, bool DIRECT>
+template <int QR, int KS, int VS, bool DIRECT, bool TWO>
 __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     tree_attn_k(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap ttk,
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         named_bar_arrive(1, kTaThreads);
     }
     if (!DIRECT) pdl_launch_dependents();  // the merge may be scheduled; it waits for this grid before it reads
-    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;  // P(j) at tP + 32 * (j & 1)
+    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;  // P(j) at tP + 32 * (j & 1), or (TWO) at tP, its low terms at tP + 32
 
     if (warp == 4 && work) {
         if (lane == 0) {
@@ -498,12 +503,17 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                 if (!warp_wait(&s.v_full[st], ph)) { ok = false; break; }
                 if (!warp_wait(&s.p_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t pa = tP + 32u * (j & 1);
+                const uint32_t pa = TWO ? tP : tP + 32u * (j & 1);
                 const uint64_t vj = vd + st * (kTaTileBytes / 16);
                 if (lead) {
 #pragma unroll
                     for (int kk = 0; kk < kTaKeys / 16; ++kk)
                         umma_f16_tmem_a(tO, pa + 8 * kk, vj + 2048 * kk / 16, idO, i == 0 && kk == 0 ? 0u : 1u);
+                    if (TWO) {
+#pragma unroll
+                        for (int kk = 0; kk < kTaKeys / 16; ++kk)
+                            umma_f16_tmem_a(tO, pa + 32 + 8 * kk, vj + 2048 * kk / 16, idO, 1u);
+                    }
                     umma_commit(&s.v_empty[st]);
                     umma_commit(&s.o_done[j & 1]);  // last: the rows end the CTA when they have seen it
                 }
@@ -624,8 +634,10 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     const float nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every p is 2^-inf = 0
                     const uint64_t scale2 = ta_f2(kTaScaleLog2, kTaScaleLog2), nm2 = ta_f2(nm, nm);
                     uint64_t ls[2] = {0, 0};
-                    // P, once PV(j-2) has read the buffer
-                    if (j >= 2 && !warp_wait(&s.o_done[j & 1], ((j >> 1) - 1) & 1)) { ok = false; break; }
+                    // P, once the product that read this buffer is complete
+                    constexpr uint32_t kBack = TWO ? 1 : 2;
+                    if (j >= kBack && !warp_wait(&s.o_done[(j - kBack) & 1], ((j - kBack) >> 1) & 1)) { ok = false; break; }
+                    const uint32_t pt = (TWO ? tP : tP + 32u * (j & 1)) + lane_off;
                     // Sixteen keys at a time, the exponentials of one group ahead of the sums and the rounding of the
                     // last (in this order: a sum right behind its exponentials waits for them)
                     float e[2][16];
@@ -645,7 +657,20 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
 #pragma unroll
                         for (int q = 0; q < 16; q += 2) {
                             ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(from[q], from[q + 1]));
-                            pk[((q0 & 16) + q) / 2] = ta_pack(from[q], from[q + 1]);
+                            const uint32_t hi = ta_pack(from[q], from[q + 1]);
+                            if (TWO) {  // eight words of each term
+                                const float2 f = __half22float2(*reinterpret_cast<const half2*>(&hi));
+                                pk[q / 2] = hi;
+                                pk[8 + q / 2] = ta_pack(from[q] - f.x, from[q + 1] - f.y);
+                            } else {
+                                pk[((q0 & 16) + q) / 2] = hi;
+                            }
+                        }
+                        if (TWO) {
+                            tmem_st8(pt + q0 / 2, pk);
+                            tmem_st8(pt + 32 + q0 / 2, pk + 8);
+                        } else if (q0 & 16) {
+                            tmem_st16(pt + (q0 - 16) / 2, pk);
                         }
                     };
                     exps(0);
@@ -653,11 +678,9 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     take(0);
                     exps(32);
                     take(16);
-                    tmem_st16(tP + 32u * (j & 1) + lane_off, pk);
                     exps(48);
                     take(32);
                     take(48);
-                    tmem_st16(tP + 32u * (j & 1) + lane_off + 16, pk);
                     float l0, l1;
                     ta_split(ta_add2(ls[0], ls[1]), l0, l1);
                     l += l0 + l1;
@@ -923,9 +946,9 @@ bool make_query_map(CUtensorMap* m, const void* base, int nodes, int H, int ldq,
 
 constexpr size_t kTaCtl = 4;  // floats before the partials: word 0 is the error word
 
-template <int QR, int KS, int VS, bool DIRECT>
+template <int QR, int KS, int VS, bool DIRECT, bool TWO>
 int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cluster, cudaStream_t st) {
-    auto kern = tree_attn_k<QR, KS, VS, DIRECT>;
+    auto kern = tree_attn_k<QR, KS, VS, DIRECT, TWO>;
     constexpr int bytes = (int)sizeof(TaSmem<QR, KS, VS>);
     static_assert(bytes <= 115712, "two CTAs share an SM");
     static_assert((KS + VS) * kTaTileBytes >= QR * kTaDim * 4, "a part's rows fit over K and V");
@@ -1009,10 +1032,16 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     a.direct = p.cluster > 0;
     const dim3 grid = a.direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W * p.mt);
     const int cluster = std::max(1, p.cluster);
-    int rc = p.rows <= 64 ? a.direct ? ta_launch<64, 3, 3, true>(m, a, err, grid, cluster, st)
-                                     : ta_launch<64, 3, 3, false>(m, a, err, grid, cluster, st)
-             : a.direct   ? ta_launch<128, 3, 2, true>(m, a, err, grid, cluster, st)
-                          : ta_launch<128, 3, 2, false>(m, a, err, grid, cluster, st);
+    int rc;
+    if (p.rows <= 64 && (long long)B * N * num_heads <= kTaTwoTermRows)
+        rc = a.direct ? ta_launch<64, 3, 3, true, true>(m, a, err, grid, cluster, st)
+                      : ta_launch<64, 3, 3, false, true>(m, a, err, grid, cluster, st);
+    else if (p.rows <= 64)
+        rc = a.direct ? ta_launch<64, 3, 3, true, false>(m, a, err, grid, cluster, st)
+                      : ta_launch<64, 3, 3, false, false>(m, a, err, grid, cluster, st);
+    else
+        rc = a.direct ? ta_launch<128, 3, 2, true, false>(m, a, err, grid, cluster, st)
+                      : ta_launch<128, 3, 2, false, false>(m, a, err, grid, cluster, st);
     if (rc || a.direct || p.W < 2) return rc;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((p.W - 1) * p.mt);
