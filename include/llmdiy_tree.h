@@ -14,8 +14,8 @@
  * The tree.  Sequence b (0 <= b < B) has nodes 0 .. tree_len[b]-1 (tree_len NULL: N each; values
  * are clamped to 0..N), N <= 256.  Node 0 is the root: the last token of the sequence, whose K/V
  * rows are not in the cache yet.  parent[b][i] < i is the node that node i continues (-1 for the root).
- * Arrays over nodes are [B][N]; what belongs to nodes at or past tree_len[b] is not read
- * and, in the outputs of tree_rope and tree_attn, left as it was.
+ * Arrays over nodes are [B][N]; what belongs to nodes at or past tree_len[b] has no
+ * effect and, in the outputs of tree_rope and tree_attn, is left as it was.
  *
  * The cache.  The batch's layout (llmdiy_batch.h): row r of kv head h of slot s is at
  * (s * slot_rows + r) * stride + h * 128 elements, in K and in V; sequence b uses slot[b] (NULL: slot

@@ -28,57 +28,69 @@ LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
 // ---------------------------------------------------------------- bias + RoPE
 // One CTA per node.  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
 // to [-pi, pi] in 64 bits (a position of 10^5 leaves fp32 angles only 2 digits after the point), its sine
-// and cosine are then taken in fp32 (absolute error < 2^-21, against 2^-11 of the fp16 outputs).
-__global__ void __launch_bounds__(256)
+// and cosine are then taken in fp32 (absolute error < 2^-21, against 2^-11 of the fp16 outputs).  The 64
+// frequencies come as a kernel argument, and the first rows' loads are under way while the angles are computed.
+struct RopeFreqs {
+    double f[kDim / 2];
+};
+constexpr int kRopeThreads = 256;
+
+__global__ void __launch_bounds__(kRopeThreads)
     tree_rope_k(const half* __restrict__ qkv, const half* __restrict__ bias, const int* __restrict__ depth,
-                const int* __restrict__ len, const int* __restrict__ tree_len, int N, int H, int KV, double log2_base,
-                half* __restrict__ Q, half* __restrict__ TK, half* __restrict__ TV) {
+                const int* __restrict__ len, const int* __restrict__ tree_len, int N, int H, int KV,
+                const __grid_constant__ RopeFreqs freqs, half* __restrict__ Q, half* __restrict__ TK,
+                half* __restrict__ TV) {
     __shared__ float cs[kDim / 2], sn[kDim / 2];
     const int b = blockIdx.y, i = blockIdx.x, tid = threadIdx.x;
-    if (i >= nodes_of(tree_len, b, N)) return;
     const size_t row = (size_t)b * N + i;
+    const half* src = qkv + row * (H + 2 * KV) * kDim;
+    // units: 8 threads per rotated head, each 8 pairs (two 16-byte loads), then 8 per value head (the same two loads)
+    const int units = (H + 2 * KV) * 8, turned = (H + KV) * 8;
+    uint4 a1, a2, c1 = make_uint4(0u, 0u, 0u, 0u), c2 = c1;
+    auto fetch = [&](int u) {
+        const int at = (u >> 3) * kDim + (u & 7) * 8;
+        a1 = ld_stream_u4(src + at);
+        a2 = ld_stream_u4(src + at + 64);
+        if (bias) {
+            c1 = __ldg(reinterpret_cast<const uint4*>(bias + at));
+            c2 = __ldg(reinterpret_cast<const uint4*>(bias + at + 64));
+        }
+    };
+    if (tid < units) fetch(tid);
+    if (i >= nodes_of(tree_len, b, N)) return;
     if (tid < kDim / 2) {
-        const double pos = (double)len[b] + depth[row];
-        const double a = pos * exp2(-log2_base * tid / (kDim / 2));
+        const double a = ((double)len[b] + depth[row]) * freqs.f[tid];
         constexpr double kTurn = 6.283185307179586476925;
         const float r = (float)(a - kTurn * rint(a * (1.0 / kTurn)));
         sincosf(r, &sn[tid], &cs[tid]);
     }
     __syncthreads();
-    const half* src = qkv + row * (H + 2 * KV) * kDim;
-    // rotated heads: 8 threads per head, each 8 pairs (two 16-byte loads); then the value rows
-    for (int u = tid; u < (H + KV) * 8; u += blockDim.x) {
+    for (int u = tid; u < units;) {
         const int h = u >> 3, t0 = (u & 7) * 8;
-        float x1[8], x2[8], r1[8], r2[8];
-        unpack8(*reinterpret_cast<const uint4*>(src + h * kDim + t0), x1);
-        unpack8(*reinterpret_cast<const uint4*>(src + h * kDim + t0 + 64), x2);
-        if (bias) {
-            float b1[8], b2[8];
-            unpack8(*reinterpret_cast<const uint4*>(bias + h * kDim + t0), b1);
-            unpack8(*reinterpret_cast<const uint4*>(bias + h * kDim + t0 + 64), b2);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { x1[e] += b1[e]; x2[e] += b2[e]; }
-        }
+        float x1[8], x2[8], b1[8], b2[8];
+        unpack8(a1, x1);
+        unpack8(a2, x2);
+        unpack8(c1, b1);
+        unpack8(c2, b2);
+        const int next = u + kRopeThreads;
+        if (next < units) fetch(next);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float c = cs[t0 + e], s = sn[t0 + e];
-            r1[e] = x1[e] * c - x2[e] * s;
-            r2[e] = x2[e] * c + x1[e] * s;
+            x1[e] += b1[e];
+            x2[e] += b2[e];
         }
-        half* dst = h < H ? Q + (row * H + h) * kDim : TK + (row * KV + (h - H)) * kDim;
-        *reinterpret_cast<uint4*>(dst + t0) = pack8(r1);
-        *reinterpret_cast<uint4*>(dst + t0 + 64) = pack8(r2);
-    }
-    for (int u = tid; u < KV * 16; u += blockDim.x) {
-        float x[8];
-        unpack8(*reinterpret_cast<const uint4*>(src + (H + KV) * kDim + u * 8), x);
-        if (bias) {
-            float bb[8];
-            unpack8(*reinterpret_cast<const uint4*>(bias + (H + KV) * kDim + u * 8), bb);
+        half* dst = h < H ? Q + (row * H + h) * kDim : (u < turned ? TK : TV) + (row * KV + (h - H) % KV) * kDim;
+        if (u < turned) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] += bb[e];
+            for (int e = 0; e < 8; ++e) {
+                const float c = cs[t0 + e], s = sn[t0 + e], y1 = x1[e], y2 = x2[e];
+                x1[e] = y1 * c - y2 * s;
+                x2[e] = y2 * c + y1 * s;
+            }
         }
-        *reinterpret_cast<uint4*>(TV + row * KV * kDim + u * 8) = pack8(x);
+        *reinterpret_cast<uint4*>(dst + t0) = pack8(x1);
+        *reinterpret_cast<uint4*>(dst + t0 + 64) = pack8(x2);
+        u = next;
     }
 }
 
@@ -363,29 +375,42 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
 }
 
 // ---------------------------------------------------------------- commit
-// One CTA per (layer, sequence); a thread copies 16 bytes of K or V of one row at a time.
-__global__ void __launch_bounds__(256)
+// One CTA per (layer, sequence, K or V); a thread copies 16-byte pieces, several loads in flight (one load at a time,
+// each behind its node's path entry, took 18.1 us for 32 x 24 caches).
+constexpr int kCommitThreads = 256;
+constexpr int kCommitBatch = 5;
+
+__global__ void __launch_bounds__(kCommitThreads)
     tree_commit_k(const half* __restrict__ TK, const half* __restrict__ TV, size_t tree_layer_stride, half* K, half* V,
                   size_t layer_stride, int stride, int slot_rows, int num_slots, const int* __restrict__ slot,
                   const int* __restrict__ len, const int* __restrict__ path, const int* __restrict__ accepted, int N,
                   int cols, int* __restrict__ len_out) {
+    __shared__ int node[kMaxNodes];  // the tree row of each committed row
     const int b = blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
+    if (tid < N) node[tid] = tid ? path[(size_t)b * N + tid - 1] : 0;
     const int at = slot ? slot[b] : b, m = len[b], acc = accepted[b];
     const bool ok = at >= 0 && at < num_slots && m >= 0 && m <= slot_rows && acc >= 0;
     const int rows = ok ? min(1 + min(acc, N - 1), slot_rows - m) : 0;
-    if (l == 0 && tid == 0 && len_out) len_out[b] = m + rows;
-    const half* tk = TK + (size_t)l * tree_layer_stride + (size_t)b * N * cols;
-    const half* tv = TV + (size_t)l * tree_layer_stride + (size_t)b * N * cols;
-    const size_t base = (size_t)l * layer_stride + ((size_t)(ok ? at : 0) * slot_rows + m) * stride;
-    const int per = cols / 8;  // 16-byte pieces of a row
-    for (int x = tid; x < rows * 2 * per; x += blockDim.x) {
-        const int row = x / (2 * per), c = x - row * 2 * per;
-        const int node = row ? path[(size_t)b * N + row - 1] : 0;
-        if (node < 0 || node >= N) continue;
-        const bool v = c >= per;
-        const int e = (v ? c - per : c) * 8;
-        const uint4 y = *reinterpret_cast<const uint4*>((v ? tv : tk) + (size_t)node * cols + e);
-        *reinterpret_cast<uint4*>((v ? V : K) + base + (size_t)row * stride + e) = y;
+    if (l == 0 && blockIdx.z == 0 && tid == 0 && len_out) len_out[b] = m + rows;
+    __syncthreads();
+    const half* src = (blockIdx.z ? TV : TK) + (size_t)l * tree_layer_stride + (size_t)b * N * cols;
+    half* dst = (blockIdx.z ? V : K) + (size_t)l * layer_stride + ((size_t)(ok ? at : 0) * slot_rows + m) * stride;
+    const int per = cols / 8, all = rows * per;  // 16-byte pieces
+    for (int x0 = tid; x0 < all; x0 += kCommitBatch * kCommitThreads) {
+        uint4 y[kCommitBatch];
+        int row[kCommitBatch], e[kCommitBatch];
+#pragma unroll
+        for (int k = 0; k < kCommitBatch; ++k) {
+            const int x = x0 + k * kCommitThreads;
+            row[k] = x < all ? x / per : -1;
+            e[k] = (x - row[k] * per) * 8;
+            const int n = row[k] >= 0 ? node[row[k]] : -1;
+            if (n < 0 || n >= N) row[k] = -1;  // past the end, or no node of this tree
+            else y[k] = ld_stream_u4(src + (size_t)n * cols + e[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kCommitBatch; ++k)
+            if (row[k] >= 0) *reinterpret_cast<uint4*>(dst + (size_t)row[k] * stride + e[k]) = y[k];
     }
 }
 
@@ -445,10 +470,12 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
         !aligned16(bias) || !aligned16(Q) || !aligned16(TK) || !aligned16(TV) || !(rope_base > 0.f) ||
         !(rope_base < INFINITY))
         return (int)cudaErrorInvalidValue;
-    tree_rope_k<<<dim3(N, B), 256, 0, S(stream)>>>(
+    RopeFreqs freqs;
+    const double step = -log2((double)rope_base) / (kDim / 2);
+    for (int t = 0; t < kDim / 2; ++t) freqs.f[t] = exp2(step * t);
+    tree_rope_k<<<dim3(N, B), kRopeThreads, 0, S(stream)>>>(
         reinterpret_cast<const half*>(qkv), reinterpret_cast<const half*>(bias), depth, len, tree_len, N, num_heads,
-        num_kv_heads, log2((double)rope_base), reinterpret_cast<half*>(Q), reinterpret_cast<half*>(TK),
-        reinterpret_cast<half*>(TV));
+        num_kv_heads, freqs, reinterpret_cast<half*>(Q), reinterpret_cast<half*>(TK), reinterpret_cast<half*>(TV));
     return (int)cudaGetLastError();
 }
 
@@ -490,7 +517,7 @@ int llmdiy_tree_commit(const uint16_t* TK, const uint16_t* TV, size_t tree_layer
                         tree_layer_stride < (size_t)B * N * cols)) ||
         !aligned16(TK) || !aligned16(TV) || !aligned16(K) || !aligned16(V))
         return (int)cudaErrorInvalidValue;
-    tree_commit_k<<<dim3(B, layers), 256, 0, S(stream)>>>(
+    tree_commit_k<<<dim3(B, layers, 2), kCommitThreads, 0, S(stream)>>>(
         reinterpret_cast<const half*>(TK), reinterpret_cast<const half*>(TV), tree_layer_stride,
         reinterpret_cast<half*>(K), reinterpret_cast<half*>(V), layer_stride, stride, slot_rows, num_slots, slot, len,
         path, accepted, N, cols, len_out);
