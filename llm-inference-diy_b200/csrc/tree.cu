@@ -133,6 +133,16 @@ LLMDIY_DEV void ver_weights(const float4& p, const float4& q, double T, double* 
     }
 }
 
+// Eight bytes into the shared memory of CTA `rank` of the cluster, counted by the mbarrier there.
+LLMDIY_DEV void ver_send(double* dst, uint64_t* bar, uint32_t rank, double v) {
+    uint32_t d, m;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(dst)), "r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(smem_u32(bar)), "r"(rank));
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(d),
+                 "l"(__double_as_longlong(v)), "r"(m)
+                 : "memory");
+}
+
 LLMDIY_DEV double warp_sum(double x) {
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
@@ -143,6 +153,7 @@ struct VerSmem {
     int parent[kMaxNodes], token[kMaxNodes], child[kMaxNodes], sibling[kMaxNodes];
     double p[kMaxNodes], q[kMaxNodes], u[kMaxNodes];
     double part[2][kVerMaxCluster * kVerWarps];  // the cluster's warp totals, in order (two rounds)
+    uint64_t got[2];                             // counts their bytes
     int dead[kMaxNodes];                         // refused tokens of the current node (no draft distribution)
 };
 
@@ -157,10 +168,17 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const size_t row0 = (size_t)b * N;
+    const int U = (V + 127) / 128, K = C * kVerWarps, k = rank * kVerWarps + warp;
+    const int u0 = (int)((long long)U * k / K), u1 = (int)((long long)U * (k + 1) / K);
     int par = -1, tok = -1;
     if (tid > 0 && tid < N) {  // (in flight together with the tree's size)
         par = parent[row0 + tid];
         tok = token[row0 + tid];
+    }
+    if (tid == 0) {
+        mbar_init(&s.got[0], 1);
+        mbar_init(&s.got[1], 1);
+        mbar_fence_init();
     }
     const int n = nodes_of(tree_len, b, N);
     if (rank == 0)
@@ -187,10 +205,8 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         s.child[tid] = child;
         s.sibling[tid] = s.parent[tid] >= 0 ? sib : -1;
     }
-    cluster.sync();  // every CTA of the cluster runs: its shared memory may be written
+    cluster.sync();  // every CTA of the cluster runs and has set up its barriers: its shared memory may be written
 
-    const int U = (V + 127) / 128, K = C * kVerWarps, k = rank * kVerWarps + warp;
-    const int u0 = (int)((long long)U * k / K), u1 = (int)((long long)U * (k + 1) / K);
     const float *prow = target, *qrow = draft;  // the current node's rows
     double T = 0.0;                             // weight of entry v: max(0, p - T q)
     int round = 0, dead0 = 0, ndead = 0;  // the current node's refused tokens: s.dead[dead0 .. dead0 + ndead)
@@ -215,9 +231,10 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         p = ver_load(prow, v0, V, vec);
         q = draft && T != 0.0 ? ver_load(qrow, v0, V, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
-    // this warp's total goes into every CTA's table; returns the table once it is complete.  Two tables
-    // take turns: a CTA writes table r & 1 again only after the barrier of round r + 1, which every CTA
-    // reaches after it has read round r's.
+    // This warp's total goes into every CTA's table by asynchronous stores that complete on the receiver's mbarrier (a
+    // cluster barrier a round took as long as the row's pass itself); returns the table once it is complete, NULL if
+    // that does not happen (bounded).  Two tables take turns: a warp sends round r + 2's total only after every warp's
+    // of round r + 1 has come, which each sends after it has read round r's table.
     auto totals = [&]() -> const double* {
         if (held_node != cur) {
             held_node = cur;
@@ -240,15 +257,19 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
             t += (w[0] + w[1]) + (w[2] + w[3]);
         }
         t = warp_sum(t);
-        double* mine = s.part[round++ & 1];
-        if (lane < C) cluster.map_shared_rank(mine, lane)[k] = t;
-        cluster.sync();
-        return mine;
+        double* mine = s.part[round & 1];
+        uint64_t* bar = &s.got[round & 1];
+        if (tid == 0) mbar_arrive_expect_tx(bar, K * (uint32_t)sizeof(double));
+        if (lane < C) ver_send(mine + k, bar, lane, t);
+        const bool ok = mbar_wait(bar, (round >> 1) & 1);
+        ++round;
+        return __all_sync(0xffffffffu, ok) ? mine : nullptr;
     };
     // lane l's share of the table: entries [l K / 32, (l + 1) K / 32)
     const int j0 = K * lane / 32, j1 = K * (lane + 1) / 32;
     auto lane_sum = [&](const double* tab) {
         double t = 0.0;
+        if (!tab) return (double)NAN;
         for (int j = j0; j < j1; ++j) t += tab[j];
         return t;
     };
