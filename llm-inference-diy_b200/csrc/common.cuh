@@ -165,6 +165,30 @@ LLMDIY_DEV uint4 ld_stream_u4(const void* p) {
     return r;
 }
 
+// The same through the coherent path, in program order: for data that the kernel ahead in a programmatic launch may
+// have written (a load that may be taken for invariant could move ahead of pdl_wait()).
+LLMDIY_DEV uint4 ld_once_u4(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+LLMDIY_DEV float4 ld_l2_f4(const void* p) {
+    float4 r;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+LLMDIY_DEV float2 ld_l2_f2(const void* p) {
+    float2 r;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(r.x), "=f"(r.y) : "l"(p) : "memory");
+    return r;
+}
+
 // Named barrier over `nthreads` threads (a multiple of 32) with id 1..15.
 LLMDIY_DEV void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

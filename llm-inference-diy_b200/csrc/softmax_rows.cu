@@ -67,8 +67,8 @@ LLMDIY_DEV SmWindow sm_window(const uint16_t* x, int n, uintptr_t first, uintptr
 }
 
 __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
-    softmax_rows_k(const half* __restrict__ logits, int ldl, const float* __restrict__ temp, int R, int V, int slice,
-                   float* __restrict__ probs, int ldp) {
+    softmax_rows_k(const half* logits, int ldl, const float* temp, int R, int V, int slice,
+                   float* probs, int ldp) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(128) uint8_t stage[];  // [kSmStages][kSmStageBytes]
     __shared__ float red_m[kSmThreads / 32], red_s[kSmThreads / 32];
@@ -103,6 +103,8 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     for (int i = tid; i < kSmStages * kSmStageBytes / 4; i += kSmThreads) reinterpret_cast<uint32_t*>(stage)[i] = 0xFC00FC00u;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
+    pdl_wait();  // nothing in global memory has been touched before this
+    pdl_launch_dependents();
     if (tid == 0)
         for (int i = 0; i < kSmStages; ++i)
             if (r0 + (long long)i * step < R) copy(r0 + i * step, i);
@@ -248,12 +250,14 @@ extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float*
     lc.blockDim = dim3(kSmThreads);
     lc.dynamicSmemBytes = kSmStages * kSmStageBytes;
     lc.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = C;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
-    lc.numAttrs = 1;
+    lc.numAttrs = 2;
     return (int)cudaLaunchKernelEx(&lc, softmax_rows_k, reinterpret_cast<const half*>(logits), ldl, temp, R, V, slice,
                                    probs, ldp);
 }

@@ -21,6 +21,23 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
+// (Pointers here carry no __restrict__: a load that the compiler may take for invariant could move ahead of pdl_wait.)
+// Launches with programmatic stream serialization: the kernel is set up while the stream's previous one ends, and
+// waits (pdl_wait) before it touches global memory.
+template <class... P, class... A>
+int launch_pdl(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid;
+    lc.blockDim = dim3(threads);
+    lc.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&lc, kern, static_cast<P>(args)...);
+}
+
 LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
     return tree_len ? min(max(tree_len[b], 0), N) : N;
 }
@@ -36,10 +53,10 @@ struct RopeFreqs {
 constexpr int kRopeThreads = 256;
 
 __global__ void __launch_bounds__(kRopeThreads)
-    tree_rope_k(const half* __restrict__ qkv, const half* __restrict__ bias, const int* __restrict__ depth,
-                const int* __restrict__ len, const int* __restrict__ tree_len, int N, int H, int KV,
-                const __grid_constant__ RopeFreqs freqs, half* __restrict__ Q, half* __restrict__ TK,
-                half* __restrict__ TV) {
+    tree_rope_k(const half* qkv, const half* bias, const int* depth,
+                const int* len, const int* tree_len, int N, int H, int KV,
+                const __grid_constant__ RopeFreqs freqs, half* Q, half* TK,
+                half* TV) {
     __shared__ float cs[kDim / 2], sn[kDim / 2];
     const int b = blockIdx.y, i = blockIdx.x, tid = threadIdx.x;
     const size_t row = (size_t)b * N + i;
@@ -49,13 +66,15 @@ __global__ void __launch_bounds__(kRopeThreads)
     uint4 a1, a2, c1 = make_uint4(0u, 0u, 0u, 0u), c2 = c1;
     auto fetch = [&](int u) {
         const int at = (u >> 3) * kDim + (u & 7) * 8;
-        a1 = ld_stream_u4(src + at);
-        a2 = ld_stream_u4(src + at + 64);
+        a1 = ld_once_u4(src + at);
+        a2 = ld_once_u4(src + at + 64);
         if (bias) {
-            c1 = __ldg(reinterpret_cast<const uint4*>(bias + at));
-            c2 = __ldg(reinterpret_cast<const uint4*>(bias + at + 64));
+            c1 = ld_once_u4(bias + at);
+            c2 = ld_once_u4(bias + at + 64);
         }
     };
+    pdl_wait();
+    pdl_launch_dependents();
     if (tid < units) fetch(tid);
     if (i >= nodes_of(tree_len, b, N)) return;
     if (tid < kDim / 2) {
@@ -110,12 +129,12 @@ LLMDIY_DEV double positive(double x) { return x > 0.0 ? x : 0.0; }  // NaN count
 
 // Entries v0 .. v0 + 3 of a row (0 past V); vec: the rows are 16-byte aligned.
 LLMDIY_DEV float4 ver_load(const float* row, int v0, int V, bool vec) {
-    if (vec && v0 + 3 < V) return __ldg(reinterpret_cast<const float4*>(row + v0));
+    if (vec && v0 + 3 < V) return *reinterpret_cast<const float4*>(row + v0);
     float4 a;
-    a.x = v0 < V ? __ldg(row + v0) : 0.f;
-    a.y = v0 + 1 < V ? __ldg(row + v0 + 1) : 0.f;
-    a.z = v0 + 2 < V ? __ldg(row + v0 + 2) : 0.f;
-    a.w = v0 + 3 < V ? __ldg(row + v0 + 3) : 0.f;
+    a.x = v0 < V ? row[v0] : 0.f;
+    a.y = v0 + 1 < V ? row[v0 + 1] : 0.f;
+    a.z = v0 + 2 < V ? row[v0 + 2] : 0.f;
+    a.w = v0 + 3 < V ? row[v0 + 3] : 0.f;
     return a;
 }
 
@@ -158,10 +177,10 @@ struct VerSmem {
 };
 
 __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
-    tree_verify_k(const float* __restrict__ target, int ldt, const float* __restrict__ draft, int ldd,
-                  const int* __restrict__ token, const int* __restrict__ parent, const int* __restrict__ tree_len,
-                  const float* __restrict__ uniform, int N, int V, int vec, int* __restrict__ path,
-                  int* __restrict__ accepted, int* __restrict__ next) {
+    tree_verify_k(const float* target, int ldt, const float* draft, int ldd,
+                  const int* token, const int* parent, const int* tree_len,
+                  const float* uniform, int N, int V, int vec, int* path,
+                  int* accepted, int* next) {
     namespace cg = cooperative_groups;
     __shared__ VerSmem s;
     cg::cluster_group cluster = cg::this_cluster();
@@ -170,15 +189,18 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
     const size_t row0 = (size_t)b * N;
     const int U = (V + 127) / 128, K = C * kVerWarps, k = rank * kVerWarps + warp;
     const int u0 = (int)((long long)U * k / K), u1 = (int)((long long)U * (k + 1) / K);
-    int par = -1, tok = -1;
-    if (tid > 0 && tid < N) {  // (in flight together with the tree's size)
-        par = parent[row0 + tid];
-        tok = token[row0 + tid];
-    }
     if (tid == 0) {
         mbar_init(&s.got[0], 1);
         mbar_init(&s.got[1], 1);
         mbar_fence_init();
+    }
+    cluster.sync();  // every CTA of the cluster runs and has set up its barriers: its shared memory may be written
+    pdl_wait();      // nothing in global memory has been touched before this
+    pdl_launch_dependents();
+    int par = -1, tok = -1;
+    if (tid > 0 && tid < N) {  // (in flight together with the tree's size)
+        par = parent[row0 + tid];
+        tok = token[row0 + tid];
     }
     const int n = nodes_of(tree_len, b, N);
     if (rank == 0)
@@ -205,7 +227,7 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         s.child[tid] = child;
         s.sibling[tid] = s.parent[tid] >= 0 ? sib : -1;
     }
-    cluster.sync();  // every CTA of the cluster runs and has set up its barriers: its shared memory may be written
+    __syncthreads();
 
     const float *prow = target, *qrow = draft;  // the current node's rows
     double T = 0.0;                             // weight of entry v: max(0, p - T q)
@@ -402,12 +424,14 @@ constexpr int kCommitThreads = 256;
 constexpr int kCommitBatch = 5;
 
 __global__ void __launch_bounds__(kCommitThreads)
-    tree_commit_k(const half* __restrict__ TK, const half* __restrict__ TV, size_t tree_layer_stride, half* K, half* V,
-                  size_t layer_stride, int stride, int slot_rows, int num_slots, const int* __restrict__ slot,
-                  const int* __restrict__ len, const int* __restrict__ path, const int* __restrict__ accepted, int N,
-                  int cols, int* __restrict__ len_out) {
+    tree_commit_k(const half* TK, const half* TV, size_t tree_layer_stride, half* K, half* V,
+                  size_t layer_stride, int stride, int slot_rows, int num_slots, const int* slot,
+                  const int* len, const int* path, const int* accepted, int N,
+                  int cols, int* len_out) {
     __shared__ int node[kMaxNodes];  // the tree row of each committed row
     const int b = blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
     if (tid < N) node[tid] = tid ? path[(size_t)b * N + tid - 1] : 0;
     const int at = slot ? slot[b] : b, m = len[b], acc = accepted[b];
     const bool ok = at >= 0 && at < num_slots && m >= 0 && m <= slot_rows && acc >= 0;
@@ -427,7 +451,7 @@ __global__ void __launch_bounds__(kCommitThreads)
             e[k] = (x - row[k] * per) * 8;
             const int n = row[k] >= 0 ? node[row[k]] : -1;
             if (n < 0 || n >= N) row[k] = -1;  // past the end, or no node of this tree
-            else y[k] = ld_stream_u4(src + (size_t)n * cols + e[k]);
+            else y[k] = ld_once_u4(src + (size_t)n * cols + e[k]);
         }
 #pragma unroll
         for (int k = 0; k < kCommitBatch; ++k)
@@ -494,10 +518,9 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
     RopeFreqs freqs;
     const double step = -log2((double)rope_base) / (kDim / 2);
     for (int t = 0; t < kDim / 2; ++t) freqs.f[t] = exp2(step * t);
-    tree_rope_k<<<dim3(N, B), kRopeThreads, 0, S(stream)>>>(
-        reinterpret_cast<const half*>(qkv), reinterpret_cast<const half*>(bias), depth, len, tree_len, N, num_heads,
-        num_kv_heads, freqs, reinterpret_cast<half*>(Q), reinterpret_cast<half*>(TK), reinterpret_cast<half*>(TV));
-    return (int)cudaGetLastError();
+    return launch_pdl(tree_rope_k, dim3(N, B), kRopeThreads, S(stream), reinterpret_cast<const half*>(qkv),
+                      reinterpret_cast<const half*>(bias), depth, len, tree_len, N, num_heads, num_kv_heads, freqs,
+                      reinterpret_cast<half*>(Q), reinterpret_cast<half*>(TK), reinterpret_cast<half*>(TV));
 }
 
 int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd, const int* token,
@@ -516,12 +539,14 @@ int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd
     lc.gridDim = dim3(B * C);
     lc.blockDim = dim3(kVerThreads);
     lc.stream = S(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = attr;
-    lc.numAttrs = 1;
+    lc.numAttrs = 2;
     return (int)cudaLaunchKernelEx(&lc, tree_verify_k, target, ldt, draft, ldd, token, parent, tree_len, uniform, N, V,
                                    vec, path, accepted, next);
 }
@@ -538,11 +563,10 @@ int llmdiy_tree_commit(const uint16_t* TK, const uint16_t* TV, size_t tree_layer
                         tree_layer_stride < (size_t)B * N * cols)) ||
         !aligned16(TK) || !aligned16(TV) || !aligned16(K) || !aligned16(V))
         return (int)cudaErrorInvalidValue;
-    tree_commit_k<<<dim3(B, layers, 2), kCommitThreads, 0, S(stream)>>>(
-        reinterpret_cast<const half*>(TK), reinterpret_cast<const half*>(TV), tree_layer_stride,
-        reinterpret_cast<half*>(K), reinterpret_cast<half*>(V), layer_stride, stride, slot_rows, num_slots, slot, len,
-        path, accepted, N, cols, len_out);
-    return (int)cudaGetLastError();
+    return launch_pdl(tree_commit_k, dim3(B, layers, 2), kCommitThreads, S(stream), reinterpret_cast<const half*>(TK),
+                      reinterpret_cast<const half*>(TV), tree_layer_stride, reinterpret_cast<half*>(K),
+                      reinterpret_cast<half*>(V), layer_stride, stride, slot_rows, num_slots, slot, len, path, accepted,
+                      N, cols, len_out);
 }
 
 }  // extern "C"

@@ -313,12 +313,6 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     Smem& s = *reinterpret_cast<Smem*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.H / a.KV;
-    TaCursor c;
-    c.left = 0;
-    if (DIRECT) {  // (its loads are under way while the barriers are set up)
-        c.b = blockIdx.z;
-        ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
-    }
     if (warp == 4 && lane == 0) {  // the thread that issues the copies: it need not wait for the others
         prefetch_tmap(&tq);
         prefetch_tmap(&tk);
@@ -351,12 +345,18 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         tmem_alloc(&s.tmem_base, kTaCols);
         tmem_relinquish();
     }
+    pdl_wait();  // nothing in global memory has been touched before this
+    pdl_launch_dependents();
+    TaCursor c;
+    c.left = 0;
     const int C = DIRECT ? (int)gridDim.x : 1, rank = DIRECT ? (int)blockIdx.x : 0;  // the unit's cluster
     // Flat: the M tiles of a kv head go to neighbouring CTAs at the same tiles, so that the second one to read a K/V
     // tile finds it in L2.
     const int mtile = DIRECT ? (int)blockIdx.y % a.mt : (int)blockIdx.x % a.mt, m0 = mtile * a.npt;
     if (DIRECT) {
+        c.b = blockIdx.z;
         c.unit = blockIdx.y / a.mt;
+        ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
         if (m0 < c.n) {
             // The unit's last tiles (the cache's tail, the tree) take up to two tiles longer: the last CTAs get that many
             // fewer where the others have as many.  16 x 17 tiles: 11.2 us with equal shares, 9.6 so; with 2 or 5
@@ -388,7 +388,6 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         __syncwarp();
         named_bar_arrive(1, kTaThreads);
     }
-    if (!DIRECT) pdl_launch_dependents();  // the merge may be scheduled; it waits for this grid before it reads
     const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;  // P(j) at tP + 32 * (j & 1), or (TWO) at tP, its low terms at tP + 32
 
     if (warp == 4 && work) {
@@ -811,14 +810,16 @@ constexpr int kTaMergeWarps = 16;
 
 __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_constant__ TaArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = blockIdx.x / a.mt + 1, m0 = blockIdx.x % a.mt * a.npt;
+    // Every thread waits for the attention kernel, also where there is nothing to join: this grid must not be
+    // over before that one is.  (That one triggers this launch only when it has itself seen the kernels before it
+    // complete, so the lengths may be read ahead of the wait.)
     const TaDeal deal(ta_total(a, lane), a.W);
     TaCursor c;
     int f0 = 0;
     const bool cut = w < deal.W;
     if (cut) f0 = ta_locate(a, deal.start(w), lane, c);
-    // every thread waits for the attention kernel, also where there is nothing to join: this grid
-    // must not be over before that one is
     pdl_wait();
+    pdl_launch_dependents();
     if (!cut || c.at <= kTaUnitCost || m0 >= c.n) return;  // no tile of the unit before the cut
     const int w0 = deal.owner(f0 + kTaUnitCost), w1 = deal.owner(f0 + kTaUnitCost + c.tiles - 1);
     // the first CTA's part of this unit is its first segment only when its range does not start before the unit
@@ -833,7 +834,7 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
     for (int q = live * share / shares + warp * 2; q < r1; q += kTaMergeWarps * 2) {
         const int r = min(q + (lane >> 4), r1 - 1);  // (lanes past the share repeat its last row)
         float M = -INFINITY;
-        for (int k = w0 + gl; k <= w1; k += 16) M = fmaxf(M, __ldcg(ml + (size_t)part(k) * a.rows + r).x);
+        for (int k = w0 + gl; k <= w1; k += 16) M = fmaxf(M, ld_l2_f2(ml + (size_t)part(k) * a.rows + r).x);
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         float Ls = 0.f;
@@ -843,7 +844,7 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
         for (int c0 = w0; c0 <= w1; c0 += 16) {
             float f = 0.f;
             if (c0 + gl <= w1) {
-                const float2 y = __ldcg(ml + (size_t)part(c0 + gl) * a.rows + r);
+                const float2 y = ld_l2_f2(ml + (size_t)part(c0 + gl) * a.rows + r);
                 // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
                 f = y.x == -INFINITY ? (y.y == y.y ? 0.f : 1.f) : exp2f(y.x - M);
                 Ls += y.y * f;
@@ -855,7 +856,7 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
                 const float4* src = reinterpret_cast<const float4*>(a.part + ((size_t)part(c0 + i) * a.rows + r) * kTaDim) + gl;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float4 y = __ldcg(src + 16 * e);
+                    const float4 y = ld_l2_f4(src + 16 * e);
                     acc[e].x = __fmaf_rn(fk, y.x, acc[e].x);
                     acc[e].y = __fmaf_rn(fk, y.y, acc[e].y);
                     acc[e].z = __fmaf_rn(fk, y.z, acc[e].z);
@@ -972,12 +973,15 @@ int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cl
     lc.blockDim = dim3(kTaThreads);
     lc.dynamicSmemBytes = bytes;
     lc.stream = st;
-    cudaLaunchAttribute at[1];
+    // programmatic serialization: the CTAs set up their barriers and TMEM while the stream's previous kernel ends
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
-    lc.numAttrs = 1;
+    lc.numAttrs = 2;
     return (int)cudaLaunchKernelEx(&lc, kern, m[0], m[1], m[2], m[3], m[4], a, err);
 }
 
