@@ -37,6 +37,27 @@ LLMDIY_DEV float sm_ex2(float x) {  // 2^x (2^-inf = 0)
     return y;
 }
 LLMDIY_DEV uint32_t sm_pair(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
+// Two fp32 values at once
+LLMDIY_DEV uint64_t sm_f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+LLMDIY_DEV float2 sm_split(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+LLMDIY_DEV uint64_t sm_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+LLMDIY_DEV uint64_t sm_mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // Eight bytes into the shared memory of CTA `rank` of the cluster, counted by the mbarrier there.
 LLMDIY_DEV void sm_send(float2* dst, uint64_t* bar, uint32_t rank, float a, float b) {
     uint32_t d, m;
@@ -162,14 +183,17 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         const float k = t > 0.f ? fminf(1.4426950408889634f / t, 1e30f) : 1e30f;
         auto weight = [&](float v, float top) { return sm_ex2((v - top) * k); };
         const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: every weight 0
-        float s = 0.f, ex[2 * kSmPairs];
+        uint64_t ex[kSmPairs], s2[2] = {0, 0};
+        const uint64_t minus = sm_f2(-ref, -ref), k2 = sm_f2(k, k);
 #pragma unroll
         for (int i = 0; i < kSmPairs; ++i) {
             const float2 f = sm_floats(w[i]);
-            ex[2 * i] = weight(f.x, ref);
-            ex[2 * i + 1] = weight(f.y, ref);
-            s += ex[2 * i] + ex[2 * i + 1];
+            const float2 d = sm_split(sm_mul2(sm_add2(sm_f2(f.x, f.y), minus), k2));
+            ex[i] = sm_f2(sm_ex2(d.x), sm_ex2(d.y));
+            s2[i & 1] = sm_add2(s2[i & 1], ex[i]);
         }
+        const float2 sp = sm_split(sm_add2(s2[0], s2[1]));
+        float s = sp.x + sp.y;
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) s += weight(h2f(__ushort_as_half(x[a])), ref);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -197,14 +221,20 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         const float top = M == -INFINITY ? 0.f : M;
         const float scale = inv * (m == -INFINITY ? 1.f : weight(m, top));
         float2* out = reinterpret_cast<float2*>(y - odd) + tid;
-        const int room = held + odd - 2 * tid;  // entries from this thread's first on
+        const int room = held + odd - 2 * tid;           // entries from this thread's first on
+        const int whole = (held + odd) / (2 * kSmThreads);  // runs that lie inside the slice as a whole
+        const bool head = odd && tid == 0;               // the pair that begins one entry early
+        const uint64_t scale2 = sm_f2(scale, scale);
 #pragma unroll
         for (int i = 0; i < kSmPairs; ++i) {
-            const float2 o = make_float2(ex[2 * i] * scale, ex[2 * i + 1] * scale);
-            const bool head = i == 0 && odd && tid == 0;  // the pair that begins one entry early
-            if (2 * i * kSmThreads + 1 < room && !head) out[i * kSmThreads] = o;
-            if (2 * i * kSmThreads + 1 == room && !head) out[i * kSmThreads].x = o.x;
-            if (head && held > 0) y[0] = o.y;
+            const float2 o = sm_split(sm_mul2(ex[i], scale2));
+            if (i == 0 && head) {
+                if (held > 0) y[0] = o.y;
+            } else if (i < whole || 2 * i * kSmThreads + 1 < room) {
+                out[i * kSmThreads] = o;
+            } else if (2 * i * kSmThreads + 1 == room) {
+                out[i * kSmThreads].x = o.x;
+            }
         }
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
     }

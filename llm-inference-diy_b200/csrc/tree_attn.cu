@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     using Smem = TaSmem<QR, KS, VS>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem& s = *reinterpret_cast<Smem*>(smem_raw);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (uniform for the compiler)
     const int G = a.H / a.KV;
     if (warp == 4 && lane == 0) {  // the thread that issues the copies: it need not wait for the others
         prefetch_tmap(&tq);
