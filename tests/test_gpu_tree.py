@@ -572,3 +572,122 @@ def test_a_step_captured_and_replayed_on_another_stream():
         t.cuda.synchronize()
         for x in ("Q", "TK", "TV", "O", "logits", "probs", "path", "acc", "next", "len_out", "K", "V_"):
             assert t.equal(getattr(a, x), getattr(b, x)), x
+
+
+# ------------------------------------------------------------------ long and many
+# Long caches of several sequences go in equal ranges over all SMs (flat), the others a cluster to a unit (direct):
+# the tests above are mostly direct, these are flat.
+@pytest.mark.parametrize("length", [40000, 26000 + 63])
+def test_attn_nothing_leaks_in_a_long_cache(length):
+    N = 24
+    a = Attn(length, 2, N, 4, 2, [length, length], max_len=length + 70, tree_len=[24, 20])
+    for s in range(2):
+        a.K[s, length:] = np.nan
+        a.V[s, length:] = np.inf
+        a.V[s, length + 1:] = np.nan
+    a.TK[1, 20:], a.TV[1, 20:] = np.inf, np.nan
+    a.TV[0, 7, 5], a.TV[0, 9, 130], a.TK[0, 11, 3] = np.nan, -np.inf, np.nan
+    a.device().call()
+    with np.errstate(invalid="ignore"):
+        a.check(rows=150)
+    clean = [i for i in range(N) if not {7, 9, 11} & a.sees[0][i]]
+    assert np.isfinite(a.d["O"].cpu().numpy()[0, clean, :4 * D]).all()
+
+
+def test_attn_long_cache_with_empty_rows_and_two_tree_tiles():
+    rng = np.random.default_rng(5)
+    N = 100
+    sees = [[set() if i % 3 == 0 else set(np.nonzero(rng.random(N) < 0.2)[0].tolist()) for i in range(N)]
+            for _ in range(3)]
+    a = Attn(6, 3, N, 4, 2, [30000, 0, 511], max_len=30001, tree_len=[100, 70, 30], sees=sees, pad=8)
+    a.device().call().check(rows=200)
+    assert np.all(a.d["O"].cpu().numpy()[1, 0, :4 * D] == 0.0)
+
+
+def test_attn_many_sequences_of_all_lengths():
+    """More sequences than a warp has lanes, several of them reading one slot, lengths from none to 13000."""
+    rng = np.random.default_rng(12)
+    B = 70
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(13000), B))]
+    lens[3], lens[40], lens[69] = 0, 13000, 12999
+    tl = [int(x) for x in rng.integers(0, 6, B)]
+    a = Attn(13, B, 5, 2, 1, lens, max_len=13000, tree_len=tl, slots=[b % 3 for b in range(B)], num_slots=3)
+    a.device().call().check(rows=400)
+
+
+def test_attn_many_short_sequences():
+    rng = np.random.default_rng(14)
+    B = 300
+    a = Attn(15, B, 4, 4, 2, [int(x) for x in rng.integers(0, 130, B)], max_len=130)
+    a.device().call().check(rows=400)
+
+
+def test_attn_long_captured_and_on_two_streams():
+    """A flat call (two launches) captured, replayed with other lengths, beside an eager one on another stream."""
+    t = torch()
+    a, b = (Attn(31, 2, 20, 4, 2, [40000, 31000], max_len=40000).device() for _ in range(2))
+    a.call()
+    t.cuda.synchronize()
+    st, other = t.cuda.Stream(), t.cuda.Stream()
+    g = t.cuda.CUDAGraph()
+    with t.cuda.graph(g, stream=st):
+        a.call(st.cuda_stream)
+        a.call(st.cuda_stream)  # the second in a row on one workspace
+    for lens in ([39999, 64], [1, 40000], [0, 0]):
+        a.lens = b.lens = lens
+        for x in (a, b):
+            x.d["len"].copy_(_i32(lens))
+            x.d["O"].fill_(7.0)
+        t.cuda.synchronize()
+        with t.cuda.stream(st):
+            g.replay()
+        b.call(other.cuda_stream)
+        t.cuda.synchronize()
+        assert t.equal(a.d["O"], b.d["O"])
+        a.check(rows=20)
+
+
+def test_softmax_many_rows_of_odd_length():
+    """More rows than clusters run at once, each starting at another alignment: no row sees its neighbours."""
+    t = torch()
+    for R, V in ((80, 151935), (900, 1001)):
+        g = t.Generator(device="cuda").manual_seed(R)
+        x = t.randn(R, V, generator=g, device="cuda", dtype=t.float16) * 3
+        x[::3] += 20  # neighbours of other sizes
+        x[1::7, : V // 2] = -float("inf")
+        out = t.zeros(R, V, device="cuda")
+        L.softmax_rows(_ptr(x), V, None, R, V, _ptr(out), V)
+        want = t.softmax(x.double(), 1)
+        big = want.clamp(min=1e-45).log().abs()
+        tol = want * (big * 2.0 ** -22 + 2.0 ** -20) + 2.0 ** -126
+        assert bool(((out.double() - want).abs() <= tol).all()), (R, V)
+
+
+def test_softmax_and_verify_past_32_bit_offsets():
+    """Rows that begin more than 2^31 entries after the first."""
+    t = torch()
+    N, V, B = 256, 151936, 57
+    assert (B * N - 1) * V > 2 ** 31
+    logits = t.zeros(B * N, V, dtype=t.float16, device="cuda")
+    g = t.Generator(device="cuda").manual_seed(3)
+    logits[-N:] = t.randn(N, V, generator=g, device="cuda", dtype=t.float16) * 3
+    probs = t.empty(B * N, V, device="cuda")
+    L.softmax_rows(_ptr(logits), V, None, B * N, V, _ptr(probs), V)
+    t.cuda.synchronize()
+    for r in (B * N - 1, B * N - N, B * N - N - 1):
+        want = t.softmax(logits[r].double(), 0)
+        tol = want * (want.log().abs() * 2.0 ** -22 + 2.0 ** -20)
+        assert bool(((probs[r].double() - want).abs() <= tol).all()), r
+    rng = np.random.default_rng(2)
+    parent = np.array([_parents(rng, N)] * B)
+    token = np.zeros((B, N), np.int64)
+    last = probs[-N:].cpu().numpy()
+    token[-1] = last.argmax(1)[np.maximum(parent[-1], 0)]
+    u = rng.random((B, N)).astype(np.float32)
+    path, acc, nxt = _i32(np.zeros((B, N))), _i32(np.zeros(B)), _i32(np.zeros(B))
+    L.tree_verify(_ptr(probs), V, None, 0, _ptr(_i32(token)), _ptr(_i32(parent)), None, _ptr(_dev(u)), B, N, V, _ptr(path),
+                  _ptr(acc), _ptr(nxt))
+    t.cuda.synchronize()
+    want = tm.verify(last, None, token[-1], parent[-1], N, u[-1])
+    assert int(acc[-1]) == len(want[0]) and int(nxt[-1]) == want[1]
+    assert path[-1, : len(want[0])].tolist() == want[0]
