@@ -50,7 +50,7 @@ LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
 struct RopeFreqs {
     double f[kDim / 2];
 };
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;  // (1536 nodes: 8.3 us with 256, 7.7 with 128)
 
 __global__ void __launch_bounds__(kRopeThreads)
     tree_rope_k(const half* qkv, const half* bias, const int* depth,
@@ -419,11 +419,11 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
 
 // ---------------------------------------------------------------- commit
 // One CTA per (layer, sequence, K or V); a thread copies 16-byte pieces, several loads in flight (one load at a time,
-// each behind its node's path entry, took 18.1 us for 32 x 24 caches).
+// each behind its node's path entry, took 18.1 us for 32 x 24 caches; so 13.3).
 constexpr int kCommitThreads = 256;
 constexpr int kCommitBatch = 5;
 
-__global__ void __launch_bounds__(kCommitThreads)
+__global__ void __launch_bounds__(kCommitThreads, 5)
     tree_commit_k(const half* TK, const half* TV, size_t tree_layer_stride, half* K, half* V,
                   size_t layer_stride, int stride, int slot_rows, int num_slots, const int* slot,
                   const int* len, const int* path, const int* accepted, int N,
