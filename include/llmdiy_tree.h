@@ -5,9 +5,10 @@
  * No counterpart in the reference, which decodes one greedy token per step (QwenEngine::step,
  * framework_src/qwen_infer.cu:614-737); each operator stands beside the launcher of its kind in
  * llmdiy_kernels.h (RoPE + KV append, flash decoding, argmax).  The conventions are that header's:
- * device pointers owned by the caller on the current device, fp16 as uint16_t bit patterns, a trailing
+ * device pointers owned by the caller on the current device, each aligned as its type, fp16 as uint16_t bit patterns, a trailing
  * stream (NULL = the legacy default stream), the cudaError_t of the launch as the return
- * value (cudaErrorInvalidValue for refused arguments, before anything is launched), no allocation,
+ * value (cudaErrorInvalidValue for refused arguments, before anything is launched; B <= 65535, at most 1024 heads,
+ * V <= 2^30), outputs that overlap no input and no other output, no allocation,
  * no synchronisation: every launcher can be captured into a CUDA graph, and the lengths, trees and slots are
  * read on the device when it runs.
  *
@@ -57,10 +58,12 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
  * Head h uses kv head h / (num_heads / num_kv_heads).  Node rows of Q and O are ldq and ldo elements
  * apart (>= num_heads*128).  max_len bounds every len[b] (larger values are clamped); it sets the grid and the
  * workspace, so a captured graph serves every length up to it.  fp32 scores, statistics and
- * accumulation, fp16 probabilities.  A row that sees nothing, or only scores of -inf, gives zeros; what
+ * accumulation; probabilities as fp16, in calls of up to 128 query rows (B * N * num_heads) as the sum of two fp16.
+ * A visible score of NaN or +inf makes its row NaN.  A row that sees nothing, or only scores of -inf, gives zeros; what
  * a node does not see (K and V rows at or past len[b], tree rows outside its mask) does not reach its
  * output even where it is Inf or NaN.
- * stride, ldq, ldo: multiples of 8 elements; fp16 pointers 16-byte aligned; num_slots * slot_rows < 2^31.
+ * stride, ldq, ldo: multiples of 8 elements; fp16 pointers 16-byte aligned; num_slots * slot_rows < 2^31;
+ * num_heads / num_kv_heads <= 128; max_len <= slot_rows.
  * work: llmdiy_tree_attn_work_bytes(...) bytes (16-byte aligned, zero-filled once before its first use),
  * which serves every smaller B, N and max_len with the same heads too; calls that may overlap on the GPU need
  * workspaces of their own. */
@@ -74,8 +77,9 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
 int llmdiy_tree_attn_status(const float* work);
 
 /* Probabilities of R rows of V fp16 logits (row pitches ldl and ldp elements, >= V):
- * probs = exp((x - max) / temp[r]) / sum in fp32, temp NULL = 1.  temp <= 0 gives the limit: equal shares of the
- * row's largest entries (greedy).  Entries of -inf get 0; a row with nothing above -inf gives zeros. */
+ * probs = exp((x - max) / temp[r]) / sum in fp32, temp NULL = 1.  temp <= 0 (or NaN) gives the limit: equal shares
+ * of the row's largest entries (greedy).  Entries of -inf get 0; a row with nothing above -inf gives zeros; one with a NaN or
+ * +inf is NaN throughout. */
 int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float* temp, int R, int V, float* probs, int ldp,
                         void* stream);
 

@@ -189,6 +189,12 @@ LLMDIY_DEV float2 ld_l2_f2(const void* p) {
     return r;
 }
 
+// Host: every pointer (NULL too) lies on a 4-byte boundary.
+template <class... P>
+inline bool words_aligned(const P*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & 3u) == 0;
+}
+
 // Named barrier over `nthreads` threads (a multiple of 32) with id 1..15.
 LLMDIY_DEV void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

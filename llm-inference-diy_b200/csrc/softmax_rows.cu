@@ -178,9 +178,9 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         m = red_m[lane & (kSmThreads / 32 - 1)];
 #pragma unroll
         for (int o = kSmThreads / 64; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        // k is bounded so that 0 * k is 0 at any t > 0; greedy (t <= 0 or NaN) takes that bound, where the
-        // smallest difference of two fp16 values gives 2^-inf
-        const float k = t > 0.f ? fminf(1.4426950408889634f / t, 1e30f) : 1e30f;
+        // k is bounded so that 0 * k is 0 and -inf * k is -inf at any t > 0; greedy (t <= 0 or NaN) takes the upper
+        // bound, where the smallest difference of two fp16 values gives 2^-inf
+        const float k = t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1e-30f), 1e30f) : 1e30f;
         auto weight = [&](float v, float top) { return sm_ex2((v - top) * k); };
         const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: every weight 0
         uint64_t ex[kSmPairs], s2[2] = {0, 0};
@@ -268,8 +268,8 @@ int sm_clusters(int C) {
 
 extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float* temp, int R, int V, float* probs,
                                    int ldp, void* stream) {
-    if (!logits || !probs || R <= 0 || V <= 0 || ldl < V || ldp < V || (reinterpret_cast<uintptr_t>(logits) & 1) ||
-        (reinterpret_cast<uintptr_t>(probs) & 3))
+    if (!logits || !probs || R <= 0 || V <= 0 || V > (1 << 30) || ldl < V || ldp < V ||
+        (reinterpret_cast<uintptr_t>(logits) & 1) || !words_aligned(probs, temp))
         return (int)cudaErrorInvalidValue;
     // CTAs per row: enough to hold it, and more while they leave SMs idle and a slice stays above 4096 entries
     int C = 1;

@@ -19,8 +19,6 @@ constexpr int kMaxNodes = LLMDIY_TREE_MAX_NODES;
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
-
 // (Pointers here carry no __restrict__: a load that the compiler may take for invariant could move ahead of pdl_wait.)
 // Launches with programmatic stream serialization: the kernel is set up while the stream's previous one ends, and
 // waits (pdl_wait) before it touches global memory.
@@ -512,8 +510,8 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
                      const int* tree_len, int B, int N, int num_heads, int num_kv_heads, float rope_base,
                      uint16_t* Q, uint16_t* TK, uint16_t* TV, void* stream) {
     if (!sizes_ok(B, N, num_heads, num_kv_heads) || !qkv || !depth || !len || !Q || !TK || !TV || !aligned16(qkv) ||
-        !aligned16(bias) || !aligned16(Q) || !aligned16(TK) || !aligned16(TV) || !(rope_base > 0.f) ||
-        !(rope_base < INFINITY))
+        !aligned16(bias) || !aligned16(Q) || !aligned16(TK) || !aligned16(TV) || !words_aligned(depth, len, tree_len) ||
+        !(rope_base > 0.f) || !(rope_base < INFINITY))
         return (int)cudaErrorInvalidValue;
     RopeFreqs freqs;
     const double step = -log2((double)rope_base) / (kDim / 2);
@@ -526,8 +524,9 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
 int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd, const int* token,
                        const int* parent, const int* tree_len, const float* uniform, int B, int N, int V, int* path,
                        int* accepted, int* next, void* stream) {
-    if (B <= 0 || B > 65535 || N <= 0 || N > kMaxNodes || V <= 0 || !target || ldt < V || (draft && ldd < V) || !token ||
-        !parent || !uniform || !path || !accepted || !next || !aligned4(target) || !aligned4(draft))
+    if (B <= 0 || B > 65535 || N <= 0 || N > kMaxNodes || V <= 0 || V > (1 << 30) || !target || ldt < V ||
+        (draft && ldd < V) || !token || !parent || !uniform || !path || !accepted || !next ||
+        !words_aligned(target, draft, token, parent, tree_len, uniform, path, accepted, next))
         return (int)cudaErrorInvalidValue;
     const int vec = aligned16(target) && ldt % 4 == 0 && (!draft || (aligned16(draft) && ldd % 4 == 0));
     // CTAs per sequence: as many as run at once (two per SM), 16 at most.  Measured at V = 151936: one
@@ -561,7 +560,8 @@ int llmdiy_tree_commit(const uint16_t* TK, const uint16_t* TV, size_t tree_layer
         (layer_stride & 7) || (tree_layer_stride & 7) || len_out == len ||
         (layers > 1 && (layer_stride < ((size_t)num_slots * slot_rows - 1) * stride + cols ||
                         tree_layer_stride < (size_t)B * N * cols)) ||
-        !aligned16(TK) || !aligned16(TV) || !aligned16(K) || !aligned16(V))
+        !aligned16(TK) || !aligned16(TV) || !aligned16(K) || !aligned16(V) ||
+        !words_aligned(slot, len, path, accepted, len_out))
         return (int)cudaErrorInvalidValue;
     return launch_pdl(tree_commit_k, dim3(B, layers, 2), kCommitThreads, S(stream), reinterpret_cast<const half*>(TK),
                       reinterpret_cast<const half*>(TV), tree_layer_stride, reinterpret_cast<half*>(K),

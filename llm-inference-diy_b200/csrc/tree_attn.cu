@@ -92,7 +92,6 @@ struct TaArgs {
     int npt;   // nodes per M tile
     int mt;    // M tiles of a kv head (of the longest tree)
     int W;     // flat: most CTAs that share the tiles of one M tile
-    int direct;
     int evict_first;
 };
 
@@ -389,7 +388,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         __syncwarp();
         named_bar_arrive(1, kTaThreads);
     }
-    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;  // P(j) at tP + 32 * (j & 1), or (TWO) at tP, its low terms at tP + 32
+    // P(j) at tP + 32 * (j & 1), or (TWO) at tP and its low terms at tP + 32
+    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;
 
     if (warp == 4 && work) {
         if (lane == 0) {
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         reinterpret_cast<float2*>(s.q[0])[tid] = make_float2(-INFINITY, 0.f);  // no tile for this CTA
     }
     if (DIRECT && C > 1) {
-        // ---------------- the cluster's parts of the unit's rows row r by CTA r C / rows
+        // ---------------- the cluster's parts of the unit joined, each CTA a share of the rows
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (m0 < c.n) {
             const int kvh = c.unit;
@@ -877,15 +877,15 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
 
 // ------------------------------------------------------------------ host
 int ta_sms() {
-    static int sms[64] = {};
+    static std::atomic<int> known[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (!sms[dev]) {
-        int n = 0;
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-        sms[dev] = n > 0 ? n : 148;
+    int n = known[dev];
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        known[dev] = n;
     }
-    return sms[dev];
+    return n;
 }
 
 struct TaPlan {
@@ -965,7 +965,6 @@ int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cl
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= 64 || !set[dev])) {
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess && dev >= 0 && dev < 64) set[dev] = true;
     }
     if (e != cudaSuccess) return (int)e;
@@ -1002,7 +1001,7 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     auto a16 = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     const TaPlan p = ta_plan(B, N, num_heads, num_kv_heads, max_len);
     if (!p.ok || !a16(Q) || !a16(K) || !a16(V) || !a16(TK) || !a16(TV) || !a16(O) || !len || !mask ||
-        (reinterpret_cast<uintptr_t>(mask) & 7) || ldq < num_heads * kTaDim || (ldq & 7) || ldo < num_heads * kTaDim ||
+        (reinterpret_cast<uintptr_t>(mask) & 7) || !words_aligned(slot, len, tree_len) || ldq < num_heads * kTaDim || (ldq & 7) || ldo < num_heads * kTaDim ||
         (ldo & 7) || stride < num_kv_heads * kTaDim || (stride & 7) || slot_rows <= 0 || num_slots <= 0 ||
         max_len > slot_rows || (long long)num_slots * slot_rows > 0x7fffffffLL || !a16(work) ||
         work_bytes < (kTaCtl + p.floats) * sizeof(float))
@@ -1040,20 +1039,20 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     a.evict_first = p.npt >= N;  // one M tile: every K/V row is read once
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int* err = reinterpret_cast<int*>(work);
-    a.direct = p.cluster > 0;
-    const dim3 grid = a.direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W * p.mt);
+    const bool direct = p.cluster > 0;
+    const dim3 grid = direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W * p.mt);
     const int cluster = std::max(1, p.cluster);
     int rc;
     if (p.rows <= 64 && (long long)B * N * num_heads <= kTaTwoTermRows)
-        rc = a.direct ? ta_launch<64, 3, 3, true, true>(m, a, err, grid, cluster, st)
+        rc = direct ? ta_launch<64, 3, 3, true, true>(m, a, err, grid, cluster, st)
                       : ta_launch<64, 3, 3, false, true>(m, a, err, grid, cluster, st);
     else if (p.rows <= 64)
-        rc = a.direct ? ta_launch<64, 3, 3, true, false>(m, a, err, grid, cluster, st)
+        rc = direct ? ta_launch<64, 3, 3, true, false>(m, a, err, grid, cluster, st)
                       : ta_launch<64, 3, 3, false, false>(m, a, err, grid, cluster, st);
     else
-        rc = a.direct ? ta_launch<128, 3, 2, true, false>(m, a, err, grid, cluster, st)
+        rc = direct ? ta_launch<128, 3, 2, true, false>(m, a, err, grid, cluster, st)
                       : ta_launch<128, 3, 2, false, false>(m, a, err, grid, cluster, st);
-    if (rc || a.direct || p.W < 2) return rc;
+    if (rc || direct || p.W < 2) return rc;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((p.W - 1) * p.mt);
     lc.blockDim = dim3(kTaMergeWarps * 32);

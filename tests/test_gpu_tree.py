@@ -324,6 +324,25 @@ def test_softmax_nan_and_inf():
     assert np.all(got[1] == np.float32(1 / 40)) and np.all(got[3] == np.float32(1 / 40))
 
 
+def test_softmax_extreme_temperatures():
+    """The largest and smallest temperatures, infinity and NaN: entries of -inf stay 0 and no NaN appears."""
+    t = torch()
+    V, temps = 300, [np.inf, 3e38, 1e30, 1e-30, 1e-44, np.nan, -np.inf]
+    rng = np.random.default_rng(11)
+    x = np.tile((rng.standard_normal(V) * 4).astype(np.float16), (len(temps), 1))
+    x[:, 5::7] = -np.inf
+    top = x[0] == x[0].max()
+    out = t.zeros((len(temps), V), device="cuda")
+    L.softmax_rows(_ptr(_dev(x)), V, _ptr(_dev(np.array(temps, np.float32))), len(temps), V, _ptr(out), V)
+    t.cuda.synchronize()
+    got = out.cpu().numpy().astype(np.float64)
+    flat = np.where(np.isinf(x[0]), 0.0, 1.0 / np.isfinite(x[0]).sum())
+    sharp = np.where(top, 1.0 / top.sum(), 0.0)
+    for r, want in enumerate([flat] * 3 + [sharp] * 4):
+        # equal shares but for the quotient's and the exponential's roundings; exponents below 2^-20 vanish
+        assert np.all(np.abs(got[r] - want) <= want * 2.0 ** -20), (r, temps[r])
+
+
 # ------------------------------------------------------------------ verification
 def _verify(target, draft, token, parent, u, tree_len=None, pad=0):
     t = torch()

@@ -144,3 +144,17 @@ def test_verification_rule_is_lossless(deterministic):
                 path, nxt = tm.verify(target, dr, tok, par, 3, [0.999999, ra + eps, rb + eps])
                 assert path == [] and nxt == int(np.nonzero(w2 > 0)[0][-1])
     assert np.allclose(out, p[0], atol=1e-12)
+
+
+@pytest.mark.parametrize("call,good,bad", [
+    (L.tree_rope, ROPE, k) for k in (dict(depth=A + 2), dict(lens=A + 1), dict(tree_len=A + 2))] + [
+    (L.softmax_rows, SOFT, k) for k in (dict(temp=A + 2), dict(V=2 ** 30 + 1, ldl=2 ** 30 + 1, ldp=2 ** 30 + 1))] + [
+    (L.tree_verify, VER, k) for k in (
+        dict(token=A + 2), dict(parent=A + 1), dict(tree_len=A + 2), dict(uniform=A + 2), dict(path=A + 3),
+        dict(accepted=A + 2), dict(next_token=A + 2), dict(V=2 ** 30 + 1, ldt=2 ** 30 + 1, ldd=2 ** 30 + 1))] + [
+    (L.tree_attn, ATTN, k) for k in (dict(slot=A + 2), dict(lens=A + 2), dict(tree_len=A + 1))] + [
+    (L.tree_commit, COM, k) for k in (
+        dict(slot=A + 2), dict(lens=A + 1), dict(path=A + 2), dict(accepted=A + 2), dict(len_out=A + 18))])
+def test_refuses_misaligned_words_and_overlong_rows(call, good, bad):
+    with pytest.raises(L.LlmdiyError, match=REFUSED):
+        call(**{**good, **bad})
