@@ -2,14 +2,20 @@
 // (include/llmdiy_tree.h).  No counterpart in the reference, whose engine takes the argmax only.
 //
 // One pass over memory, by persistent clusters of C CTAs: cluster c takes rows c, c + clusters, ..., slice k of
-// a row in CTA k.  Bulk copies bring the next two rows' slices into shared memory while a row is
-// worked on; its entries go to registers, which frees their stage for the copy after next.  Each CTA finds
-// its slice's maximum m_c and its sum s_c of exponentials relative to it (kept in registers as
-// fp32); one exchange of the C pairs through distributed shared memory (asynchronous stores that complete on the
-// receiver's mbarrier: a cluster barrier would also wait for the last row's output to be written) gives
-// the row's maximum M and sum S = sum_c s_c 2^{(m_c - M) k}, k = log2(e) / t, and every thread writes its share times
-// 2^{(m_c - M) k} / S.  x - m is exact in fp32 for fp16 x (but for far smaller x, whose share is 0), so the
-// exponent carries two roundings (k and the product).  Reading 2 and writing 4 bytes an entry is the bound.
+// a row in CTA k, each warp a run of it.  Bulk copies bring the next two rows' slices into shared memory while a row
+// is worked on; its entries go to registers.  Each warp finds its run's maximum m_w and its sum s_w of exponentials
+// relative to it (kept in registers as fp32) and sends the pair to every CTA of the cluster by asynchronous stores
+// that complete on the receiver's mbarrier; with all the pairs it forms the row's maximum M and sum
+// S = sum_w s_w 2^{(m_w - M) k}, k = log2(e) / t, and writes its run times 2^{(m_w - M) k} / S.  With C > 1 no barrier stands in the
+// loop.  x - m is exact in fp32 for fp16 x (but for far smaller x, whose share is 0), so
+// the exponent carries two roundings (k and the product).
+//
+// Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 139.6 us, 5.0 TB/s of the 6.5 of
+// a copy.  A row is in work for about 6 us (shared-memory loads, 16 warps' exponentials, the exchange, and 76 KB of
+// output at up to 32 bytes a cycle and SM), with 33 clusters of 8 resident.  Rejected: the whole CTA's maximum and sum
+// by barriers (141.7 us), results through shared memory and bulk stores (140.8, and 6.0 us against 5.5 for 9 rows),
+// clusters of 9 to 16 (158 to 311: a row takes as long, and fewer are in work), fp16 entries held and
+// their exponentials taken twice (188).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -25,6 +31,8 @@ namespace {
 constexpr int kSmThreads = 512;
 constexpr int kSmPairs = 20;                                  // pairs of entries a thread holds
 constexpr int kSmSlice = kSmThreads * kSmPairs * 2 - 8;       // entries a CTA holds (pairs may start one entry early)
+constexpr int kSmWarps = kSmThreads / 32;
+constexpr int kSmRun = kSmPairs * 64;                         // a warp's run of entries
 constexpr int kSmStages = 2;
 // A stage: eight entries before the slice's first granule, the granules, and room for every thread's pairs
 constexpr int kSmStageBytes = (16 + (kSmThreads * kSmPairs * 2 + 16) * 2 + 127) / 128 * 128;
@@ -67,7 +75,14 @@ LLMDIY_DEV void sm_send(float2* dst, uint64_t* bar, uint32_t rank, float a, floa
                  "f"(a), "f"(b), "r"(m)
                  : "memory");
 }
-LLMDIY_DEV float2 sm_floats(uint32_t w) { return __half22float2(*reinterpret_cast<const half2*>(&w)); }
+// x + c for both fp16 halves x of w, in fp32 (one instruction each, without a conversion)
+LLMDIY_DEV float2 sm_add_halves(uint32_t w, float c) {
+    float2 r;
+    asm("{\n .reg .f16 a, b;\n mov.b32 {a, b}, %2;\n add.f32.f16 %0, a, %3;\n add.f32.f16 %1, b, %3;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(w), "f"(c));
+    return r;
+}
 
 // The 16-byte granules around entries [v0, v0 + n) of a row, cut at the ends of the whole buffer
 // [first, last): what a bulk copy brings.  `lead`: where entry v0 lies in a stage, in entries.
@@ -92,10 +107,11 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
                    float* probs, int ldp) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(128) uint8_t stage[];  // [kSmStages][kSmStageBytes]
-    __shared__ float red_m[kSmThreads / 32], red_s[kSmThreads / 32];
-    __shared__ float2 part[2][kSmMaxCluster];  // (m_c, s_c) of the cluster's CTAs: odd and even rows
+    __shared__ float2 part[2][kSmMaxCluster * kSmWarps];  // (m_w, s_w) of the cluster's warps: odd and even rows
     __shared__ uint64_t full[kSmStages], got[2];
     cg::cluster_group cluster = cg::this_cluster();
+    // whether some copy begins or ends inside a granule
+    const bool edges = (reinterpret_cast<uintptr_t>(logits) & 15) || (ldl & 7) || (V & 7);
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r0 = blockIdx.x / C, step = gridDim.x / C;
@@ -139,31 +155,36 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         const float t = temp ? temp[r] : 1.f;
         const SmWindow win = sm_window(x, held, first, last);
         uint16_t* sx = reinterpret_cast<uint16_t*>(stage + st * kSmStageBytes + 16) + win.lead;
-        const bool ok = mbar_wait(&full[st], (it / kSmStages) & 1);
+        // pairs begin where 8-byte stores of the output do
+        const int odd = (int)(reinterpret_cast<uintptr_t>(y) >> 2) & 1;
+        const int run0 = warp * kSmRun - odd;  // this warp's entries: [run0, run0 + kSmRun) of the slice
+        bool ok = mbar_wait(&full[st], (it / kSmStages) & 1);
         // The copy's first and last granules hold up to seven entries of the rows beside this slice, and the
         // last row in this stage may have ended up to fourteen entries further on: -inf for those; and
-        // where the whole buffer ends inside a granule, its entries come from global memory.
-        if (tid < 40) {
+        // where the whole buffer ends inside a granule, its entries come from global memory.  Each warp sees to its own run.
+        if (edges) {
             const uintptr_t xa = reinterpret_cast<uintptr_t>(x);
             const int c0 = win.from > xa ? (int)(win.from - xa) / 2 : 0;
             const int c1 = win.to > xa ? min(held, (int)((win.to - xa) / 2)) : 0;
-            const int a = tid < 16 ? tid - 8 : max(held - 8, 8) + tid - 16;  // -8 .. 7 and held - 8 .. held + 15
-            const bool in = a >= 0 && a < held;
-            if (!in) sx[a] = 0xFC00;
-            else if (a < c0 || a >= c1) sx[a] = x[a];
+            for (int i = lane; i < 40; i += 32) {
+                const int a = i < 16 ? i - 8 : max(held - 8, 8) + i - 16;  // -8 .. 7 and held - 8 .. held + 15
+                if (a < run0 || a >= run0 + kSmRun) continue;
+                const bool in = a >= 0 && a < held;
+                if (!in) sx[a] = 0xFC00;
+                else if (a < c0 || a >= c1) sx[a] = x[a];
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a later copy writes there too
+            __syncwarp();
         }
-        __syncthreads();
-        // pairs begin where 8-byte stores of the output do
-        const int odd = (int)(reinterpret_cast<uintptr_t>(y) >> 2) & 1;
-        const uint16_t* mine = sx - odd + 2 * tid;
+        const uint16_t* mine = sx + run0 + 2 * lane;
         uint32_t w[kSmPairs];
         if (((win.lead - odd) & 1) == 0) {
 #pragma unroll
-            for (int i = 0; i < kSmPairs; ++i) w[i] = *reinterpret_cast<const uint32_t*>(mine + 2 * i * kSmThreads);
+            for (int i = 0; i < kSmPairs; ++i) w[i] = *reinterpret_cast<const uint32_t*>(mine + 64 * i);
         } else {
 #pragma unroll
             for (int i = 0; i < kSmPairs; ++i)
-                w[i] = sm_pair(mine[2 * i * kSmThreads], mine[2 * i * kSmThreads + 1]);
+                w[i] = sm_pair(mine[64 * i], mine[64 * i + 1]);
         }
         half2 h = __half2half2(__ushort_as_half(0xFC00));
 #pragma unroll
@@ -172,23 +193,17 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) m = fmaxf(m, h2f(__ushort_as_half(x[a])));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) red_m[warp] = m;
-        __syncthreads();  // the stage has been read
-        if (tid == 0 && row + (long long)kSmStages * step < R) copy((int)row + kSmStages * step, st);
-        m = red_m[lane & (kSmThreads / 32 - 1)];
-#pragma unroll
-        for (int o = kSmThreads / 64; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         // k is bounded so that 0 * k is 0 and -inf * k is -inf at any t > 0; greedy (t <= 0 or NaN) takes the upper
         // bound, where the smallest difference of two fp16 values gives 2^-inf
         const float k = t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1e-30f), 1e30f) : 1e30f;
         auto weight = [&](float v, float top) { return sm_ex2((v - top) * k); };
         const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: every weight 0
         uint64_t ex[kSmPairs], s2[2] = {0, 0};
-        const uint64_t minus = sm_f2(-ref, -ref), k2 = sm_f2(k, k);
+        const uint64_t k2 = sm_f2(k, k);
 #pragma unroll
         for (int i = 0; i < kSmPairs; ++i) {
-            const float2 f = sm_floats(w[i]);
-            const float2 d = sm_split(sm_mul2(sm_add2(sm_f2(f.x, f.y), minus), k2));
+            const float2 f = sm_add_halves(w[i], -ref);
+            const float2 d = sm_split(sm_mul2(sm_f2(f.x, f.y), k2));
             ex[i] = sm_f2(sm_ex2(d.x), sm_ex2(d.y));
             s2[i & 1] = sm_add2(s2[i & 1], ex[i]);
         }
@@ -197,43 +212,53 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) s += weight(h2f(__ushort_as_half(x[a])), ref);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) red_s[warp] = s;
-        __syncthreads();
-        float M = m, total = red_s[lane & (kSmThreads / 32 - 1)];
-#pragma unroll
-        for (int o = kSmThreads / 64; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (!ok) total = NAN;  // a copy that never landed shows in its row
+        if (!ok) s = NAN;  // a copy that never landed shows in its row
+        // Two tables take turns: a warp sends row i + 2's pair only after every warp's pair of row i + 1 has come,
+        // which each sends after it has read row i's table.
+        float2* tab = part[it & 1];
         if (C > 1) {
-            // Two tables take turns: a CTA sends row i + 2's pair only after every CTA's pair of row i + 1 has come,
-            // which each sends after it has read row i's table.
-            float2* tab = part[it & 1];
-            if (tid == 0) mbar_arrive_expect_tx(&got[it & 1], C * 8);
-            if (tid < C) sm_send(&tab[rank], &got[it & 1], tid, m, total);
-            const bool all = mbar_wait(&got[it & 1], (it >> 1) & 1);
-            const float2 q = tab[lane & (C - 1)];
-            M = q.x;
-            for (int o = C / 2; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            total = q.y * (q.x == -INFINITY ? 1.f : weight(q.x, M));  // (q.x = -inf: a sum of 0, or NaN)
-            for (int o = C / 2; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            if (!all) total = NAN;
+            if (tid == 0) mbar_arrive_expect_tx(&got[it & 1], C * kSmWarps * 8);
+            if (lane < C) sm_send(&tab[rank * kSmWarps + warp], &got[it & 1], lane, m, s);
+            ok = mbar_wait(&got[it & 1], (it >> 1) & 1);
+        } else {  // (a barrier is quicker within one CTA: a row of 8192 entries 3.7 us against 4.4)
+            if (lane == 0) tab[warp] = make_float2(m, s);
+            __syncthreads();
         }
+        // (every warp has sent its pair, so it has read the stage)
+        if (tid == 0 && row + (long long)kSmStages * step < R) copy((int)row + kSmStages * step, st);
+        float2 q[kSmMaxCluster * kSmWarps / 32];
+        float M = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int j = 0; j < kSmMaxCluster * kSmWarps / 32; ++j) {
+            const int at = lane + 32 * j;
+            q[j] = at < C * kSmWarps ? tab[at] : make_float2(-INFINITY, 0.f);
+            M = fmaxf(M, q[j].x);
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll
+        for (int j = 0; j < kSmMaxCluster * kSmWarps / 32; ++j)  // (q.x = -inf: a sum of 0, or NaN)
+            total += q[j].y * (q[j].x == -INFINITY ? 1.f : weight(q[j].x, M));
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (!ok) total = NAN;
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const float top = M == -INFINITY ? 0.f : M;
         const float scale = inv * (m == -INFINITY ? 1.f : weight(m, top));
-        float2* out = reinterpret_cast<float2*>(y - odd) + tid;
-        const int room = held + odd - 2 * tid;           // entries from this thread's first on
-        const int whole = (held + odd) / (2 * kSmThreads);  // runs that lie inside the slice as a whole
-        const bool head = odd && tid == 0;               // the pair that begins one entry early
+        float* out = y + run0 + 2 * lane;
+        const int room = held - run0 - 2 * lane;  // entries from this thread's first on
+        const int whole = (held - run0) / 64;     // pairs' runs that lie inside the slice as a whole
+        const bool head = odd && tid == 0;        // the pair that begins one entry early
         const uint64_t scale2 = sm_f2(scale, scale);
 #pragma unroll
         for (int i = 0; i < kSmPairs; ++i) {
             const float2 o = sm_split(sm_mul2(ex[i], scale2));
             if (i == 0 && head) {
                 if (held > 0) y[0] = o.y;
-            } else if (i < whole || 2 * i * kSmThreads + 1 < room) {
-                out[i * kSmThreads] = o;
-            } else if (2 * i * kSmThreads + 1 == room) {
-                out[i * kSmThreads].x = o.x;
+            } else if (i < whole || 64 * i + 1 < room) {
+                *reinterpret_cast<float2*>(out + 64 * i) = o;
+            } else if (64 * i + 1 == room) {
+                out[64 * i] = o.x;
             }
         }
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
@@ -271,9 +296,10 @@ extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float*
     if (!logits || !probs || R <= 0 || V <= 0 || V > (1 << 30) || ldl < V || ldp < V ||
         (reinterpret_cast<uintptr_t>(logits) & 1) || !words_aligned(probs, temp))
         return (int)cudaErrorInvalidValue;
-    // CTAs per row: enough to hold it, and more while they leave SMs idle and a slice stays above 4096 entries
+    // CTAs per row: a power of two that holds it.  (Twice as many gained 0.2 us of 4.9 at 32000 entries up to 16 rows and lost
+    // from 32 on, 5.7 against 5.0; at 8192 entries they cost 0.9 of 3.6.)
     int C = 1;
-    while (C < kSmMaxCluster && ((V + C - 1) / C > kSmSlice || ((long long)R * C < 74 && V / C >= 8192))) C *= 2;
+    while (C < kSmMaxCluster && (V + C - 1) / C > kSmSlice) C *= 2;
     const int slice = (((V + C - 1) / C) + 7) / 8 * 8;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(std::min(R, sm_clusters(C)) * C);
