@@ -235,6 +235,11 @@ LLMDIY_DEV void ta_store4(half* dst, const float4& v, float scale) {
     u.y = *reinterpret_cast<const uint32_t*>(&y1);
     *reinterpret_cast<uint2*>(dst) = u;
 }
+LLMDIY_DEV void ta_store8(float* dst, const float* v) {  // 32 bytes, a whole sector
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
 LLMDIY_DEV bool elect_one() {  // one lane of a converged warp
     uint32_t p;
     asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(p));
@@ -737,13 +742,16 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                         for (int e = 0; e < 32; ++e) v[e] *= inv;
 #pragma unroll
                         for (int e = 0; e < 32; e += 8) *reinterpret_cast<uint4*>(dst + q + e) = pack8(v + e);
-                    } else {
+                    } else if (DIRECT) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
                             // (16-byte pieces of a row turned by the row: 32 rows' stores meet different banks)
-                            float* to = DIRECT ? own + (((q + e) / 4) ^ lane) * 4 : pdst + q + e;
+                            float* to = own + (((q + e) / 4) ^ lane) * 4;
                             *reinterpret_cast<float4*>(to) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) ta_store8(pdst + q + e, v + e);
                     }
                 }
                 if (live && !whole && !DIRECT)
@@ -952,7 +960,8 @@ bool make_query_map(CUtensorMap* m, const void* base, int nodes, int H, int ldq,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr size_t kTaCtl = 4;  // floats before the partials: word 0 is the error word
+constexpr size_t kTaCtl = 8;  // floats before the partials, which begin on 32 bytes: word 0 is the error word
+size_t ta_work_bytes(const TaPlan& p) { return (kTaCtl + p.floats) * sizeof(float); }
 
 template <int QR, int KS, int VS, bool DIRECT, bool TWO>
 int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cluster, cudaStream_t st) {
@@ -991,7 +1000,7 @@ extern "C" {
 
 size_t llmdiy_tree_attn_work_bytes(int B, int N, int num_heads, int num_kv_heads, int max_len) {
     const TaPlan p = ta_plan(B, N, num_heads, num_kv_heads, max_len);
-    return p.ok ? (kTaCtl + p.floats) * sizeof(float) : 0;
+    return p.ok ? ta_work_bytes(p) : 0;
 }
 
 int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16_t* V, int stride, int slot_rows,
@@ -1004,7 +1013,7 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
         (reinterpret_cast<uintptr_t>(mask) & 7) || !words_aligned(slot, len, tree_len) || ldq < num_heads * kTaDim || (ldq & 7) || ldo < num_heads * kTaDim ||
         (ldo & 7) || stride < num_kv_heads * kTaDim || (stride & 7) || slot_rows <= 0 || num_slots <= 0 ||
         max_len > slot_rows || (long long)num_slots * slot_rows > 0x7fffffffLL || !a16(work) ||
-        work_bytes < (kTaCtl + p.floats) * sizeof(float))
+        work_bytes < ta_work_bytes(p))
         return (int)cudaErrorInvalidValue;
     CUtensorMap m[5];
     const int cols = num_kv_heads * kTaDim;
@@ -1022,7 +1031,7 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     a.TK = reinterpret_cast<const half*>(TK);
     a.TV = reinterpret_cast<const half*>(TV);
     a.O = reinterpret_cast<half*>(O);
-    a.part = work + kTaCtl;
+    a.part = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(work) & ~(uintptr_t)31) + kTaCtl * 4);
     a.B = B;
     a.N = N;
     a.H = num_heads;
