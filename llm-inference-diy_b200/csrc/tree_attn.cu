@@ -1,6 +1,9 @@
 // tree_attn.cu — attention of a tree of drafted tokens over the cache (include/llmdiy_tree.h), on the
 // tcgen05 tensor cores.  No counterpart in the reference, which attends one query token per step.
 //
+// (Units of one to four query rows with short caches have a kernel of their own on the CUDA cores, tree_attn_few.cuh: a
+// CTA's setup of TMEM, tensor maps and MMAs costs more there than the products.)
+//
 // Work.  A unit is (sequence, kv head, M tile): the query rows m = node * G + g of the G heads that share the kv
 // head, at most 128 rows (the MMA's M) of whole nodes.  A unit's keys are 64-row tiles: the cache
 // rows [0, len), then the tree's own rows.  Two ways to share them out (ta_plan):
@@ -883,6 +886,8 @@ __global__ void __launch_bounds__(kTaMergeWarps * 32) tree_merge_k(const __grid_
     }
 }
 
+#include "tree_attn_few.cuh"
+
 // ------------------------------------------------------------------ host
 int ta_sms() {
     static std::atomic<int> known[64];
@@ -899,6 +904,7 @@ int ta_sms() {
 struct TaPlan {
     int G, npt, rows, mt, W;  // W: flat CTAs per M tile
     int cluster;  // direct: CTAs per unit (0: flat)
+    int few;      // CTAs per unit of the kernel for few rows (0: not that one)
     bool ok;
     size_t floats;  // of the flat partials
 };
@@ -921,6 +927,15 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     // flat CTAs have four tiles or more
     p.W = (int)std::max<long long>(1, std::min<long long>(slots / p.mt, units / p.mt * tiles / 4));
     p.floats = (size_t)std::min<long long>(slots, units * tiles) * 2 * p.rows * (kTaDim + 2);
+    // Units of up to four rows whose CTAs' shares are short go to the kernel for those: the products of a CTA, rows x
+    // cache rows, decide.  Measured (this kernel / the one for few rows): 16 units of 1 row over 1023 9.4 / 5.6, over 8192
+    // (1024 a CTA) 23.4 / 19.9, over 131072 183 / 243; 2 rows over 4096 (512 a CTA) 15.7 / 13.8, over 8192 23.8 / 23.3; 4 over
+    // 1023 9.6 / 7.9, over 4000 (500 a CTA) 15.5 / 20.0; 32 units of 4 over 2048 (256 a CTA) 13.4 / 14.4; 1024 units of 1
+    // over up to 300 36.7 / 26.5, over up to 1000 57.6 / 52.2.
+    if (p.rows <= kFewRows) {
+        const int c = (int)std::max<long long>(1, std::min<long long>({kTaMaxCluster, slots / units, (max_len + 63) / 64}));
+        if ((long long)p.rows * ((max_len + c - 1) / c) <= (p.rows <= 2 ? 1024 : 768)) p.few = c;
+    }
     // Direct or flat, by what both would take if every sequence were max_len long, in us.  A CTA that runs its chain of
     // products undisturbed needs 0.75 a tile (1.0 with more than 32 rows), and all slots together 1.46 a tile and slot from
     // HBM; a flat call pays for its second launch and for joining W / units partials a row.  Of sequences
@@ -1015,13 +1030,6 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
         max_len > slot_rows || (long long)num_slots * slot_rows > 0x7fffffffLL || !a16(work) ||
         work_bytes < ta_work_bytes(p))
         return (int)cudaErrorInvalidValue;
-    CUtensorMap m[5];
-    const int cols = num_kv_heads * kTaDim;
-    if (!make_query_map(&m[0], Q, B * N, num_heads, ldq, p.G, p.npt) ||
-        !make_kmajor_map(&m[1], K, num_slots * slot_rows, cols, stride, kTaKeys) ||
-        !make_kmajor_map(&m[2], V, num_slots * slot_rows, cols, stride, kTaKeys) ||
-        !make_kmajor_map(&m[3], TK, B * N, cols, cols, kTaKeys) || !make_kmajor_map(&m[4], TV, B * N, cols, cols, kTaKeys))
-        return (int)cudaErrorInvalidValue;
     TaArgs a = {};
     a.slot = slot;
     a.len = len;
@@ -1048,6 +1056,19 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     a.evict_first = p.npt >= N;  // one M tile: every K/V row is read once
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int* err = reinterpret_cast<int*>(work);
+    if (p.few) {
+        const half *hk = reinterpret_cast<const half*>(K), *hv = reinterpret_cast<const half*>(V);
+        return p.rows == 1   ? few_launch<1, 8>(a, hk, hv, stride, err, p.few, st)
+               : p.rows == 2 ? few_launch<2, 8>(a, hk, hv, stride, err, p.few, st)
+                             : few_launch<4, 4>(a, hk, hv, stride, err, p.few, st);
+    }
+    CUtensorMap m[5];
+    const int cols = num_kv_heads * kTaDim;
+    if (!make_query_map(&m[0], Q, B * N, num_heads, ldq, p.G, p.npt) ||
+        !make_kmajor_map(&m[1], K, num_slots * slot_rows, cols, stride, kTaKeys) ||
+        !make_kmajor_map(&m[2], V, num_slots * slot_rows, cols, stride, kTaKeys) ||
+        !make_kmajor_map(&m[3], TK, B * N, cols, cols, kTaKeys) || !make_kmajor_map(&m[4], TV, B * N, cols, cols, kTaKeys))
+        return (int)cudaErrorInvalidValue;
     const bool direct = p.cluster > 0;
     const dim3 grid = direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W * p.mt);
     const int cluster = std::max(1, p.cluster);

@@ -126,6 +126,48 @@ def test_attn_matches(B, N, H, KV, lens):
     Attn(B * 1000 + N, B, N, H, KV, lens).device().call().check(rows=400)
 
 
+@pytest.mark.parametrize("B,N,H,KV,lens,tree_len", [
+    (1, 1, 1, 1, [0], None), (1, 1, 4, 4, [1], None), (2, 1, 2, 2, [15, 17], None), (1, 1, 3, 3, [8200], None),
+    (1, 2, 4, 4, [511], None), (3, 2, 6, 3, [0, 129, 300], [2, 1, 2]), (1, 4, 2, 2, [1000], None),
+    (4, 4, 2, 2, [5, 0, 64, 700], [0, 4, 3, 1]), (2, 1, 12, 4, [63, 513], None), (2, 3, 2, 2, [100, 0], [3, 9]),
+    (40, 1, 16, 16, [7 * i for i in range(40)], None), (70, 1, 8, 2, [5 * i for i in range(70)], [i % 3 for i in range(70)]),
+    (1, 2, 4, 2, [300], None), (1, 4, 4, 4, [2500], None), (300, 2, 2, 2, [i % 37 for i in range(300)], None)])
+def test_attn_of_one_to_four_rows(B, N, H, KV, lens, tree_len):
+    """Units of one to four query rows: lengths on either side of a half warp's and a CTA's share, empty trees, one CTA
+    and several per unit, short and long shares, padded rows, slots in another order; the same bits again."""
+    a = Attn(B * 77 + N, B, N, H, KV, lens, tree_len=tree_len, slots=list(range(B))[::-1], pad=8).device().call()
+    first = a.d["O"].clone()
+    a.call()
+    torch().cuda.synchronize()
+    assert torch().equal(a.d["O"], first)
+    if tree_len:
+        a.tree_len = [min(n, N) for n in tree_len]
+    a.check(rows=300)
+
+
+@pytest.mark.parametrize("length", [0, 30, 400])
+def test_attn_of_few_rows_nothing_leaks(length):
+    """Two and four rows: Inf and NaN in cache rows past the length and in tree rows that a node does not see; rows
+    that see nothing give zeros; one that sees a NaN score is NaN."""
+    t = torch()
+    for N, H, KV in ((2, 2, 2), (4, 3, 3), (1, 4, 1)):
+        sees = [[set(), {1}, {0, 1}, {3}][:N]]
+        a = Attn(9 + length, 1, N, H, KV, [length], max_len=length + 60, sees=sees)
+        a.K[0, length:], a.V[0, length:] = np.nan, np.inf
+        a.TK[0, 0] = np.nan if N < 3 else a.TK[0, 0]
+        a.TV[0, 0] = -np.inf if N < 3 else a.TV[0, 0]
+        if N == 4:
+            a.TV[0, 2] = a.TK[0, 2] = np.nan
+        a.device().call().check()
+        if length == 0:
+            assert t.all(a.d["O"][0, 0, :H * D] == 0)
+    a = Attn(3, 1, 2, 2, 2, [50])
+    a.K[0, 49, :D] = np.nan
+    a.device().call()
+    t.cuda.synchronize()
+    assert t.isnan(a.d["O"][0, :, :D]).all() and not t.isnan(a.d["O"][0, :, D:2 * D]).any()
+
+
 def test_attn_strides_slots_and_ragged_trees():
     """Padded rows, slots of a larger pool in mixed order, trees of different sizes (one empty), lengths
     past max_len, negative lengths and slots that do not exist."""
