@@ -8,7 +8,7 @@
 // head, at most 128 rows (the MMA's M) of whole nodes.  A unit's keys are 64-row tiles: the cache
 // rows [0, len), then the tree's own rows.  Two ways to share them out (ta_plan):
 //
-// Direct: a cluster of C CTAs per unit, its tiles in C equal runs; the CTAs' parts (o unnormalised, m, l) are
+// Direct: a cluster of C <= 16 CTAs per unit, its tiles in C equal runs; the CTAs' parts (o unnormalised, m, l) are
 // joined through distributed shared memory, each CTA finishing a share of the rows.  One launch, no global
 // scratch.
 //
@@ -63,7 +63,7 @@ constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0
 constexpr int kTaTwoTermRows = 128;
 constexpr int kTaDirectTiles = 48;  // (see ta_plan)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
-constexpr int kTaMaxCluster = 8;  // (clusters of 16 do not all run at once: 16 x 16 CTAs took 24.6 us, 16 x 8 13.7)
+constexpr int kTaCluster = 8;     // CTAs per unit (direct); long caches of few units take 12 or 16 (see ta_plan)
 constexpr int kTaUnitCost = 4;  // a unit's beginning and end take about as long as four tiles
 
 // Two layouts of the same kernel: units of up to 64 rows need only 16 KB for Q and get a third V
@@ -933,7 +933,7 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     // 1023 9.6 / 7.9, over 4000 (500 a CTA) 15.5 / 20.0; 32 units of 4 over 2048 (256 a CTA) 13.4 / 14.4; 1024 units of 1
     // over up to 300 36.7 / 26.5, over up to 1000 57.6 / 52.2.
     if (p.rows <= kFewRows) {
-        const int c = (int)std::max<long long>(1, std::min<long long>({kTaMaxCluster, slots / units, (max_len + 63) / 64}));
+        const int c = (int)std::max<long long>(1, std::min<long long>({kFewCluster, slots / units, (max_len + 63) / 64}));
         if ((long long)p.rows * ((max_len + c - 1) / c) <= (p.rows <= 2 ? 1024 : 768)) p.few = c;
     }
     // Direct or flat, by what both would take if every sequence were max_len long, in us.  A CTA that runs its chain of
@@ -942,7 +942,13 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     // of different lengths direct waits for the longest, so several of them with more than
     // kTaDirectTiles tiles a CTA go flat.  Measured (direct / flat): 16 units of 17 tiles 9.9 / 17.4, 16 of 2049 203 / 184,
     // 16 of 514 (128 rows) 78 / 68, 2 of 126 20 / 59, 1024 of up to 33 103 / 122, 256 of up to 66 67 / 67.
-    const int c = (int)std::max<long long>(1, std::min<long long>({kTaMaxCluster, slots / units, tiles}));
+    int c = (int)std::max<long long>(1, std::min<long long>({kTaCluster, slots / units, tiles}));
+    // Clusters of 12 or 16 for many tiles, where the units' all run at once: such clusters leave gaps, 21 and 14 of them fit
+    // on 148 SMs (16 x 16 CTAs do not, and took 17.6 us against 10.7), so three quarters of the slots are counted.
+    // Measured (8 / 16 CTAs), 8 units of 34 tiles 11.7 / 13.4, 2 of 65 14.7 / 11.2, 8 of 129 18.7 / 14.9; (8 / 12), 16
+    // of 34 10.7 / 10.7, of 129 23.8 / 21.1.
+    if (tiles > 6 * kTaCluster && c == kTaCluster)
+        c = units * 16 * 4 <= slots * 3 ? 16 : units * 12 * 4 <= slots * 3 ? 12 : c;
     const double t = (double)((tiles + c - 1) / c), chain = p.rows > 32 ? 1.0 : 0.75, hbm = 1.46 / slots;
     const double flat_ctas = (double)p.W * p.mt;
     const double direct_us = 9.0 + t * std::max(chain, hbm * std::min<double>(slots, units * c));
@@ -989,6 +995,7 @@ int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cl
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= 64 || !set[dev])) {
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess && dev >= 0 && dev < 64) set[dev] = true;
     }
     if (e != cudaSuccess) return (int)e;

@@ -15,7 +15,8 @@
 
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kFewRows = 4;  // most query rows of a unit
+constexpr int kFewRows = 4;     // most query rows of a unit
+constexpr int kFewCluster = 8;  // most CTAs of a unit
 
 LLMDIY_DEV void few_send4(float4* dst, uint64_t* bar, uint32_t rank, const float4& v) {
     uint32_t d, m;
@@ -68,8 +69,8 @@ LLMDIY_DEV void few_unpack(const uint4& v, uint64_t* x) {  // eight halves as fo
 template <int R, int U>
 __global__ void __launch_bounds__(kFewThreads, 2)
     tree_attn_few_k(const __grid_constant__ TaArgs a, const half* K, const half* V, int stride, int* err) {
-    __shared__ float4 wo[kFewWarps][R][32], po[R][kTaMaxCluster][32];  // the warps' and the CTAs' parts of each row
-    __shared__ float2 wml[kFewWarps][R], pml[R][kTaMaxCluster];
+    __shared__ float4 wo[kFewWarps][R][32], po[R][kFewCluster][32];  // the warps' and the CTAs' parts of each row
+    __shared__ float2 wml[kFewWarps][R], pml[R][kFewCluster];
     __shared__ uint64_t got[R];
     const int C = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
