@@ -37,6 +37,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <atomic>
 #include <mutex>
 
@@ -924,8 +925,12 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     const long long units = (long long)B * KV * p.mt;
     p.ok = units * (tiles + kTaUnitCost) <= 0x7fffffffLL;
     const int slots = std::max(kTaCtasPerSm * ta_sms(), p.mt);
-    // flat CTAs have four tiles or more
-    p.W = (int)std::max<long long>(1, std::min<long long>(slots / p.mt, units / p.mt * tiles / 4));
+    // Flat CTAs have four tiles or more, and a unit is cut into sqrt(2 tiles) parts at most: joining costs about half as much
+    // a part as the products a tile.  1 unit of 1025 tiles, 128 rows: 47.3 us with sqrt(tiles) parts, 43.8 so,
+    // 45.2 with sqrt(5 tiles), 93.6 with 296.
+    const double parts = std::sqrt(2.0 * (double)tiles);
+    p.W = (int)std::max<long long>(
+        1, std::min<long long>({slots / p.mt, units / p.mt * tiles / 4, (long long)((double)(units / p.mt) * parts)}));
     p.floats = (size_t)std::min<long long>(slots, units * tiles) * 2 * p.rows * (kTaDim + 2);
     // Units of up to four rows whose CTAs' shares are short go to the kernel for those: the products of a CTA, rows x
     // cache rows, decide.  Measured (this kernel / the one for few rows): 16 units of 1 row over 1023 9.4 / 5.6, over 8192
