@@ -13,7 +13,7 @@
 // Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 139.6 us, 5.0 TB/s of the 6.5 of
 // a copy.  A row is in work for about 6 us (shared-memory loads, 16 warps' exponentials, the exchange, and 76 KB of
 // output at up to 32 bytes a cycle and SM), with 33 clusters of 8 resident.  Rejected: the whole CTA's maximum and sum
-// by barriers (141.7 us), results through shared memory and bulk stores (140.8, and 6.0 us against 5.5 for 9 rows),
+// by barriers (141.7 us), results through shared memory and bulk stores (140.8, and 6.0 us against 5.5 for 5 rows),
 // clusters of 9 to 16 (158 to 311: a row takes as long, and fewer are in work), fp16 entries held and
 // their exponentials taken twice (188).
 #include <cooperative_groups.h>

@@ -41,7 +41,8 @@ LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
 }
 
 // ---------------------------------------------------------------- bias + RoPE
-// One CTA per node.  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
+// One CTA per node, bound by the latency of its loads (1536 nodes of 48 heads' rows 7.5 us, 4.2 TB/s of the 6.5 of a copy, in
+// one wave and a half).  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
 // to [-pi, pi] in 64 bits (a position of 10^5 leaves fp32 angles only 2 digits after the point), its sine
 // and cosine are then taken in fp32 (absolute error < 2^-21, against 2^-11 of the fp16 outputs).  The 64
 // frequencies come as a kernel argument, and the first rows' loads are under way while the angles are computed.
@@ -117,6 +118,11 @@ __global__ void __launch_bounds__(kRopeThreads)
 // child needs the sum of max(0, p - T q) over the row, and the end of the walk its running sum.  The row is cut
 // into blocks of 128 entries, dealt contiguously to the cluster's warps (warp k of K: blocks
 // [k U / K, (k + 1) U / K)), so the warps' totals in order are a running sum over the row.
+//
+// What bounds it is the walk: a refusal needs the sum over two rows before the next child can be tried, about 2.5 us a
+// round, 1.3 of them the rows' loads and 1.2 the exchange.  V = 151936: a chain 8.8 us, 24 trees of 32 nodes 34 to 37.
+// Tried: the root's rows fetched into L2 while the tree is read (24 trees 38.9 us against 35.5), more blocks held or unrolled
+// (no gain), the weights as two fp32 terms in place of fp64 (37.5 against 36.3).
 constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerMaxCluster = 16;
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
 
 // ---------------------------------------------------------------- commit
 // One CTA per (layer, sequence, K or V); a thread copies 16-byte pieces, several loads in flight (one load at a time,
-// each behind its node's path entry, took 18.1 us for 32 x 24 caches; so 13.3).
+// each behind its node's path entry, took 18.1 us for 32 x 24 caches; so 13.3, 4.8 TB/s of the 6.5 of a copy).
 constexpr int kCommitThreads = 256;
 constexpr int kCommitBatch = 5;
 
@@ -529,8 +535,8 @@ int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd
         !words_aligned(target, draft, token, parent, tree_len, uniform, path, accepted, next))
         return (int)cudaErrorInvalidValue;
     const int vec = aligned16(target) && ldt % 4 == 0 && (!draft || (aligned16(draft) && ldd % 4 == 0));
-    // CTAs per sequence: as many as run at once (two per SM), 16 at most.  Measured at V = 151936: one
-    // chain 12.5 us with 8, 9.6 us with 16; 24 trees of 32 nodes 61 us with 4, 45 with 6, 41 with 8, 49 with 16.
+    // CTAs per sequence: as many as run at once (two per SM), 16 at most.  Measured at V = 151936 (first form): one
+    // chain 12.5 us with 8, 9.6 us with 16; 24 trees of 32 nodes 61 us with 4, 45 with 6, 41 with 8, 49 with 16 (12 now: 36).
     const int C = std::max(1, std::min(kVerMaxCluster, kVerCtasPerSm * sm_count() / B));
     cudaError_t e = ver_allow_clusters();
     if (e != cudaSuccess) return (int)e;

@@ -32,6 +32,14 @@
 // (K may hold anything there), and V rows past the end, as well as tree rows with an Inf or NaN, are zeroed in
 // shared memory before PV; the few rows that do see such a tree row add p * v themselves at the end.
 //
+// Bounds and what was measured.  Short caches: launch, barriers, TMEM and first instructions (about 7 us) and 0.75 us a tile;
+// 26 nodes x 16 heads over 2047 rows take 10.8 us (5 tiles a CTA).  Long ones: HBM for few rows (64 nodes over 131072 rows of
+// 16 heads 198 us, 5.4 TB/s of the 6.5 of a copy), the softmax of a tile's rows for many (2 x 48 nodes, 32 heads on 8, over 65536
+// rows 153 us, 637 TFLOP/s: 128 rows x 64 exponentials, two CTAs to an SM, one tile in 1.2 us each).  Ragged batches:
+// 16 trees of 64 nodes, 16 heads, over up to 4160 rows 66.5 us, about 56 of products at 5.4 TB/s and 10 of joining.
+// Rejected: two threads a row (94 us there), unrolling the tile loop (78), fetching K and V into L2 a tile further
+// ahead (131072 rows 211 us against 182), rows repeated over the lanes of small units, other joins (4 or 8 warps a block).
+//
 // Every wait is bounded; on expiry the CTA records an error in *err, waits (bounded) for its copies and
 // MMAs in flight, frees its TMEM and returns.
 #include <cuda.h>
@@ -65,7 +73,7 @@ constexpr int kTaTwoTermRows = 128;
 constexpr int kTaDirectTiles = 48;  // (see ta_plan)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
 constexpr int kTaCluster = 8;     // CTAs per unit (direct); long caches of few units take 12 or 16 (see ta_plan)
-constexpr int kTaUnitCost = 4;  // a unit's beginning and end take about as long as four tiles
+constexpr int kTaUnitCost = 4;  // a unit's beginning and end in tiles (16 ragged trees: 1 70.9 us, 2 67.9, 4 67.2, 6 66.8, 10 68.4)
 
 // Two layouts of the same kernel: units of up to 64 rows need only 16 KB for Q and get a third V
 // stage; the MMA still reads 128 rows, so rows 64-127 of its A operand are whatever lies behind
