@@ -521,7 +521,12 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
         return (int)cudaErrorInvalidValue;
     RopeFreqs freqs;
     const double step = -log2((double)rope_base) / (kDim / 2);
-    for (int t = 0; t < kDim / 2; ++t) freqs.f[t] = exp2(step * t);
+    double coarse[8], fine[8];  // base^(-t/64), t = 8 i + j, from 16 powers
+    for (int i = 0; i < 8; ++i) {
+        coarse[i] = exp2(step * 8 * i);
+        fine[i] = exp2(step * i);
+    }
+    for (int t = 0; t < kDim / 2; ++t) freqs.f[t] = coarse[t >> 3] * fine[t & 7];
     return launch_pdl(tree_rope_k, dim3(N, B), kRopeThreads, S(stream), reinterpret_cast<const half*>(qkv),
                       reinterpret_cast<const half*>(bias), depth, len, tree_len, N, num_heads, num_kv_heads, freqs,
                       reinterpret_cast<half*>(Q), reinterpret_cast<half*>(TK), reinterpret_cast<half*>(TV));
