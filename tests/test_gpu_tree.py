@@ -145,6 +145,42 @@ def test_attn_of_one_to_four_rows(B, N, H, KV, lens, tree_len):
     a.check(rows=300)
 
 
+@pytest.mark.parametrize("B,N,H,KV,lens,tree_len", [
+    (1, 16, 8, 2, [4096], None), (1, 8, 16, 16, [3333], None), (2, 9, 8, 4, [5000, 70], [9, 2]), (1, 70, 8, 2, [3500], None),
+    (1, 16, 8, 1, [40001], None), (2, 33, 4, 1, [20000, 33], [33, 12]), (1, 1, 8, 1, [30000], None)])
+def test_attn_of_few_units_with_long_caches(B, N, H, KV, lens, tree_len):
+    """Clusters of 12 and 16 CTAs, and single units cut into many parts; sequences that end long before the others."""
+    a = Attn(B * 31 + N, B, N, H, KV, lens, tree_len=tree_len).device().call()
+    first = a.d["O"].clone()
+    a.call().check(rows=60)
+    assert torch().equal(a.d["O"], first)
+
+
+def test_attn_single_tokens_captured_and_on_two_streams():
+    """One row per head: a graph replayed while lengths change (down to none), beside calls on another stream."""
+    t = torch()
+    a, b = (Attn(70 + i, 3, 1, 8, 4, [500, 3, 200], max_len=500).device() for i in range(2))
+    s1, s2 = t.cuda.Stream(), t.cuda.Stream()
+    for x in (a, b):
+        x.call()
+    t.cuda.synchronize()
+    g = t.cuda.CUDAGraph()
+    with t.cuda.graph(g, stream=s1):
+        a.call(stream=t.cuda.current_stream().cuda_stream)
+    for lens in ([500, 3, 200], [0, 499, 1], [64, 128, 0]):
+        a.lens = b.lens = lens
+        for x in (a, b):
+            x.d["len"].copy_(t.tensor(lens, dtype=t.int32))
+            x.d["O"].fill_(7.0)
+        t.cuda.synchronize()
+        for _ in range(4):
+            with t.cuda.stream(s1):
+                g.replay()
+            b.call(stream=s2.cuda_stream)
+        a.check()
+        b.check()
+
+
 @pytest.mark.parametrize("length", [0, 30, 400])
 def test_attn_of_few_rows_nothing_leaks(length):
     """Two and four rows: Inf and NaN in cache rows past the length and in tree rows that a node does not see; rows
