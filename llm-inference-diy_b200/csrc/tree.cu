@@ -127,7 +127,8 @@ constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerMaxCluster = 16;
 constexpr int kVerCtasPerSm = 2;
-constexpr int kVerHeld = 2;  // blocks of a warp's share kept in registers between rounds
+constexpr int kVerHeld = 6;  // blocks of a warp's share kept in shared memory between rounds (two CTAs share an SM)
+constexpr int kVerHeldBytes = kVerWarps * kVerHeld * 2 * 512;
 
 LLMDIY_DEV double positive(double x) { return x > 0.0 ? x : 0.0; }  // NaN counts as 0
 
@@ -154,6 +155,14 @@ LLMDIY_DEV void ver_weights(const float4& p, const float4& q, double T, double* 
         w[2] = positive(w[2] - T * positive(q.z));
         w[3] = positive(w[3] - T * positive(q.w));
     }
+}
+
+// The same into this thread's place in shared memory, without waiting where it can.
+LLMDIY_DEV void ver_hold(float4* dst, const float* row, int v0, int V, bool vec) {
+    if (vec && v0 + 3 < V)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(row + v0) : "memory");
+    else
+        *dst = ver_load(row, v0, V, vec);
 }
 
 // Eight bytes into the shared memory of CTA `rank` of the cluster, counted by the mbarrier there.
@@ -187,6 +196,7 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
                   int* accepted, int* next) {
     namespace cg = cooperative_groups;
     __shared__ VerSmem s;
+    extern __shared__ __align__(16) uint8_t ver_rows[];  // [warp][block][target, draft][lane] float4
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -236,9 +246,10 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
     const float *prow = target, *qrow = draft;  // the current node's rows
     double T = 0.0;                             // weight of entry v: max(0, p - T q)
     int round = 0, dead0 = 0, ndead = 0;  // the current node's refused tokens: s.dead[dead0 .. dead0 + ndead)
-    // The first kVerHeld blocks of the warp's share stay in registers while the walk is at a node; rows
-    // too long for that read the others again in every round.
-    float4 hp[kVerHeld], hq[kVerHeld];
+    // The first kVerHeld blocks of the warp's share stay in shared memory while the walk is at a node (each lane reads what
+    // it has copied itself); rows too long for that read the others again in every round.
+    float4* held = reinterpret_cast<float4*>(ver_rows) + warp * kVerHeld * 64 + lane;
+    const int uh = min(u1, u0 + kVerHeld);
     int held_node = -1;
     int cur = 0, cand = -1, count = 0;
     double Sj = 1.0;
@@ -264,18 +275,21 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
     auto totals = [&]() -> const double* {
         if (held_node != cur) {
             held_node = cur;
-#pragma unroll
-            for (int i = 0; i < kVerHeld; ++i) fetch(u0 + i < u1 ? u0 + i : U, hp[i], hq[i]);  // block U: past V, zeros
+            for (int u = u0; u < uh; ++u) {
+                ver_hold(held + (u - u0) * 64, prow, u * 128 + lane * 4, V, vec);
+                if (draft && T != 0.0) ver_hold(held + (u - u0) * 64 + 32, qrow, u * 128 + lane * 4, V, vec);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
         double t = 0.0;
-#pragma unroll
-        for (int i = 0; i < kVerHeld; ++i) {
+#pragma unroll 2
+        for (int u = u0; u < uh; ++u) {
             double w[4];
-            weigh(u0 + i, hp[i], hq[i], w);
+            weigh(u, held[(u - u0) * 64], held[(u - u0) * 64 + 32], w);
             t += (w[0] + w[1]) + (w[2] + w[3]);
         }
 #pragma unroll 2
-        for (int u = u0 + kVerHeld; u < u1; ++u) {
+        for (int u = uh; u < u1; ++u) {
             float4 p, q;
             double w[4];
             fetch(u, p, q);
@@ -405,13 +419,12 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         done = base + block > goal;
         base += block;
     };
-#pragma unroll
-    for (int i = 0; i < kVerHeld; ++i) {
+    for (int u = u0; u < uh && !done; ++u) {
         double w[4];
-        weigh(u0 + i, hp[i], hq[i], w);
-        search(u0 + i, w);
+        weigh(u, held[(u - u0) * 64], held[(u - u0) * 64 + 32], w);
+        search(u, w);
     }
-    for (int u = u0 + kVerHeld; u < u1 && !done; ++u) {
+    for (int u = uh; u < u1 && !done; ++u) {
         float4 p, q;
         double w[4];
         fetch(u, p, q);
@@ -478,12 +491,14 @@ int sm_count() {
     }
     return n;
 }
-// Clusters of more than 8 CTAs have to be asked for, once per device.
-cudaError_t ver_allow_clusters() {
+// Clusters of more than 8 CTAs and more than 48 KB of shared memory have to be asked for, once per device.
+cudaError_t ver_allow() {
     static std::atomic<bool> done[64];
     const int dev = current_device();
     if (dev >= 0 && done[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(tree_verify_k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaFuncSetAttribute(tree_verify_k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(tree_verify_k, cudaFuncAttributeMaxDynamicSharedMemorySize, kVerHeldBytes);
     if (e == cudaSuccess && dev >= 0) done[dev] = true;
     return e;
 }
@@ -543,11 +558,12 @@ int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd
     // CTAs per sequence: as many as run at once (two per SM), 16 at most.  Measured at V = 151936 (first form): one
     // chain 12.5 us with 8, 9.6 us with 16; 24 trees of 32 nodes 61 us with 4, 45 with 6, 41 with 8, 49 with 16 (12 now: 36).
     const int C = std::max(1, std::min(kVerMaxCluster, kVerCtasPerSm * sm_count() / B));
-    cudaError_t e = ver_allow_clusters();
+    cudaError_t e = ver_allow();
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(B * C);
     lc.blockDim = dim3(kVerThreads);
+    lc.dynamicSmemBytes = kVerHeldBytes;
     lc.stream = S(stream);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
