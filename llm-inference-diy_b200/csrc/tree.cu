@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kRopeThreads)
 // (no gain), the weights as two fp32 terms in place of fp64 (37.5 against 36.3).
 constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;
-constexpr int kVerMaxCluster = 16;
+constexpr int kVerMaxCluster = 14;
 constexpr int kVerCtasPerSm = 2;
 constexpr int kVerHeld = 6;  // blocks of a warp's share kept in shared memory between rounds (two CTAs share an SM)
 constexpr int kVerHeldBytes = kVerWarps * kVerHeld * 2 * 512;
@@ -555,9 +555,11 @@ int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd
         !words_aligned(target, draft, token, parent, tree_len, uniform, path, accepted, next))
         return (int)cudaErrorInvalidValue;
     const int vec = aligned16(target) && ldt % 4 == 0 && (!draft || (aligned16(draft) && ldd % 4 == 0));
-    // CTAs per sequence: as many as run at once (two per SM), 16 at most.  Measured at V = 151936 (first form): one
-    // chain 12.5 us with 8, 9.6 us with 16; 24 trees of 32 nodes 61 us with 4, 45 with 6, 41 with 8, 49 with 16 (12 now: 36).
-    const int C = std::max(1, std::min(kVerMaxCluster, kVerCtasPerSm * sm_count() / B));
+    // CTAs per sequence: as many as run at once (two per SM), 14 at most, and 10 rather than 11 to 13, of which 21 clusters fit
+    // on 148 SMs.  Measured at V = 151936, trees of 16: 1 sequence 9.7 us with 14, 11.0 with 16, 13.1 with 8; 16 20.5, 24.5, 24.9;
+    // 24 29.5 with 10, 33.5 with 12, 35.2 with 8; 32 36.4 with 9, 34.7 with 10; at V = 64000 48 sequences 24.8 with 6, 28.9 with 8.
+    int C = kVerCtasPerSm * sm_count() / B;
+    C = C >= kVerMaxCluster ? kVerMaxCluster : C > 10 ? 10 : std::max(C, 1);
     cudaError_t e = ver_allow();
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t lc = {};
