@@ -120,9 +120,9 @@ __global__ void __launch_bounds__(kRopeThreads)
 // [k U / K, (k + 1) U / K)), so the warps' totals in order are a running sum over the row.
 //
 // What bounds it is the walk: a refusal needs the sum over two rows before the next child can be tried, about 2.5 us a
-// round, 1.3 of them the rows' loads and 1.2 the exchange.  V = 151936: a chain 8.8 us, 24 trees of 32 nodes 34 to 37.
-// Tried: the root's rows fetched into L2 while the tree is read (24 trees 38.9 us against 35.5), more blocks held or unrolled
-// (no gain), the weights as two fp32 terms in place of fp64 (37.5 against 36.3).
+// round at a new node, 1.3 of them the rows' loads, and 1.2 (the exchange) at the same one.  V = 151936: a chain 7.6 us, 24
+// trees of 32 nodes 33.  Tried: blocks held in registers (two fit; 8.8 and 36.5 us), the root's rows fetched into L2 while
+// the tree is read (24 trees 38.9 us against 35.5), the weights as two fp32 terms in place of fp64 (37.5 against 36.3).
 constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerMaxCluster = 14;
