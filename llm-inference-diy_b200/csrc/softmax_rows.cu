@@ -29,14 +29,17 @@ using namespace llmdiy;
 namespace {
 
 constexpr int kSmThreads = 512;
-constexpr int kSmPairs = 20;                                  // pairs of entries a thread holds
+constexpr int kSmPairs = 17;                                  // pairs of entries a thread holds
 constexpr int kSmSlice = kSmThreads * kSmPairs * 2 - 8;       // entries a CTA holds (pairs may start one entry early)
 constexpr int kSmWarps = kSmThreads / 32;
 constexpr int kSmRun = kSmPairs * 64;                         // a warp's run of entries
-constexpr int kSmStages = 2;
-// A stage: eight entries before the slice's first granule, the granules, and room for every thread's pairs
+// The stage: eight entries before the slice's first granule, the granules, and room for every thread's pairs
 constexpr int kSmStageBytes = (16 + (kSmThreads * kSmPairs * 2 + 16) * 2 + 127) / 128 * 128;
-constexpr int kSmMaxCluster = 8;
+// Results on their way out: a warp's run, at either 8-byte offset within 16 bytes
+constexpr int kSmOutBytes = kSmRun * 4 + 16;
+constexpr int kSmBytes = kSmStageBytes + kSmWarps * kSmOutBytes;
+constexpr int kSmMaxCluster = 9;
+constexpr int kSmTable = (kSmMaxCluster * kSmWarps + 31) / 32;  // pairs of a row that a lane reads
 constexpr int kSmCtasPerSm = 2;
 
 LLMDIY_DEV float sm_ex2(float x) {  // 2^x (2^-inf = 0)
@@ -65,6 +68,11 @@ LLMDIY_DEV uint64_t sm_mul2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+LLMDIY_DEV void sm_bulk_out(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\ncp.async.bulk.commit_group;" ::"l"(dst),
+                 "r"(smem_u32(src)), "r"(bytes)
+                 : "memory");
 }
 // Eight bytes into the shared memory of CTA `rank` of the cluster, counted by the mbarrier there.
 LLMDIY_DEV void sm_send(float2* dst, uint64_t* bar, uint32_t rank, float a, float b) {
@@ -106,9 +114,9 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     softmax_rows_k(const half* logits, int ldl, const float* temp, int R, int V, int slice,
                    float* probs, int ldp) {
     namespace cg = cooperative_groups;
-    extern __shared__ __align__(128) uint8_t stage[];  // [kSmStages][kSmStageBytes]
+    extern __shared__ __align__(128) uint8_t stage[];  // kSmStageBytes, then the warps' results
     __shared__ float2 part[2][kSmMaxCluster * kSmWarps];  // (m_w, s_w) of the cluster's warps: odd and even rows
-    __shared__ uint64_t full[kSmStages], got[2];
+    __shared__ uint64_t full, empty, got[2];
     cg::cluster_group cluster = cg::this_cluster();
     // whether some copy begins or ends inside a granule
     const bool edges = (reinterpret_cast<uintptr_t>(logits) & 15) || (ldl & 7) || (V & 7);
@@ -120,45 +128,42 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     const uint16_t* base = reinterpret_cast<const uint16_t*>(logits);
     const uintptr_t first = reinterpret_cast<uintptr_t>(base), last = first + 2 * ((uintptr_t)(R - 1) * ldl + V);
     const uint64_t pol = l2_policy_evict_first();
-    auto copy = [&](int r, int st) {  // (one thread)
+    auto copy = [&](int r) {  // (one thread)
         const SmWindow w = sm_window(base + (size_t)r * ldl + v0, held, first, last);
         const uint32_t bytes = (uint32_t)(w.to - w.from);
-        mbar_arrive_expect_tx(&full[st], bytes);
-        // (a stage begins with the granule that holds the slice's first entry)
+        mbar_arrive_expect_tx(&full, bytes);
+        // (the stage begins with the granule that holds the slice's first entry)
         const uintptr_t g0 = reinterpret_cast<uintptr_t>(base + (size_t)r * ldl + v0) & ~(uintptr_t)15;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // after the plain stores to this stage
         if (bytes)
-            bulk_g2s(stage + st * kSmStageBytes + 16 + (w.from - g0), reinterpret_cast<const void*>(w.from), bytes, &full[st],
-                     pol);
+            bulk_g2s(stage + 16 + (w.from - g0), reinterpret_cast<const void*>(w.from), bytes, &full, pol);
     };
     if (tid == 0) {
-        for (int i = 0; i < kSmStages; ++i) mbar_init(&full[i], 1);
+        mbar_init(&full, 1);
+        mbar_init(&empty, kSmWarps);
         for (int i = 0; i < 2; ++i) mbar_init(&got[i], 1);
         mbar_fence_init();
     }
     // what no copy writes is -inf for every row
-    for (int i = tid; i < kSmStages * kSmStageBytes / 4; i += kSmThreads) reinterpret_cast<uint32_t*>(stage)[i] = 0xFC00FC00u;
+    for (int i = tid; i < kSmStageBytes / 4; i += kSmThreads) reinterpret_cast<uint32_t*>(stage)[i] = 0xFC00FC00u;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
     pdl_wait();  // nothing in global memory has been touched before this
     pdl_launch_dependents();
-    if (tid == 0)
-        for (int i = 0; i < kSmStages; ++i)
-            if (r0 + (long long)i * step < R) copy(r0 + i * step, i);
+    if (tid == 0 && r0 < R) copy(r0);
     if (C > 1) cluster.sync();  // every CTA of the cluster runs: its shared memory may be written
     int it = 0;
     for (long long row = r0; row < R; row += step, ++it) {
         const size_t r = (size_t)row;
         const uint16_t* x = base + r * ldl + v0;
         float* y = probs + r * ldp + v0;
-        const int st = it % kSmStages;
         const float t = temp ? temp[r] : 1.f;
         const SmWindow win = sm_window(x, held, first, last);
-        uint16_t* sx = reinterpret_cast<uint16_t*>(stage + st * kSmStageBytes + 16) + win.lead;
+        uint16_t* sx = reinterpret_cast<uint16_t*>(stage + 16) + win.lead;
         // pairs begin where 8-byte stores of the output do
         const int odd = (int)(reinterpret_cast<uintptr_t>(y) >> 2) & 1;
         const int run0 = warp * kSmRun - odd;  // this warp's entries: [run0, run0 + kSmRun) of the slice
-        bool ok = mbar_wait(&full[st], (it / kSmStages) & 1);
+        bool ok = mbar_wait(&full, it & 1);
         // The copy's first and last granules hold up to seven entries of the rows beside this slice, and the
         // last row in this stage may have ended up to fourteen entries further on: -inf for those; and
         // where the whole buffer ends inside a granule, its entries come from global memory.  Each warp sees to its own run.
@@ -193,6 +198,8 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) m = fmaxf(m, h2f(__ushort_as_half(x[a])));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const bool more = row + step < R;
+        if (lane == 0) mbar_arrive(&empty);  // this warp has read the stage
         // k is bounded so that 0 * k is 0 and -inf * k is -inf at any t > 0; greedy (t <= 0 or NaN) takes the upper
         // bound, where the smallest difference of two fp16 values gives 2^-inf
         const float k = t > 0.f ? fminf(fmaxf(1.4426950408889634f / t, 1e-30f), 1e30f) : 1e30f;
@@ -216,6 +223,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         // Two tables take turns: a warp sends row i + 2's pair only after every warp's pair of row i + 1 has come,
         // which each sends after it has read row i's table.
         float2* tab = part[it & 1];
+        if (tid == 0 && more && mbar_wait(&empty, it & 1)) copy((int)row + step);
         if (C > 1) {
             if (tid == 0) mbar_arrive_expect_tx(&got[it & 1], C * kSmWarps * 8);
             if (lane < C) sm_send(&tab[rank * kSmWarps + warp], &got[it & 1], lane, m, s);
@@ -224,12 +232,10 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
             if (lane == 0) tab[warp] = make_float2(m, s);
             __syncthreads();
         }
-        // (every warp has sent its pair, so it has read the stage)
-        if (tid == 0 && row + (long long)kSmStages * step < R) copy((int)row + kSmStages * step, st);
-        float2 q[kSmMaxCluster * kSmWarps / 32];
+        float2 q[kSmTable];
         float M = -INFINITY, total = 0.f;
 #pragma unroll
-        for (int j = 0; j < kSmMaxCluster * kSmWarps / 32; ++j) {
+        for (int j = 0; j < kSmTable; ++j) {
             const int at = lane + 32 * j;
             q[j] = at < C * kSmWarps ? tab[at] : make_float2(-INFINITY, 0.f);
             M = fmaxf(M, q[j].x);
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
 #pragma unroll
-        for (int j = 0; j < kSmMaxCluster * kSmWarps / 32; ++j)  // (q.x = -inf: a sum of 0, or NaN)
+        for (int j = 0; j < kSmTable; ++j)  // (q.x = -inf: a sum of 0, or NaN)
             total += q[j].y * (q[j].x == -INFINITY ? 1.f : weight(q[j].x, M));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -245,6 +251,28 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const float top = M == -INFINITY ? 0.f : M;
         const float scale = inv * (m == -INFINITY ? 1.f : weight(m, top));
+        if (more && run0 < held) {
+            // The next row's entries are taken up while these leave as one bulk copy of each warp: entries c of its run
+            // (c = 0: entry run0 of the slice) from [lo, hi), of which [b0, b1) lies between 16-byte boundaries.
+            float* to = y + run0;
+            const int lo = run0 < 0, end = min(held - run0, kSmRun);
+            const int turn = (int)(reinterpret_cast<uintptr_t>(to) >> 2) & 3;  // 0 or 2
+            const int b0 = turn ? 2 : 4 * lo, b1 = ((end + turn) & ~3) - turn;
+            float* mo = reinterpret_cast<float*>(stage + kSmStageBytes + warp * kSmOutBytes) + turn;
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last row's have left
+            __syncwarp();
+            const uint64_t scale2 = sm_f2(scale, scale);
+#pragma unroll
+            for (int i = 0; i < kSmPairs; ++i)
+                *reinterpret_cast<float2*>(mo + 2 * lane + 64 * i) = sm_split(sm_mul2(ex[i], scale2));
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && b1 > b0) sm_bulk_out(to + b0, mo + b0, (b1 - b0) * 4);
+            const int c = lane < 4 ? lo + lane : max(b1, min(b0, end)) + lane - 4;  // up to three before and behind it
+            if (lane < 8 && c < (lane < 4 ? min(b0, end) : end)) to[c] = mo[c];
+            for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
+            continue;
+        }
         float* out = y + run0 + 2 * lane;
         const int room = held - run0 - 2 * lane;  // entries from this thread's first on
         const int whole = (held - run0) / 64;     // pairs' runs that lie inside the slice as a whole
@@ -263,21 +291,22 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         }
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // Clusters of C CTAs that run at once on the current device.
 int sm_clusters(int C) {
-    static std::atomic<int> known[64][4];
+    static std::atomic<int> known[64][kSmMaxCluster + 1];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
-    const int slot = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
-    int n = known[dev][slot];
+    int n = known[dev][C];
     if (n) return n;
-    cudaFuncSetAttribute(softmax_rows_k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmStages * kSmStageBytes);
+    cudaFuncSetAttribute(softmax_rows_k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmBytes);
+    cudaFuncSetAttribute(softmax_rows_k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(C);
     lc.blockDim = dim3(kSmThreads);
-    lc.dynamicSmemBytes = kSmStages * kSmStageBytes;
+    lc.dynamicSmemBytes = kSmBytes;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = C;
@@ -285,7 +314,7 @@ int sm_clusters(int C) {
     lc.attrs = at;
     lc.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, softmax_rows_k, &lc) != cudaSuccess || n < 1) n = 1;
-    known[dev][slot] = n;
+    known[dev][C] = n;
     return n;
 }
 
@@ -298,13 +327,12 @@ extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float*
         return (int)cudaErrorInvalidValue;
     // CTAs per row: a power of two that holds it.  (Twice as many gained 0.2 us of 4.9 at 32000 entries up to 16 rows and lost
     // from 32 on, 5.7 against 5.0; at 8192 entries they cost 0.9 of 3.6.)
-    int C = 1;
-    while (C < kSmMaxCluster && (V + C - 1) / C > kSmSlice) C *= 2;
+    const int C = std::min(kSmMaxCluster, (V + kSmSlice - 1) / kSmSlice);
     const int slice = (((V + C - 1) / C) + 7) / 8 * 8;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(std::min(R, sm_clusters(C)) * C);
     lc.blockDim = dim3(kSmThreads);
-    lc.dynamicSmemBytes = kSmStages * kSmStageBytes;
+    lc.dynamicSmemBytes = kSmBytes;
     lc.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
