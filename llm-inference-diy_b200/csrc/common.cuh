@@ -189,6 +189,13 @@ LLMDIY_DEV float2 ld_l2_f2(const void* p) {
     return r;
 }
 
+// Largest value of a warp's lanes (NaN only where all are).
+LLMDIY_DEV float redux_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Host: every pointer (NULL too) lies on a 4-byte boundary.
 template <class... P>
 inline bool words_aligned(const P*... p) {

@@ -2,20 +2,21 @@
 // (include/llmdiy_tree.h).  No counterpart in the reference, whose engine takes the argmax only.
 //
 // One pass over memory, by persistent clusters of C CTAs: cluster c takes rows c, c + clusters, ..., slice k of
-// a row in CTA k, each warp a run of it.  Bulk copies bring the next two rows' slices into shared memory while a row
-// is worked on; its entries go to registers.  Each warp finds its run's maximum m_w and its sum s_w of exponentials
+// a row in CTA k, each warp a run of it.  A bulk copy brings the next row's slice into shared memory while a row, whose
+// entries are in registers, is worked on, and its results leave the same way.  Each warp finds its run's maximum m_w and its sum s_w of exponentials
 // relative to it (kept in registers as fp32) and sends the pair to every CTA of the cluster by asynchronous stores
 // that complete on the receiver's mbarrier; with all the pairs it forms the row's maximum M and sum
 // S = sum_w s_w 2^{(m_w - M) k}, k = log2(e) / t, and writes its run times 2^{(m_w - M) k} / S.  With C > 1 no barrier stands in the
 // loop.  x - m is exact in fp32 for fp16 x (but for far smaller x, whose share is 0), so
 // the exponent carries two roundings (k and the product).
 //
-// Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 139.6 us, 5.0 TB/s of the 6.5 of
-// a copy.  A row is in work for about 6 us (shared-memory loads, 16 warps' exponentials, the exchange, and 76 KB of
-// output at up to 32 bytes a cycle and SM), with 33 clusters of 8 resident.  Rejected: the whole CTA's maximum and sum
-// by barriers (141.7 us), results through shared memory and bulk stores (140.8, and 6.0 us against 5.5 for 5 rows),
-// clusters of 9 to 16 (158 to 311: a row takes as long, and fewer are in work), fp16 entries held and
-// their exponentials taken twice (188).
+// Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 127.9 us, 5.5 TB/s of the 6.5 of
+// a copy.  A row is in work for about 5 us (shared-memory loads, 16 warps' exponentials, the exchange of the cluster's
+// pairs), with 30 clusters of 9 resident.  Rejected: the whole CTA's maximum and sum by barriers and plain stores (clusters
+// of 8, 141.7 us; an SM writes 32 bytes a cycle, and the warps wait for that), plain stores without barriers (139.7), one or
+// two of a thread's pairs in plain stores for clusters of 8 (137 to 142), clusters of 10 (138.6), rows fetched into L2 two
+// ahead (139.0), fp16 entries held and their exponentials taken twice (188).  The last row's results are stored
+// plainly (5 rows in all took 5.5 us so and 6.0 by bulk copies when first tried; now 5.3).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -196,8 +197,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         for (int i = 0; i < kSmPairs; ++i) h = __hmax2(h, *reinterpret_cast<const half2*>(&w[i]));  // (NaN reaches the sum)
         float m = fmaxf(__low2float(h), __high2float(h));
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) m = fmaxf(m, h2f(__ushort_as_half(x[a])));
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = redux_max(m);
         const bool more = row + step < R;
         if (lane == 0) mbar_arrive(&empty);  // this warp has read the stage
         // k is bounded so that 0 * k is 0 and -inf * k is -inf at any t > 0; greedy (t <= 0 or NaN) takes the upper
@@ -240,8 +240,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
             q[j] = at < C * kSmWarps ? tab[at] : make_float2(-INFINITY, 0.f);
             M = fmaxf(M, q[j].x);
         }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        M = redux_max(M);
 #pragma unroll
         for (int j = 0; j < kSmTable; ++j)  // (q.x = -inf: a sum of 0, or NaN)
             total += q[j].y * (q[j].x == -INFINITY ? 1.f : weight(q[j].x, M));
@@ -325,7 +324,7 @@ extern "C" int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float*
     if (!logits || !probs || R <= 0 || V <= 0 || V > (1 << 30) || ldl < V || ldp < V ||
         (reinterpret_cast<uintptr_t>(logits) & 1) || !words_aligned(probs, temp))
         return (int)cudaErrorInvalidValue;
-    // CTAs per row: a power of two that holds it.  (Twice as many gained 0.2 us of 4.9 at 32000 entries up to 16 rows and lost
+    // CTAs per row: as many as hold it.  (Twice as many gained 0.2 us of 4.9 at 32000 entries up to 16 rows and lost
     // from 32 on, 5.7 against 5.0; at 8192 entries they cost 0.9 of 3.6.)
     const int C = std::min(kSmMaxCluster, (V + kSmSlice - 1) / kSmSlice);
     const int slice = (((V + C - 1) / C) + 7) / 8 * 8;

@@ -790,9 +790,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             for (int r = live * rank / C + warp; r < r1; r += kTaThreads / 32) {
                 float2 w = make_float2(-INFINITY, 0.f);
                 if (lane < C) w = ta_peer_f2(ml + r * 8, lane);
-                float M = w.x;
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                const float M = redux_max(w.x);
                 const unsigned parts = __ballot_sync(0xffffffffu, w.x != -INFINITY || w.y != w.y);
                 // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
                 const float f = w.x == -INFINITY ? (w.y == w.y ? 0.f : 1.f) : exp2f(w.x - M);

@@ -37,9 +37,7 @@ LLMDIY_DEV void few_send2(float2* dst, uint64_t* bar, uint32_t rank, const float
 // Joins up to 32 parts of a row in order, part k's (m, l) in lane k (-inf, 0 past the last), o(k) its dims of this lane.
 template <class O>
 LLMDIY_DEV float2 few_join(const float2& w, int parts, O o, float4& acc) {
-    float M = w.x;
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    const float M = redux_max(w.x);
     const float f = ta_ex2(w.x - (M == -INFINITY ? 0.f : M));  // nothing seen: 0 (its l is 0, or NaN, which stays)
     float L = w.y * f;
 #pragma unroll
@@ -112,7 +110,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[r][e] = ta_fma2(pp, x[e], acc[r][e]);
     };
-    auto rescale = [&](int r, float top) {  // returns the reference point
+    auto rescale = [&](int r, float top) {  // returns the reference point, the warp's
         const float to = fmaxf(m[r], top), nm = to == -INFINITY ? 0.f : to, f = ta_ex2(m[r] - nm);
         const uint64_t ff = ta_f2(f, f);
         m[r] = to;
@@ -164,10 +162,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
                 }
             }
             const float x = mine ? s[r][0] * kTaScaleLog2 : -INFINITY;
-            float top = x;
-#pragma unroll
-            for (int d = 8; d >= kOwn; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float nm = rescale(r, top);
+            const float nm = rescale(r, redux_max(x));
             p[r] = ta_ex2(x - nm);
             l[r] += p[r];
         }
@@ -193,7 +188,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
             for (int d = 8; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
             x *= kTaScaleLog2;
-            const float nm = rescale(r, sees ? x : -INFINITY);
+            const float nm = rescale(r, redux_max(sees ? x : -INFINITY));
             if (sees) {
                 const float p = ta_ex2(x - nm);
                 if (own == 0) l[r] += p;  // (one key: in the first one's lanes)
@@ -204,7 +199,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     // ---------------- the warp's two halves, the CTA's warps, the cluster's CTAs
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        (void)rescale(r, __shfl_xor_sync(0xffffffffu, m[r], 16));
 #pragma unroll
         for (int d = 16; d >= kOwn; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
         float x[8];
