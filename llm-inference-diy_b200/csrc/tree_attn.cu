@@ -787,29 +787,42 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             const int kvh = c.unit;
             const int live = min(a.rows, (c.n - m0) * G), r1 = live * (rank + 1) / C;
             const uint32_t ml = smem_u32(s.q[0]), oo = smem_u32(s.k[0][0]);
-            for (int r = live * rank / C + warp; r < r1; r += kTaThreads / 32) {
-                float2 w = make_float2(-INFINITY, 0.f);
-                if (lane < C) w = ta_peer_f2(ml + r * 8, lane);
-                const float M = redux_max(w.x);
-                const unsigned parts = __ballot_sync(0xffffffffu, w.x != -INFINITY || w.y != w.y);
+            // two rows to a warp, half a warp each (C <= 16)
+            const int gl = lane & 15;
+            for (int r0 = live * rank / C + 2 * warp; r0 < r1; r0 += 2 * (kTaThreads / 32)) {
+                const int r = min(r0 + (lane >> 4), r1 - 1);  // (the last row twice where they are odd)
+                const float2 w = gl < C ? ta_peer_f2(ml + r * 8, gl) : make_float2(-INFINITY, 0.f);
+                float M = w.x;
+#pragma unroll
+                for (int o = 8; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                const unsigned parts = __ballot_sync(0xffffffffu, w.x != -INFINITY || w.y != w.y) >> (lane & 16);
                 // nothing seen by a part: weight 0 (its l is 0, or NaN, which stays)
                 const float f = w.x == -INFINITY ? (w.y == w.y ? 0.f : 1.f) : exp2f(w.x - M);
                 float L = w.y * f;
 #pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+                for (int o = 8; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+                float4 acc[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
                 for (int k = 0; k < C; ++k) {
-                    const float fk = __shfl_sync(0xffffffffu, f, k);
-                    if (!((parts >> k) & 1)) continue;  // (a part that saw nothing has no o)
-                    const float4 y = ta_peer_f4(oo + r * (kTaDim * 4) + ((lane ^ (r & 31)) * 16), k);
-                    acc.x = __fmaf_rn(fk, y.x, acc.x);
-                    acc.y = __fmaf_rn(fk, y.y, acc.y);
-                    acc.z = __fmaf_rn(fk, y.z, acc.z);
-                    acc.w = __fmaf_rn(fk, y.w, acc.w);
+                    const float fk = __shfl_sync(0xffffffffu, f, k, 16);
+                    if ((parts >> k) & 1) {  // (a part that saw nothing has no o)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float4 y = ta_peer_f4(oo + r * (kTaDim * 4) + (((gl + 16 * e) ^ (r & 31)) * 16), k);
+                            acc[e].x = __fmaf_rn(fk, y.x, acc[e].x);
+                            acc[e].y = __fmaf_rn(fk, y.y, acc[e].y);
+                            acc[e].z = __fmaf_rn(fk, y.z, acc[e].z);
+                            acc[e].w = __fmaf_rn(fk, y.w, acc[e].w);
+                        }
+                    }
                 }
                 const int node = m0 + r / G, h = kvh * G + r - (r / G) * G;
-                ta_store4(a.O + ((size_t)c.b * a.N + node) * a.ldo + h * kTaDim + lane * 4, acc, L == 0.f ? 0.f : 1.f / L);
+                half* dst = a.O + ((size_t)c.b * a.N + node) * a.ldo + h * kTaDim + gl * 4;
+                if (r0 + (lane >> 4) < r1)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) ta_store4(dst + 64 * e, acc[e], L == 0.f ? 0.f : 1.f / L);
             }
         }
         // The peers have read this CTA's part (relaxed: nothing written has to be seen).
@@ -953,7 +966,23 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     // of different lengths direct waits for the longest, so several of them with more than
     // kTaDirectTiles tiles a CTA go flat.  Measured (direct / flat): 16 units of 17 tiles 9.9 / 17.4, 16 of 2049 203 / 184,
     // 16 of 514 (128 rows) 78 / 68, 2 of 126 20 / 59, 1024 of up to 33 103 / 122, 256 of up to 66 67 / 67.
-    int c = (int)std::max<long long>(1, std::min<long long>({kTaCluster, slots / units, tiles}));
+    // CTAs per unit (direct): the tiles of one, the cluster's barriers and its join (rows by 14 a time) against one another, in
+    // us.  Clusters of more than two leave gaps: 7/8 of the slots are counted, and where 8 GPCs' SMs do not take all clusters one CTA to an
+    // SM, units of many rows slow each other.  Measured with 1 / 2 / 4 / 8 CTAs: 12 units of 2 tiles and 115 rows 7.7 / 10.5 / 9.1 / 9.2;
+    // 96 of 4 and 83 rows 11.1 / 11.9 / 17.5 / 27.3; 64 of 6 and 8 rows 10.3 / 9.9 / 8.8 / 15.9; 16 of 33 and 26 rows 29.9 / 19.3 /
+    // 12.8 / 10.8; 20 of 28 and 125 rows 28.2 / 21.1 / 15.1 / 15.4 (14.0 with 5).
+    int c = 1;
+    double best = 1e30;
+    for (int k = 1; k <= std::min<long long>(kTaCluster, tiles); ++k) {
+        if (units * k > slots || (k > 2 && units * k * 8 > slots * 7LL)) break;
+        const bool lone = units <= 8 * (slots / kTaCtasPerSm / 8 / k);
+        const double us = std::max(1.0, (double)tiles / k) * (lone || p.rows <= 32 ? 0.75 : 1.1) +
+                          (k > 1 ? 0.6 + 0.1 * k + 0.6 * ((p.rows + 14 * k - 1) / (14 * k)) : 0.0);
+        if (us < best) {
+            best = us;
+            c = k;
+        }
+    }
     // Clusters of 12 or 16 for many tiles, where the units' all run at once: such clusters leave gaps, 21 and 14 of them fit
     // on 148 SMs (16 x 16 CTAs do not, and took 17.6 us against 10.7), so three quarters of the slots are counted.
     // Measured (8 / 16 CTAs), 8 units of 34 tiles 11.7 / 13.4, 2 of 65 14.7 / 11.2, 8 of 129 18.7 / 14.9; (8 / 12), 16
