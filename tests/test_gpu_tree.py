@@ -156,6 +156,20 @@ def test_attn_of_few_units_with_long_caches(B, N, H, KV, lens, tree_len):
     assert torch().equal(a.d["O"], first)
 
 
+@pytest.mark.parametrize("B,N,H,KV,lens,tree_len", [
+    (4, 5, 32, 32, [280, 0, 64, 131], None), (4, 8, 16, 16, [300, 65, 128, 1], [8, 0, 5, 8]),
+    (3, 20, 16, 16, [500, 499, 20], None), (5, 9, 8, 8, [700, 0, 3, 640, 128], [9, 9, 1, 4, 0]),
+    (1, 101, 20, 4, [1616], None), (2, 60, 12, 12, [600, 90], [60, 33]), (3, 23, 20, 4, [35, 0, 64], None),
+    (1, 64, 32, 8, [200], None), (8, 83, 3, 3, [65, 0, 1, 64, 63, 30, 10, 5], None)])
+def test_attn_of_every_cluster_size(B, N, H, KV, lens, tree_len):
+    """Short caches on clusters of one to eight CTAs: odd numbers of joined rows, CTAs without a tile, sequences that are
+    shorter than a cluster; the same bits again."""
+    a = Attn(B * 13 + N, B, N, H, KV, lens, tree_len=tree_len, pad=8).device().call()
+    first = a.d["O"].clone()
+    a.call().check(rows=250)
+    assert torch().equal(a.d["O"], first)
+
+
 def test_attn_single_tokens_captured_and_on_two_streams():
     """One row per head: a graph replayed while lengths change (down to none), beside calls on another stream."""
     t = torch()
