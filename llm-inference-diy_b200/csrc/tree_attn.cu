@@ -25,8 +25,8 @@
 // next scores waiting (with P written over S and two S buffers, S(j+2) waited for PV(j) to complete,
 // and a tile took 1.2 us however few rows there were).  Warps 0-3 own the rows (thread = row = TMEM lane): mask, online
 // softmax in base 2, P as fp16; O is rescaled only when a row's maximum grows by more than 2^8 (P stays
-// within fp16, and O / l does not depend on the reference point).  fp16 P costs 2^-11 of each
-// probability, as the fp16 output does; l sums the unrounded fp32 values.
+// within fp16, and O / l does not depend on the reference point).  fp16 P costs half a step, 2^-11, of each
+// probability down to 2^-21 of the row's largest and 2^-32 of that below (kTaRaise); l sums the unrounded fp32 values.
 //
 // What a row does not see must not reach it even as NaN * 0: masked scores are replaced by -inf
 // (K may hold anything there), and V rows past the end, as well as tree rows with an Inf or NaN, are zeroed in
@@ -303,6 +303,11 @@ LLMDIY_DEV float ta_ex2v(float x) {  // as ta_ex2, issued where it stands
     return y;
 }
 constexpr float kTaScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
+// Probabilities are formed as 2^(x - m + kTaRaise), o and l alike, which divides out. A row's reference m stays within
+// 2^8 of its maximum, so they reach 2^15 at most, and of fp16's range below 1 as much as can be is left to the small
+// ones: beside a key that takes nearly all the weight but has a small value, the output is made of those. Relative to
+// the largest the rounding is 2^-32 at least where it was 2^-25 without (keys at 2^-24.6 of it were 52% off).
+constexpr float kTaRaise = 7.f;
 
 // add[e] += p v[dim0 + e] of the tree rows base + bit that `hit` names, for one query row (out of line: rare).
 __device__ __noinline__ void ta_add_bad(const TaArgs& a, uint64_t hit, int b, int node, int base, int kvh, int h,
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                         l *= f;
                     }
                     if (grow) m = top;
-                    const float nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every p is 2^-inf = 0
+                    const float nm = m == -INFINITY ? 0.f : kTaRaise - m;  // nothing seen yet: every p is 2^-inf = 0
                     const uint64_t scale2 = ta_f2(kTaScaleLog2, kTaScaleLog2), nm2 = ta_f2(nm, nm);
                     uint64_t ls[2] = {0, 0};
                     // P, once the product that read this buffer is complete
@@ -745,7 +750,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                         for (int e = 0; e < 32; ++e) add[e] = 0.f;
                         for (int tt = tt0; tt < t0 + cnt - tc; ++tt)
                             ta_add_bad(a, *reinterpret_cast<volatile uint64_t*>(s.bad[tree_units & 1][tt]) & mrow[tt], c.b, node,
-                                       tt * 64, kvh, kvh * G + g, q, m == -INFINITY ? 0.f : -m, add);
+                                       tt * 64, kvh, kvh * G + g, q, m == -INFINITY ? 0.f : kTaRaise - m, add);
                         for (int e = 0; e < 32; ++e) v[e] += add[e];
                     }
                     if (!live) continue;

@@ -1,0 +1,58 @@
+"""Precision of the tree attention's probabilities (llmdiy_tree_attn, include/llmdiy_tree.h) where a bound per
+probability shows: rows dominated by a few keys whose values are 0, so that the output is made of small probabilities
+alone, and values that cancel. Scores are exact (powers of two), so the bounds hold only what the kernels round."""
+import numpy as np
+import pytest
+
+import treemath as tm
+from gpu_util import torch
+from test_gpu_tree import Attn, D, _free_after_the_test  # noqa: F401  (the fixture ends every test here too)
+
+pytestmark = pytest.mark.gpu
+
+
+def _score(a, rows, exponent):
+    """Gives the cache rows `rows` of every slot the score -exponent * ln 2 (nearly), all others 0."""
+    a.Q[...] = 0
+    for i in range(a.N):
+        for h in range(a.H):
+            a.Q[:, i, h * D + (i + h) % 8] = 16.0  # (one dim of eight: another one for each node)
+    for x in (a.K, a.TK):
+        x[...] = 0
+    for g in range(a.KV):
+        a.K[:, rows, g * D:g * D + 8] = np.float16(-exponent * np.log(2.0) * np.sqrt(128.0) / 16.0)
+
+
+def _check(a, bits):
+    torch().cuda.synchronize()
+    got = a.d["O"].cpu().numpy().astype(np.float64)
+    for b in range(a.B):
+        for i in sorted({0, a.N // 2, a.N - 1}):
+            for h in sorted({0, a.H - 1}):
+                cols = slice(h * a.KV // a.H * D, (h * a.KV // a.H + 1) * D)
+                js, m = sorted(a.sees[b][i]), a.lens[b]
+                K = np.concatenate([a.K[b, :m, cols], a.TK[b, js][:, cols]])
+                V = np.concatenate([a.V[b, :m, cols], a.TV[b, js][:, cols]])
+                o, tol = tm.attention_row_close(a.Q[b, i, h * D:(h + 1) * D], K, V, bits)
+                err = np.abs(got[b, i, h * D:(h + 1) * D] - o)
+                assert np.all(err <= tol), (b, i, h, float((err / tol).max()), float((err / np.abs(o)).max()))
+
+
+# trees of one M tile and of two, one sequence and several, caches for clusters and for the flat order
+SHAPES = [(1, 26, 16, 16, 2047), (4, 8, 16, 16, 1000), (1, 100, 4, 2, 1500), (1, 64, 2, 2, 500), (1, 5, 2, 1, 300),
+          (2, 8, 4, 2, 70000), (2, 100, 4, 2, 70000), (1, 2, 1, 1, 1000)]
+
+
+@pytest.mark.parametrize("exponent", [14.3, 18.6, 22.4, 24.6, 26.1, 30.2])
+@pytest.mark.parametrize("B,N,H,KV,room", SHAPES)
+def test_attn_small_probabilities_beside_dominating_keys(B, N, H, KV, room, exponent):
+    """The first key of every 64 dominates and its value is 0: the output is what the small probabilities add up to."""
+    m = min(room, 2047)
+    a = Attn(N, B, N, H, KV, [m - 3 * b for b in range(B)], max_len=room)
+    _score(a, slice(0, None, 64), -exponent)
+    for x in (a.V, a.TV):
+        x[...] = (1000 + 3000 * np.abs(np.sin(np.arange(x.size)))).reshape(x.shape).astype(np.float16)
+    a.V[:, ::64] = 0
+    # (a node sees itself: a key of score 0 with a value like the others)
+    a.device().call()
+    _check(a, 11)

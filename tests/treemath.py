@@ -107,3 +107,25 @@ def verify(target, draft, token, parent, n, u):
     run = np.cumsum(left)
     hit = np.nonzero((run > float(u[0]) * run[-1]) & (left > 0))[0]
     return path, int(hit[0]) if len(hit) else int(np.nonzero(left > 0)[0][-1])
+
+
+def attention_row_close(q, K, V, bits):
+    """(softmax(q K^T / sqrt(d)) V, bound on the kernel's error) for a row whose scores are exact in fp32 (few powers of
+    two in q and K) and lie within 32 doublings of the largest.
+
+    The bound, relative to the largest probability: each is rounded to `bits` significant bits (half a step 2^-bits) or by
+    2^-32, whichever is more (fp16 below 2^-14 has steps of 2^-24, half of one is 2^-25, and the largest is taken as 2^7 or
+    more); its exponent, up to 39, is formed with two roundings of 2^-24 (39 * 2 * 2^-24 * ln 2 < 2^-17.6; 2^-22 the
+    exponential). Each product entering the fp32 sums may lose 2^-23 of the sum's largest value (n products and 64 more of
+    the joins), and the sum of the probabilities n / 64 + 64 roundings of 2^-24. The output is fp16 (half a step 2^-11
+    relative, 2^-25 absolute)."""
+    n = len(K)
+    s = K.astype(np.float64) @ q.astype(np.float64) / np.sqrt(len(q))
+    e = np.exp(s - s.max())
+    assert e.min() > 2.0 ** -32
+    l = e.sum()
+    v = V.astype(np.float64)
+    o, size = (e / l) @ v, (e / l) @ np.abs(v)
+    err_p = np.maximum(e * 2.0 ** -bits, 2.0 ** -32) + e * 2.0 ** -17.5
+    tol = (err_p / l) @ np.abs(v) + size * (n + 64) * 2.0 ** -23 + np.abs(o) * ((n / 64 + 64) * 2.0 ** -24 + 2.0 ** -11)
+    return o, tol + 2.0 ** -25
