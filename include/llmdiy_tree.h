@@ -58,7 +58,8 @@ int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth
  * Head h uses kv head h / (num_heads / num_kv_heads).  Node rows of Q and O are ldq and ldo elements
  * apart (>= num_heads*128).  max_len bounds every len[b] (larger values are clamped); it sets the grid and the
  * workspace, so a captured graph serves every length up to it.  fp32 scores, statistics and
- * accumulation; probabilities as fp16, in calls of up to 128 query rows (B * N * num_heads) as the sum of two fp16.
+ * accumulation; probabilities as the sum of two fp16, which rounds each by 2^-22 of itself or 2^-32 of its row's largest,
+ * whichever is more, whatever else is in the call.
  * A visible score of NaN or +inf makes its row NaN.  A row that sees nothing, or only scores of -inf, gives zeros; what
  * a node does not see (K and V rows at or past len[b], tree rows outside its mask) does not reach its
  * output even where it is Inf or NaN.

@@ -19,14 +19,19 @@
 //
 // CTA.  Warp 4 streams Q (once per unit) and the K and V tiles by TMA through rings that run on
 // across units; warps 5 and 6 issue the MMAs:
-//   S(j)  = Q K(j)^T          128 x 64,  K = 128 dims  -> TMEM
-//   O    += P(j) V(j)         128 x 128, K = 64 keys   -> TMEM (P from TMEM, two buffers)
-// S(j+1) follows as soon as the rows have S(j) in registers, so that neither the softmax nor PV(j) keeps the
-// next scores waiting (with P written over S and two S buffers, S(j+2) waited for PV(j) to complete,
-// and a tile took 1.2 us however few rows there were).  Warps 0-3 own the rows (thread = row = TMEM lane): mask, online
-// softmax in base 2, P as fp16; O is rescaled only when a row's maximum grows by more than 2^8 (P stays
-// within fp16, and O / l does not depend on the reference point).  fp16 P costs half a step, 2^-11, of each
-// probability down to 2^-21 of the row's largest and 2^-32 of that below (kTaRaise); l sums the unrounded fp32 values.
+//   S(j)  = Q K(j)^T          128 x 64,  K = 128 dims      -> TMEM, two buffers
+//   O    += P(j) V(j)         128 x 128, K = 2 x 64 keys   -> TMEM (P from TMEM, in the place of S(j))
+// S(j+1) is computed while the rows are at S(j), S(j+2) when the product that reads P(j) is complete.  Warps 0-3 own the
+// rows (thread = row = TMEM lane): mask, online softmax in base 2; O is rescaled only when a row's maximum grows by more
+// than 2^8 (P stays within fp16, and O / l does not depend on the reference point).
+//
+// P goes to the tensor cores as the sum of two fp16 terms, p = hi + lo, for rows of every call alike: half a step of one
+// term is 2^-11 of each probability, whose scatter in the output is as large as the output's own rounding (2.9e-4 of the
+// norm together on normal inputs, 2.1e-4 with two terms, as fp32 probabilities give), and shows as it is where values cancel.  Two terms leave
+// 2^-22 of each, or 2^-32 of the row's largest (kTaRaise); l sums the unrounded fp32 values.  They cost 1.0 us of 11.3
+// (26 nodes over 2047 rows), 9 of 72 (16 ragged trees) and 31 of 183 (2 x 48 nodes over 65536 rows, grouped), for the second
+// product and a conversion back.  With one S buffer, and P beside it, the rows wait for the last product before they can store P: 12.1,
+// 85 and 226 us for these.
 //
 // What a row does not see must not reach it even as NaN * 0: masked scores are replaced by -inf
 // (K may hold anything there), and V rows past the end, as well as tree rows with an Inf or NaN, are zeroed in
@@ -64,12 +69,7 @@ constexpr int kTaRows = 128;     // query rows of a unit at most (MMA M)
 constexpr int kTaThreads = 224;  // warps 0-3: rows; warp 4: TMA; warps 5 and 6: the MMAs of S and of O
 constexpr int kTaCtasPerSm = 2;
 constexpr int kTaTileBytes = kTaKeys * kTaDim * 2;  // one K or V tile
-constexpr uint32_t kTaCols = 256;                   // TMEM: S (64 columns) | P0 | P1, or P's two terms (32 each) | O (128)
-// Calls of up to this many query rows in all (sequences x nodes x heads) take P in two fp16 terms (p = hi + lo): the
-// rounding of a few rows' few large probabilities does not average out.  Of 16 rows over 1023 keys one term put
-// up to 3.3e-4 of the output's norm, two terms leave the output's own rounding, 2.1e-4; over more rows one term keeps to
-// 2.9e-4.  Two terms take 10.6 us there against 10.0, and 194 against 185 over 131072 keys.
-constexpr int kTaTwoTermRows = 128;
+constexpr uint32_t kTaCols = 256;                   // TMEM: two buffers of S, then P over it (64 columns each) | O (128)
 constexpr int kTaDirectTiles = 48;  // (see ta_plan)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
 constexpr int kTaCluster = 8;     // CTAs per unit (direct); long caches of few units take 12 or 16 (see ta_plan)
@@ -84,7 +84,7 @@ struct TaSmem {
     half k[KS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, K-major (8 KB each)
     half v[VS][2][kTaKeys * 64];  // per stage, dims 0-63 | 64-127, MN-major (8 KB each)
     uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
-    uint64_t s_full, s_free, p_full[2], o_done[2], drain[2];
+    uint64_t s_full[2], p_full[2], o_done[2], drain[2];
     // tree rows with a non-finite V, by tree tile and quarter (a warp's 16 rows); two units' worth
     alignas(8) uint16_t bad[2][4][4];
     uint32_t tmem_base;
@@ -292,6 +292,11 @@ LLMDIY_DEV uint64_t ta_add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+LLMDIY_DEV uint64_t ta_sub2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 LLMDIY_DEV float ta_max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -324,7 +329,7 @@ __device__ __noinline__ void ta_add_bad(const TaArgs& a, uint64_t hit, int b, in
     }
 }
 
-template <int QR, int KS, int VS, bool DIRECT, bool TWO>
+template <int QR, int KS, int VS, bool DIRECT>
 __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     tree_attn_k(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap ttk,
@@ -351,9 +356,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             mbar_init(&s.v_full[i], 1);
             mbar_init(&s.v_empty[i], 1);
         }
-        mbar_init(&s.s_full, 1);
-        mbar_init(&s.s_free, 4);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.s_full[i], 1);
             mbar_init(&s.p_full[i], 4);
             mbar_init(&s.o_done[i], 1);
         }
@@ -410,8 +414,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         __syncwarp();
         named_bar_arrive(1, kTaThreads);
     }
-    // P(j) at tP + 32 * (j & 1), or (TWO) at tP and its low terms at tP + 32
-    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tP = tmem + 64, tO = tmem + 128;
+    // S(j) at tmem + 64 * (j & 1); P(j) takes its place, the low terms 32 columns behind the high ones
+    const uint32_t tmem = warp != 4 ? s.tmem_base : 0, tO = tmem + 128;
 
     if (warp == 4 && work) {
         if (lane == 0) {
@@ -488,17 +492,17 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             const int cnt = seg(t0);
             for (int i = 0; i < cnt; ++i, ++j) {
                 if (i == 0 && !warp_wait(&s.q_full, unit_no++ & 1)) { ok = false; break; }
-                // S(j) takes the place of S(j-1) as soon as the rows have that in registers
-                if (j && !warp_wait(&s.s_free, (j - 1) & 1)) { ok = false; break; }
+                // S(j) takes the place of P(j-2) when the product that reads it is complete
+                if (j >= 2 && !warp_wait(&s.o_done[j & 1], ((j - 2) >> 1) & 1)) { ok = false; break; }
                 if (!warp_wait(&s.k_full[st], ph)) { ok = false; break; }
                 tc_fence_after();
                 const uint64_t kj = kd + st * (kTaTileBytes / 16);
                 if (lead) {
 #pragma unroll
                     for (int kk = 0; kk < kTaDim / 16; ++kk)
-                        umma_f16(tmem, qd + ((kk >> 2) * (QR * 128) + 32 * (kk & 3)) / 16,
+                        umma_f16(tmem + 64 * (j & 1), qd + ((kk >> 2) * (QR * 128) + 32 * (kk & 3)) / 16,
                                  kj + ((kk >> 2) * 8192 + 32 * (kk & 3)) / 16, idS, kk != 0 ? 1u : 0u);
-                    umma_commit(&s.s_full);
+                    umma_commit(&s.s_full[j & 1]);
                     umma_commit(&s.k_empty[st]);
                     if (i + 1 == cnt) umma_commit(&s.q_empty);
                 }
@@ -531,17 +535,11 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                 if (!warp_wait(&s.v_full[st], ph)) { ok = false; break; }
                 if (!warp_wait(&s.p_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t pa = TWO ? tP : tP + 32u * (j & 1);
                 const uint64_t vj = vd + st * (kTaTileBytes / 16);
                 if (lead) {
 #pragma unroll
-                    for (int kk = 0; kk < kTaKeys / 16; ++kk)
-                        umma_f16_tmem_a(tO, pa + 8 * kk, vj + 2048 * kk / 16, idO, i == 0 && kk == 0 ? 0u : 1u);
-                    if (TWO) {
-#pragma unroll
-                        for (int kk = 0; kk < kTaKeys / 16; ++kk)
-                            umma_f16_tmem_a(tO, pa + 32 + 8 * kk, vj + 2048 * kk / 16, idO, 1u);
-                    }
+                    for (int kk = 0; kk < kTaKeys / 8; ++kk)  // both terms against the same V
+                        umma_f16_tmem_a(tO, tmem + 64 * (j & 1) + 8 * kk, vj + 2048 * (kk & 3) / 16, idO, i == 0 && kk == 0 ? 0u : 1u);
                     umma_commit(&s.v_empty[st]);
                     umma_commit(&s.o_done[j & 1]);  // last: the rows end the CTA when they have seen it
                 }
@@ -617,16 +615,15 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     if (tree && lane == 0) s.bad[tree_units & 1][tt][warp] = (uint16_t)bad16;
                     fence_async_smem();
                 }
-                if (!warp_wait(&s.s_full, j & 1)) { ok = false; break; }
+                if (!warp_wait(&s.s_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
                 if (warp_live) {
                     tc_fence_after();
+                    const uint32_t pt = tmem + 64 * (j & 1) + lane_off;  // S(j), then P(j)
                     float x[kTaKeys];
 #pragma unroll
                     for (int q = 0; q < kTaKeys; q += 16)
-                        tmem_ld16(tmem + lane_off + q, reinterpret_cast<uint32_t*>(x + q));
+                        tmem_ld16(pt + q, reinterpret_cast<uint32_t*>(x + q));
                     tmem_ld_wait();
-                    tc_fence_before();
-                    if (lane == 0) mbar_arrive(&s.s_free);
                     if (__builtin_expect(t >= plain, 0)) {
                         const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
 #pragma unroll
@@ -662,10 +659,6 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     const float nm = m == -INFINITY ? 0.f : kTaRaise - m;  // nothing seen yet: every p is 2^-inf = 0
                     const uint64_t scale2 = ta_f2(kTaScaleLog2, kTaScaleLog2), nm2 = ta_f2(nm, nm);
                     uint64_t ls[2] = {0, 0};
-                    // P, once the product that read this buffer is complete
-                    constexpr uint32_t kBack = TWO ? 1 : 2;
-                    if (j >= kBack && !warp_wait(&s.o_done[(j - kBack) & 1], ((j - kBack) >> 1) & 1)) { ok = false; break; }
-                    const uint32_t pt = (TWO ? tP : tP + 32u * (j & 1)) + lane_off;
                     // Sixteen keys at a time, the exponentials of one group ahead of the sums and the rounding of the
                     // last (in this order: a sum right behind its exponentials waits for them)
                     float e[2][16];
@@ -686,20 +679,14 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                         for (int q = 0; q < 16; q += 2) {
                             ls[(q >> 1) & 1] = ta_add2(ls[(q >> 1) & 1], ta_f2(from[q], from[q + 1]));
                             const uint32_t hi = ta_pack(from[q], from[q + 1]);
-                            if (TWO) {  // eight words of each term
-                                const float2 f = __half22float2(*reinterpret_cast<const half2*>(&hi));
-                                pk[q / 2] = hi;
-                                pk[8 + q / 2] = ta_pack(from[q] - f.x, from[q + 1] - f.y);
-                            } else {
-                                pk[((q0 & 16) + q) / 2] = hi;
-                            }
+                            const float2 h = __half22float2(*reinterpret_cast<const half2*>(&hi));
+                            float l0, l1;
+                            ta_split(ta_sub2(ta_f2(from[q], from[q + 1]), ta_f2(h.x, h.y)), l0, l1);
+                            pk[q / 2] = hi;
+                            pk[8 + q / 2] = ta_pack(l0, l1);
                         }
-                        if (TWO) {
-                            tmem_st8(pt + q0 / 2, pk);
-                            tmem_st8(pt + 32 + q0 / 2, pk + 8);
-                        } else if (q0 & 16) {
-                            tmem_st16(pt + (q0 - 16) / 2, pk);
-                        }
+                        tmem_st8(pt + q0 / 2, pk);
+                        tmem_st8(pt + 32 + q0 / 2, pk + 8);
                     };
                     exps(0);
                     exps(16);
@@ -714,8 +701,6 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     l += l0 + l1;
                     tmem_st_wait();
                     tc_fence_before();
-                } else if (lane == 0) {
-                    mbar_arrive(&s.s_free);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.p_full[j & 1]);
@@ -1029,9 +1014,9 @@ bool make_query_map(CUtensorMap* m, const void* base, int nodes, int H, int ldq,
 constexpr size_t kTaCtl = 8;  // floats before the partials, which begin on 32 bytes: word 0 is the error word
 size_t ta_work_bytes(const TaPlan& p) { return (kTaCtl + p.floats) * sizeof(float); }
 
-template <int QR, int KS, int VS, bool DIRECT, bool TWO>
+template <int QR, int KS, int VS, bool DIRECT>
 int ta_launch(const CUtensorMap* m, const TaArgs& a, int* err, dim3 grid, int cluster, cudaStream_t st) {
-    auto kern = tree_attn_k<QR, KS, VS, DIRECT, TWO>;
+    auto kern = tree_attn_k<QR, KS, VS, DIRECT>;
     constexpr int bytes = (int)sizeof(TaSmem<QR, KS, VS>);
     static_assert(bytes <= 115712, "two CTAs share an SM");
     static_assert((KS + VS) * kTaTileBytes >= QR * kTaDim * 4, "a part's rows fit over K and V");
@@ -1125,15 +1110,12 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
     const dim3 grid = direct ? dim3(p.cluster, num_kv_heads * p.mt, B) : dim3(p.W * p.mt);
     const int cluster = std::max(1, p.cluster);
     int rc;
-    if (p.rows <= 64 && (long long)B * N * num_heads <= kTaTwoTermRows)
-        rc = direct ? ta_launch<64, 3, 3, true, true>(m, a, err, grid, cluster, st)
-                      : ta_launch<64, 3, 3, false, true>(m, a, err, grid, cluster, st);
-    else if (p.rows <= 64)
-        rc = direct ? ta_launch<64, 3, 3, true, false>(m, a, err, grid, cluster, st)
-                      : ta_launch<64, 3, 3, false, false>(m, a, err, grid, cluster, st);
+    if (p.rows <= 64)
+        rc = direct ? ta_launch<64, 3, 3, true>(m, a, err, grid, cluster, st)
+                    : ta_launch<64, 3, 3, false>(m, a, err, grid, cluster, st);
     else
-        rc = direct ? ta_launch<128, 3, 2, true, false>(m, a, err, grid, cluster, st)
-                      : ta_launch<128, 3, 2, false, false>(m, a, err, grid, cluster, st);
+        rc = direct ? ta_launch<128, 3, 2, true>(m, a, err, grid, cluster, st)
+                    : ta_launch<128, 3, 2, false>(m, a, err, grid, cluster, st);
     if (rc || direct || p.W < 2) return rc;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((p.W - 1) * p.mt);

@@ -55,4 +55,22 @@ def test_attn_small_probabilities_beside_dominating_keys(B, N, H, KV, room, expo
     a.V[:, ::64] = 0
     # (a node sees itself: a key of score 0 with a value like the others)
     a.device().call()
-    _check(a, 11)
+    _check(a, 22)
+
+
+@pytest.mark.parametrize("drop", [0.46875, 0.9140625, 1.45703125])
+@pytest.mark.parametrize("B,N,H,KV,room", SHAPES + [(1, 8, 16, 16, 64), (2, 8, 16, 16, 64), (1, 1, 128, 1, 200),
+                                                    (1, 100, 1, 1, 200), (3, 100, 4, 2, 70000)])
+def test_attn_values_that_cancel(B, N, H, KV, room, drop):
+    """Half of 64 keys has probability 1 (relative), half one that fp16 rounds by 1.7 to 1.9 quarters of its step
+    2^-10, with values that cancel: what is left of the output is that rounding, whatever else is in the call."""
+    a = Attn(N, B, N, H, KV, [64] * B, max_len=room, sees=[[set()] * N for _ in range(B)])
+    _score(a, slice(1, None, 2), 0.0)
+    p = np.exp(-16.0 * drop / np.sqrt(128.0))
+    for g in range(KV):
+        a.K[:, 1::2, g * D:g * D + 8] = np.float16(-drop)
+    v = 1 + np.abs(np.sin(np.arange(a.V[:, ::2].size))).reshape(a.V[:, ::2].shape)
+    a.V[:, ::2] = v.astype(np.float16)
+    a.V[:, 1::2] = (-a.V[:, ::2][:, : a.V[:, 1::2].shape[1]].astype(np.float64) / p).astype(np.float16)
+    a.device().call()
+    _check(a, 22)
