@@ -73,6 +73,10 @@ int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16
                      int num_slots, const int* slot, const int* len, int max_len, const uint16_t* TK,
                      const uint16_t* TV, const uint64_t* mask, const int* tree_len, int B, int N, int num_heads,
                      int num_kv_heads, uint16_t* O, int ldo, float* work, size_t work_bytes, void* stream);
+/* Which way a call of these sizes runs on the current device: 0 all units' keys dealt in equal ranges over the SMs, cut
+ * units joined by a second launch; 1 a cluster of CTAs per unit; 2 the same on the CUDA cores (one to four query rows per
+ * kv head and sequence); -1 for sizes that are refused. */
+int llmdiy_tree_attn_path(int B, int N, int num_heads, int num_kv_heads, int max_len);
 /* After the stream is synchronised: 0, or -5 when a pipeline wait of a call with this workspace expired
  * since the last status query (that output is then not valid); the query clears the word. */
 int llmdiy_tree_attn_status(const float* work);

@@ -1055,6 +1055,11 @@ size_t llmdiy_tree_attn_work_bytes(int B, int N, int num_heads, int num_kv_heads
     return p.ok ? ta_work_bytes(p) : 0;
 }
 
+int llmdiy_tree_attn_path(int B, int N, int num_heads, int num_kv_heads, int max_len) {
+    const TaPlan p = ta_plan(B, N, num_heads, num_kv_heads, max_len);
+    return !p.ok ? -1 : p.few ? 2 : p.cluster ? 1 : 0;
+}
+
 int llmdiy_tree_attn(const uint16_t* Q, int ldq, const uint16_t* K, const uint16_t* V, int stride, int slot_rows,
                      int num_slots, const int* slot, const int* len, int max_len, const uint16_t* TK,
                      const uint16_t* TV, const uint64_t* mask, const int* tree_len, int B, int N, int num_heads,

@@ -100,6 +100,7 @@ def lib() -> ctypes.CDLL:
         "llmdiy_tree_rope": [P, P, P, P, P, I, I, I, I, F, P, P, P, P],
         "llmdiy_tree_attn": [P, I, P, P, I, I, I, P, P, I, P, P, P, P, I, I, I, I, P, I, P, SZ, P],
         "llmdiy_tree_attn_status": [P],
+        "llmdiy_tree_attn_path": [I, I, I, I, I],
         "llmdiy_softmax_rows": [P, I, P, I, I, P, I, P],
         "llmdiy_tree_verify": [P, I, P, I, P, P, P, P, I, I, I, P, P, P, P],
         "llmdiy_tree_commit": [P, P, SZ, P, P, SZ, I, I, I, P, P, P, P, I, I, I, I, P, P],
@@ -347,6 +348,11 @@ def tree_rope(qkv, bias, depth, lens, tree_len, B, N, num_heads, num_kv_heads, r
 
 def tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len):
     return int(lib().llmdiy_tree_attn_work_bytes(B, N, num_heads, num_kv_heads, max_len))
+
+
+def tree_attn_path(B, N, num_heads, num_kv_heads, max_len) -> int:
+    """Which way tree_attn runs for these sizes: 0 equal ranges over all SMs, 1 a cluster per unit, 2 CUDA cores, -1 invalid."""
+    return int(lib().llmdiy_tree_attn_path(B, N, num_heads, num_kv_heads, max_len))
 
 
 def tree_attn(Q, ldq, K, V, stride, slot_rows, num_slots, slot, lens, max_len, TK, TV, mask, tree_len, B, N,

@@ -4,6 +4,7 @@ alone, and values that cancel. Scores are exact (powers of two), so the bounds h
 import numpy as np
 import pytest
 
+import llmdiy_b200 as L
 import treemath as tm
 from gpu_util import torch
 from test_gpu_tree import Attn, D, _free_after_the_test  # noqa: F401  (the fixture ends every test here too)
@@ -40,7 +41,7 @@ def _check(a, bits):
 
 # trees of one M tile and of two, one sequence and several, caches for clusters and for the flat order
 SHAPES = [(1, 26, 16, 16, 2047), (4, 8, 16, 16, 1000), (1, 100, 4, 2, 1500), (1, 64, 2, 2, 500), (1, 5, 2, 1, 300),
-          (2, 8, 4, 2, 70000), (2, 100, 4, 2, 70000), (1, 2, 1, 1, 1000)]
+          (2, 8, 8, 1, 33000), (3, 100, 8, 1, 13000), (1, 2, 1, 1, 1000)]
 
 
 @pytest.mark.parametrize("exponent", [14.3, 18.6, 22.4, 24.6, 26.1, 30.2])
@@ -54,13 +55,14 @@ def test_attn_small_probabilities_beside_dominating_keys(B, N, H, KV, room, expo
         x[...] = (1000 + 3000 * np.abs(np.sin(np.arange(x.size)))).reshape(x.shape).astype(np.float16)
     a.V[:, ::64] = 0
     # (a node sees itself: a key of score 0 with a value like the others)
+    assert L.tree_attn_path(B, N, H, KV, room) == (2 if N * H // KV <= 4 else 0 if room > 3000 else 1)
     a.device().call()
     _check(a, 22)
 
 
 @pytest.mark.parametrize("drop", [0.46875, 0.9140625, 1.45703125])
 @pytest.mark.parametrize("B,N,H,KV,room", SHAPES + [(1, 8, 16, 16, 64), (2, 8, 16, 16, 64), (1, 1, 128, 1, 200),
-                                                    (1, 100, 1, 1, 200), (3, 100, 4, 2, 70000)])
+                                                    (1, 100, 1, 1, 200), (2, 70, 1, 1, 33000)])
 def test_attn_values_that_cancel(B, N, H, KV, room, drop):
     """Half of 64 keys has probability 1 (relative), half one that fp16 rounds by 1.7 to 1.9 quarters of its step
     2^-10, with values that cancel: what is left of the output is that rounding, whatever else is in the call."""
