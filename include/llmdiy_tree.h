@@ -103,7 +103,8 @@ int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float* temp, int 
  * Writes path[b][0..accepted-1] = the accepted nodes in order (then -1 up to N), accepted[b] and next[b].
  * A node whose token is outside 0..V-1 or whose parent is not in 0..i-1 is never tried; entries of the distributions that
  * are not > 0 count as 0; next is -1 when p has none above 0.  A sequence without nodes (tree_len 0)
- * gets accepted = -1, next = -1. */
+ * gets accepted = -1, next = -1; one for which a bounded wait expired accepted = -2, next = -1 (its path is not valid, and
+ * llmdiy_tree_commit moves nothing for it). */
 int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd, const int* token,
                        const int* parent, const int* tree_len, const float* uniform, int B, int N, int V, int* path,
                        int* accepted, int* next, void* stream);

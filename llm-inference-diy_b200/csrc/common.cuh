@@ -17,7 +17,13 @@ namespace llmdiy {
 // Upper bound on polls of any spin-wait (mbarrier or a global flag).  A wait
 // that runs out sets an error flag and the kernel returns instead of hanging.
 // With the nanosleep back-off below this is on the order of a few seconds.
-constexpr uint32_t kSpinLimit = 1u << 24;
+// (-DLLMDIY_SPIN_LIMIT=0 builds kernels whose waits all expire at once, to test what they do then.)
+#ifndef LLMDIY_SPIN_LIMIT
+#define LLMDIY_SPIN_LIMIT (1u << 24)
+#endif
+constexpr uint32_t kSpinLimit = LLMDIY_SPIN_LIMIT;
+// The bound of the waits for what is still in flight once another wait has expired.
+constexpr uint32_t kDrainLimit = 1u << 24;
 
 // Error codes a kernel may record in its error word.
 enum : int {
@@ -69,6 +75,21 @@ LLMDIY_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* ab
         if (i > 64) __nanosleep(64);
     }
     return false;
+}
+
+// After some wait has expired: copies, products or peers' stores that complete on `bar` have landed before the CTA
+// exits (bounded).
+LLMDIY_DEV void mbar_drain(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kDrainLimit && !mbar_try_wait(bar, parity); ++i)
+        if (i > 64) __nanosleep(64);
+}
+// The same for a cluster's asynchronous stores into this CTA: a warp (converged) whose wait has expired calls this before it
+// exits.  The barrier counts threads that have exited as arrived, so the other warps and CTAs need not take part: all
+// of them have issued their last stores when it opens, and those land within the pause.
+LLMDIY_DEV void cluster_drain() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int i = 0; i < 128; ++i) __nanosleep(1000);
 }
 
 // ---------------- bulk copies (TMA engine) ----------------

@@ -269,9 +269,10 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         q = draft && T != 0.0 ? ver_load(qrow, v0, V, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     // This warp's total goes into every CTA's table by asynchronous stores that complete on the receiver's mbarrier (a
-    // cluster barrier a round took as long as the row's pass itself); returns the table once it is complete, NULL if
-    // that does not happen (bounded).  Two tables take turns: a warp sends round r + 2's total only after every warp's
+    // cluster barrier a round took as long as the row's pass itself); returns the table once it is complete, or sets
+    // `lost` if that does not happen (bounded).  Two tables take turns: a warp sends round r + 2's total only after every warp's
     // of round r + 1 has come, which each sends after it has read round r's table.
+    bool lost = false;  // a wait of this warp has expired
     auto totals = [&]() -> const double* {
         if (held_node != cur) {
             held_node = cur;
@@ -303,13 +304,13 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         if (lane < C) ver_send(mine + k, bar, lane, t);
         const bool ok = mbar_wait(bar, (round >> 1) & 1);
         ++round;
-        return __all_sync(0xffffffffu, ok) ? mine : nullptr;
+        lost = !__all_sync(0xffffffffu, ok);
+        return mine;
     };
     // lane l's share of the table: entries [l K / 32, (l + 1) K / 32)
     const int j0 = K * lane / 32, j1 = K * (lane + 1) / 32;
     auto lane_sum = [&](const double* tab) {
         double t = 0.0;
-        if (!tab) return (double)NAN;
         for (int j = j0; j < j1; ++j) t += tab[j];
         return t;
     };
@@ -342,15 +343,24 @@ __global__ void __launch_bounds__(kVerThreads, kVerCtasPerSm)
         } else {
             T += Sj;
             if (s.sibling[cand] >= 0) Sj = warp_sum(lane_sum(totals()));
+            if (lost) break;
         }
         cand = s.sibling[cand];
     }
 
     // the last token: first entry whose running sum of weights exceeds u_0 * their sum
-    const double* tab;
+    const double* tab = nullptr;
     double t, inc, total;
     for (int attempt = 0;; ++attempt) {
-        tab = totals();
+        if (!lost) tab = totals();
+        if (lost) {  // this sequence has no result (the walk's steps are no longer the same everywhere)
+            cluster_drain();
+            if (lane == 0) {
+                accepted[b] = -2;
+                next[b] = -1;
+            }
+            return;
+        }
         t = lane_sum(tab);
         inc = t;
 #pragma unroll
