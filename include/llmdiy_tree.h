@@ -84,7 +84,8 @@ int llmdiy_tree_attn_status(const float* work);
 /* Probabilities of R rows of V fp16 logits (row pitches ldl and ldp elements, >= V):
  * probs = exp((x - max) / temp[r]) / sum in fp32, temp NULL = 1.  temp <= 0 (or NaN) gives the limit: equal shares
  * of the row's largest entries (greedy).  Entries of -inf get 0; a row with nothing above -inf gives zeros; one with a NaN or
- * +inf is NaN throughout. */
+ * +inf is NaN throughout.  A bounded wait that expires (nothing else reports it) makes NaN of its row, or of parts of it, and of those that
+ * were still to come. */
 int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float* temp, int R, int V, float* probs, int ldp,
                         void* stream);
 

@@ -86,7 +86,7 @@ LLMDIY_DEV void mbar_drain(uint64_t* bar, uint32_t parity) {
 // The same for a cluster's asynchronous stores into this CTA: a warp (converged) whose wait has expired calls this before it
 // exits.  The barrier counts threads that have exited as arrived, so the other warps and CTAs need not take part: all
 // of them have issued their last stores when it opens, and those land within the pause.
-LLMDIY_DEV void cluster_drain() {
+static __device__ __noinline__ void cluster_drain() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     for (int i = 0; i < 128; ++i) __nanosleep(1000);

@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     extern __shared__ __align__(128) uint8_t stage[];  // kSmStageBytes, then the warps' results
     __shared__ float2 part[2][kSmMaxCluster * kSmWarps];  // (m_w, s_w) of the cluster's warps: odd and even rows
     __shared__ uint64_t full, empty, got[2];
+    __shared__ int copied;  // copies issued (the thread that issues them writes and reads it)
     cg::cluster_group cluster = cg::this_cluster();
     // whether some copy begins or ends inside a granule
     const bool edges = (reinterpret_cast<uintptr_t>(logits) & 15) || (ldl & 7) || (V & 7);
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     auto copy = [&](int r) {  // (one thread)
         const SmWindow w = sm_window(base + (size_t)r * ldl + v0, held, first, last);
         const uint32_t bytes = (uint32_t)(w.to - w.from);
+        ++copied;
         mbar_arrive_expect_tx(&full, bytes);
         // (the stage begins with the granule that holds the slice's first entry)
         const uintptr_t g0 = reinterpret_cast<uintptr_t>(base + (size_t)r * ldl + v0) & ~(uintptr_t)15;
@@ -140,6 +142,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
             bulk_g2s(stage + 16 + (w.from - g0), reinterpret_cast<const void*>(w.from), bytes, &full, pol);
     };
     if (tid == 0) {
+        copied = 0;
         mbar_init(&full, 1);
         mbar_init(&empty, kSmWarps);
         for (int i = 0; i < 2; ++i) mbar_init(&got[i], 1);
@@ -154,7 +157,9 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     if (tid == 0 && r0 < R) copy(r0);
     if (C > 1) cluster.sync();  // every CTA of the cluster runs: its shared memory may be written
     int it = 0;
-    for (long long row = r0; row < R; row += step, ++it) {
+    bool lost = false;  // a wait of this warp has expired (of this CTA where it is a cluster)
+    long long row = r0;
+    for (; row < R && !lost; row += step, ++it) {
         const size_t r = (size_t)row;
         const uint16_t* x = base + r * ldl + v0;
         float* y = probs + r * ldp + v0;
@@ -223,14 +228,18 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         // Two tables take turns: a warp sends row i + 2's pair only after every warp's pair of row i + 1 has come,
         // which each sends after it has read row i's table.
         float2* tab = part[it & 1];
-        if (tid == 0 && more && mbar_wait(&empty, it & 1)) copy((int)row + step);
+        if (tid == 0 && more) {
+            if (mbar_wait(&empty, it & 1)) copy((int)row + step);
+            else ok = false;
+        }
         if (C > 1) {
             if (tid == 0) mbar_arrive_expect_tx(&got[it & 1], C * kSmWarps * 8);
             if (lane < C) sm_send(&tab[rank * kSmWarps + warp], &got[it & 1], lane, m, s);
-            ok = mbar_wait(&got[it & 1], (it >> 1) & 1);
+            ok = mbar_wait(&got[it & 1], (it >> 1) & 1) && ok;
+            lost = __any_sync(0xffffffffu, !ok);
         } else {  // (a barrier is quicker within one CTA: a row of 8192 entries 3.7 us against 4.4)
             if (lane == 0) tab[warp] = make_float2(m, s);
-            __syncthreads();
+            lost = __syncthreads_or(!ok);
         }
         float2 q[kSmTable];
         float M = -INFINITY, total = 0.f;
@@ -246,11 +255,11 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
             total += q[j].y * (q[j].x == -INFINITY ? 1.f : weight(q[j].x, M));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (!ok) total = NAN;
+        if (lost) total = NAN;
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const float top = M == -INFINITY ? 0.f : M;
         const float scale = inv * (m == -INFINITY ? 1.f : weight(m, top));
-        if (more && run0 < held) {
+        if (more && run0 < held && !lost) {
             // The next row's entries are taken up while these leave as one bulk copy of each warp: entries c of its run
             // (c = 0: entry run0 of the slice) from [lo, hi), of which [b0, b1) lies between 16-byte boundaries.
             float* to = y + run0;
@@ -291,6 +300,16 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
         for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = weight(h2f(__ushort_as_half(x[a])), top) * inv;
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lost) {  // this warp's part of the rows that are left is NaN too
+        for (; row < R; row += step) {
+            float* y = probs + (size_t)row * ldp + v0;
+            const int run0 = warp * kSmRun - ((int)(reinterpret_cast<uintptr_t>(y) >> 2) & 1);
+            for (int a = max(run0, 0) + lane; a < min(held, run0 + kSmRun); a += 32) y[a] = NAN;
+            for (int a = kSmSlice + tid; a < n; a += kSmThreads) y[a] = NAN;
+        }
+        if (tid == 0 && copied) mbar_drain(&full, (copied - 1) & 1);
+        if (C > 1) cluster_drain();
+    }
 }
 
 // Clusters of C CTAs that run at once on the current device.

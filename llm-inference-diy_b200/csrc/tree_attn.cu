@@ -273,7 +273,7 @@ __device__ __noinline__ bool ta_wait_slow(uint64_t* bar, uint32_t parity, const 
     return mbar_wait(bar, parity, fail);
 }
 LLMDIY_DEV bool ta_wait(uint64_t* bar, uint32_t parity, const volatile int* fail) {
-    return mbar_try_wait(bar, parity) || ta_wait_slow(bar, parity, fail);
+    return (kSpinLimit && mbar_try_wait(bar, parity)) || ta_wait_slow(bar, parity, fail);
 }
 // Two fp32 values at once
 LLMDIY_DEV uint64_t ta_f2(float a, float b) {
@@ -473,9 +473,9 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                 if (ok) c.next(a);
             }
             // the last copies land in this CTA's shared memory: they have before it exits, whatever happens
-            for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i) (void)mbar_wait(&s.k_full[i % KS], (i / KS) & 1);
-            for (uint32_t i = vn > VS ? vn - VS : 0; i < vn; ++i) (void)mbar_wait(&s.v_full[i % VS], (i / VS) & 1);
-            if (unit_no) (void)mbar_wait(&s.q_full, (unit_no - 1) & 1);
+            for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i) mbar_drain(&s.k_full[i % KS], (i / KS) & 1);
+            for (uint32_t i = vn > VS ? vn - VS : 0; i < vn; ++i) mbar_drain(&s.v_full[i % VS], (i / VS) & 1);
+            if (unit_no) mbar_drain(&s.q_full, (unit_no - 1) & 1);
             if (!ok) s.fail = 1;
         }
         __syncwarp();
@@ -515,11 +515,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             if (DIRECT) break;
             c.next(a);
         }
-        if (!ok) {
-            s.fail = 1;
-            if (lead) umma_commit(&s.drain[0]);  // every MMA issued so far completes before the CTA exits
-            (void)mbar_wait(&s.drain[0], 0);
-        }
+        if (!ok) s.fail = 1;
         __syncwarp();
     } else if (warp == 6 && work) {
         // ---------------- O (+)= P(j) V(j), then release V(j)'s stage
@@ -552,11 +548,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
             if (DIRECT) break;
             c.next(a);
         }
-        if (!ok) {
-            s.fail = 1;
-            if (lead) umma_commit(&s.drain[1]);
-            (void)mbar_wait(&s.drain[1], 0);
-        }
+        if (!ok) s.fail = 1;
         __syncwarp();
     } else if (warp < 4 && work) {
         // ---------------- rows
@@ -820,7 +812,16 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
     }
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && s.fail) atomicExch(err, 1);
+    if (__builtin_expect(*reinterpret_cast<volatile int*>(&s.fail), 0)) {
+        if (tid == 0) atomicExch(err, 1);
+        // whichever warp gave up: every MMA issued completes before the TMEM is freed and the CTA exits
+        if (work && (warp == 5 || warp == 6)) {
+            if (elect_one()) umma_commit(&s.drain[warp - 5]);
+            mbar_drain(&s.drain[warp - 5], 0);
+            __syncwarp();
+        }
+        __syncthreads();
+    }
     if (warp == 0) tmem_dealloc(tmem, kTaCols);
 }
 

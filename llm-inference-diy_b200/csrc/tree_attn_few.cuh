@@ -226,7 +226,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         if (lane == 0) few_send2(&pml[r][rank], &got[r], owner, ml);
         if (rank != owner) return;
         const bool ok = mbar_wait(&got[r], 0);
-        if (!ok && lane == 0) atomicExch(err, 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+            if (lane == 0) atomicExch(err, 1);
+            cluster_drain();
+        }
         ml = few_join(lane < C ? pml[r][lane] : none, C, [&](int k) { return po[r][k][lane]; }, o);
     }
     ta_store4(a.O + ((size_t)b * a.N + node) * a.ldo + (kvh * G + r - node * G) * kTaDim + lane * 4, o,
