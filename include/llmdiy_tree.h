@@ -18,7 +18,7 @@
  * Arrays over nodes are [B][N]; what belongs to nodes at or past tree_len[b] has no
  * effect and, in the outputs of tree_rope and tree_attn, is left as it was.
  *
- * The cache.  The batch's layout (llmdiy_batch.h): row r of kv head h of slot s is at
+ * The cache.  The caller's, laid out as a batch's (llmdiy_batch.h), whose own is not handed out: row r of kv head h of slot s is at
  * (s * slot_rows + r) * stride + h * 128 elements, in K and in V; sequence b uses slot[b] (NULL: slot
  * b) and has len[b] committed rows (positions 0 .. len[b]-1).  The tree's own K/V rows live in buffers
  * [B][N][num_kv_heads*128] until llmdiy_tree_commit.  A slot outside 0..num_slots-1 has no rows.
@@ -83,9 +83,9 @@ int llmdiy_tree_attn_status(const float* work);
 
 /* Probabilities of R rows of V fp16 logits (row pitches ldl and ldp elements, >= V):
  * probs = exp((x - max) / temp[r]) / sum in fp32, temp NULL = 1.  temp <= 0 (or NaN) gives the limit: equal shares
- * of the row's largest entries (greedy).  Entries of -inf get 0; a row with nothing above -inf gives zeros; one with a NaN or
- * +inf is NaN throughout.  A bounded wait that expires (nothing else reports it) makes NaN of its row, or of parts of it, and of those that
- * were still to come. */
+ * of the row's largest entries (greedy; llmdiy_argmax picks one of them by a rule of its own).  Entries of -inf get 0; a
+ * row with nothing above -inf gives zeros; one with a NaN or +inf is NaN throughout.  A bounded wait that expires (nothing
+ * else reports it) makes NaN of its row, or of parts of it, and of those that were still to come. */
 int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float* temp, int R, int V, float* probs, int ldp,
                         void* stream);
 
