@@ -45,8 +45,8 @@ int llmdiy_tree_layout(const int* parent, int n, int* depth, uint64_t* mask, int
 /* Bias and rotary position of the tree's rows (stands beside llmdiy_fused_qkv_rope_cache, whose pairing
  * (t, t + 64) it shares).  qkv is [B][N][(num_heads + 2 num_kv_heads) * 128] (queries, keys, values);
  * bias is one such row, or NULL.  Node i of sequence b turns by the angles (len[b] + depth[b][i]) *
- * rope_base^(-t/64), t < 64, computed in 64 bits and rounded to fp32 as cosine and sine; the bias
- * is added in fp32 and each output is rounded to fp16 once.  Writes Q [B][N][num_heads*128], TK and TV
+ * rope_base^(-t/64), t < 64, formed and reduced to one turn in 64 bits; their cosines and sines are fp32, within 2^-21 for
+ * angles up to 2^24.  The bias is added in fp32 and each output is rounded to fp16 once.  Writes Q [B][N][num_heads*128], TK and TV
  * [B][N][num_kv_heads*128], which may not overlap qkv.  All pointers to fp16 are 16-byte aligned. */
 int llmdiy_tree_rope(const uint16_t* qkv, const uint16_t* bias, const int* depth, const int* len,
                      const int* tree_len, int B, int N, int num_heads, int num_kv_heads, float rope_base,
