@@ -23,7 +23,7 @@
 //   O    += P(j) V(j)         128 x 128, K = 2 x 64 keys   -> TMEM (P from TMEM, in the place of S(j))
 // S(j+1) is computed while the rows are at S(j), S(j+2) when the product that reads P(j) is complete.  Warps 0-3 own the
 // rows (thread = row = TMEM lane): mask, online softmax in base 2; O is rescaled only when a row's maximum grows by more
-// than 2^8 (P stays within fp16, and O / l does not depend on the reference point).
+// than 2^7 (P stays within fp16, and O / l does not depend on the reference point).
 //
 // P goes to the tensor cores as the sum of two fp16 terms, p = hi + lo, for rows of every call alike: half a step of one
 // term is 2^-11 of each probability, whose scatter in the output is as large as the output's own rounding (2.9e-4 of the
@@ -309,10 +309,13 @@ LLMDIY_DEV float ta_ex2v(float x) {  // as ta_ex2, issued where it stands
 }
 constexpr float kTaScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
 // Probabilities are formed as 2^(x - m + kTaRaise), o and l alike, which divides out. A row's reference m stays within
-// 2^8 of its maximum, so they reach 2^15 at most, and of fp16's range below 1 as much as can be is left to the small
-// ones: beside a key that takes nearly all the weight but has a small value, the output is made of those. Relative to
+// 2^kTaGrow of its maximum, so they reach 2^15 at most (7 - m may round to 8 - m), and of fp16's range below 1 as much as
+// can be is left to the small ones: beside a key that takes nearly all the weight but has a small value, the output is made of those. Relative to
 // the largest the rounding is 2^-32 at least where it was 2^-25 without (keys at 2^-24.6 of it were 52% off).
-constexpr float kTaRaise = 7.f;
+// The exponent is a rounded product, as m is one, and then a sum, and what m is compared by is a difference: both are exact
+// near the maximum whatever the scores' size (in one fused operation the product's rounding error is left over, which
+// passes fp16 from scores of 2^24 doublings on; a packed product and sum are made into one, a packed fma and a sum are not).
+constexpr float kTaRaise = 7.f, kTaGrow = 7.f;
 
 // add[e] += p v[dim0 + e] of the tree rows base + bit that `hit` names, for one query row (out of line: rare).
 __device__ __noinline__ void ta_add_bad(const TaArgs& a, uint64_t hit, int b, int node, int base, int kvh, int h,
@@ -324,7 +327,7 @@ __device__ __noinline__ void ta_add_bad(const TaArgs& a, uint64_t hit, int b, in
         const half* qr = a.Q + ((size_t)b * a.N + node) * a.ldq + h * kTaDim;
         float d = 0.f;
         for (int e = 0; e < kTaDim; ++e) d = __fmaf_rn(h2f(qr[e]), h2f(kr[e]), d);
-        const float p = ta_ex2(__fmaf_rn(d, kTaScaleLog2, nm));
+        const float p = ta_ex2(__fadd_rn(__fmul_rn(d, kTaScaleLog2), nm));
         for (int e = 0; e < 32; ++e) add[e] = __fmaf_rn(p, h2f(vr[dim0 + e]), add[e]);
     }
 }
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
                     for (int q = 12; q < 60; q += 2) mx[(q >> 1) & 3] = ta_max3(mx[(q >> 1) & 3], x[q], x[q + 1]);
                     const float top = ta_max3(ta_max3(mx[0], x[60], x[61]), ta_max3(mx[1], x[62], x[63]),
                                               fmaxf(mx[2], mx[3])) * kTaScaleLog2;
-                    const bool grow = live && top > m + (t == t0 ? 0.f : 8.f);  // (a NaN maximum leaves m)
+                    const bool grow = live && top - m > kTaGrow;  // (m = -inf at first; a NaN maximum leaves m)
                     if (__builtin_expect(t != t0 && __any_sync(0xffffffffu, grow), 0)) {
                         // rescale O, complete through PV(j-1) (the whole warp: TMEM moves 32 rows at a time)
                         if (!warp_wait(&s.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) { ok = false; break; }
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
 #pragma unroll
                         for (int q = 0; q < 16; q += 2) {
                             float a0, a1;
-                            ta_split(ta_fma2(ta_f2(x[q0 + q], x[q0 + q + 1]), scale2, nm2), a0, a1);
+                            ta_split(ta_add2(ta_fma2(ta_f2(x[q0 + q], x[q0 + q + 1]), scale2, 0), nm2), a0, a1);
                             to[q] = ta_ex2v(a0);
                             to[q + 1] = ta_ex2v(a1);
                         }

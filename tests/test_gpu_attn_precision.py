@@ -76,3 +76,33 @@ def test_attn_values_that_cancel(B, N, H, KV, room, drop):
     a.V[:, 1::2] = (-a.V[:, ::2][:, : a.V[:, 1::2].shape[1]].astype(np.float64) / p).astype(np.float16)
     a.device().call()
     _check(a, 22)
+
+
+@pytest.mark.parametrize("size", [300.0, 3000.0, 10000.0])
+@pytest.mark.parametrize("B,N,H,KV,room", [(1, 26, 16, 16, 2047), (1, 100, 4, 2, 1500), (2, 8, 8, 1, 33000),
+                                           (3, 100, 8, 1, 13000), (1, 2, 1, 1, 1000)])
+def test_attn_scores_of_any_size(B, N, H, KV, room, size):
+    """Scores of up to 2^36 doublings: a row's largest takes all, to the last bit of the output."""
+    m = min(room, 2047)
+    a = Attn(N, B, N, H, KV, [m - 3 * b for b in range(B)], max_len=room)
+    for x in (a.Q, a.K, a.TK):
+        x[...] = (x.astype(np.float32) * size).astype(np.float16)
+    a.device().call()
+    torch().cuda.synchronize()
+    got = a.d["O"].cpu().numpy()
+    seen = 0
+    for b in range(B):
+        for i in range(0, N, 5):
+            for h in range(H):
+                cols = slice(h * KV // H * D, (h * KV // H + 1) * D)
+                js = sorted(a.sees[b][i])
+                K = np.concatenate([a.K[b, :a.lens[b], cols], a.TK[b, js][:, cols]]).astype(np.float64)
+                V = np.concatenate([a.V[b, :a.lens[b], cols], a.TV[b, js][:, cols]])
+                q = a.Q[b, i, h * D:(h + 1) * D].astype(np.float64)
+                s = K @ q / np.sqrt(128.0)
+                first, second = np.argsort(s)[[-1, -2]]
+                # sums of 128 products, each addition within 2^-23 of the products' sizes, and 64 more doublings
+                if s[first] - s[second] > (np.abs(K) @ np.abs(q)).max() * 128 * 2.0 ** -23 + 64:
+                    seen += 1
+                    assert np.array_equal(got[b, i, h * D:(h + 1) * D], V[first]), (b, i, h)
+    assert seen >= 2 * ((N + 4) // 5) * H * B // 3
