@@ -939,17 +939,17 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     p.ok = units * (tiles + kTaUnitCost) <= 0x7fffffffLL;
     const int slots = std::max(kTaCtasPerSm * ta_sms(), p.mt);
     // Flat CTAs have four tiles or more, and a unit is cut into sqrt(2 tiles) parts at most: joining costs about half as much
-    // a part as the products a tile.  1 unit of 1025 tiles, 128 rows: 47.3 us with sqrt(tiles) parts, 43.8 so,
-    // 45.2 with sqrt(5 tiles), 93.6 with 296.
+    // a part as the products a tile.  1 unit of 1025 tiles, 128 rows: 49.4 us with sqrt(tiles) parts, 45.6 so,
+    // 47.3 with sqrt(5 tiles), 106 with 296.
     const double parts = std::sqrt(2.0 * (double)tiles);
     p.W = (int)std::max<long long>(
         1, std::min<long long>({slots / p.mt, units / p.mt * tiles / 4, (long long)((double)(units / p.mt) * parts)}));
     p.floats = (size_t)std::min<long long>(slots, units * tiles) * 2 * p.rows * (kTaDim + 2);
     // Units of up to four rows whose CTAs' shares are short go to the kernel for those: the products of a CTA, rows x
-    // cache rows, decide.  Measured (this kernel / the one for few rows): 16 units of 1 row over 1023 9.4 / 5.6, over 8192
-    // (1024 a CTA) 23.4 / 19.9, over 131072 183 / 243; 2 rows over 4096 (512 a CTA) 15.7 / 13.8, over 8192 23.8 / 23.3; 4 over
-    // 1023 9.6 / 7.9, over 4000 (500 a CTA) 15.5 / 20.0; 32 units of 4 over 2048 (256 a CTA) 13.4 / 14.4; 1024 units of 1
-    // over up to 300 36.7 / 26.5, over up to 1000 57.6 / 52.2.
+    // cache rows, decide.  Measured (this kernel / the one for few rows): 16 units of 1 row over 1023 8.8 / 4.9, over 8192
+    // (1024 a CTA) 19.3 / 18.8, over 131072 179 / 240; 2 rows over 4096 (512 a CTA) 13.8 / 13.1, over 8192 19.4 / 22.3; 4 over
+    // 1023 9.2 / 7.4, over 4000 (500 a CTA) 13.6 / 19.2; 32 units of 4 over 2048 (256 a CTA) 12.9 / 13.3; 1024 units of 1
+    // over up to 300 37.6 / 24.1, over up to 1000 61.7 / 50.1.
     if (p.rows <= kFewRows) {
         const int c = (int)std::max<long long>(1, std::min<long long>({kFewCluster, slots / units, (max_len + 63) / 64}));
         if ((long long)p.rows * ((max_len + c - 1) / c) <= (p.rows <= 2 ? 1024 : 768)) p.few = c;
@@ -957,14 +957,16 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
     // Direct or flat, by what both would take if every sequence were max_len long, in us.  A CTA that runs its chain of
     // products undisturbed needs 0.75 a tile (1.0 with more than 32 rows), and all slots together 1.46 a tile and slot from
     // HBM; a flat call pays for its second launch and for joining W / units partials a row.  Of sequences
-    // of different lengths direct waits for the longest, so several of them with more than
-    // kTaDirectTiles tiles a CTA go flat.  Measured (direct / flat): 16 units of 17 tiles 9.9 / 17.4, 16 of 2049 203 / 184,
-    // 16 of 514 (128 rows) 78 / 68, 2 of 126 20 / 59, 1024 of up to 33 103 / 122, 256 of up to 66 67 / 67.
+    // of different lengths direct waits for the longest, and its clusters do not fill the GPU evenly, so calls with more than
+    // kTaDirectTiles tiles a CTA go flat.  Measured (direct / flat), 16 rows: 16 units of 17 tiles 9.3 / 14.5, 2 of 126 12.2 /
+    // 18.9, 1024 of up to 33 110 / 118, 256 of up to 66 75 / 59; 8 rows: 16 units of 513 53 / 57, 769 77 / 78, 1025 102 / 96,
+    // 2049 201 / 180, 8 of 513 41 / 41, 1025 74 / 62; 64 rows: 16 of 513 58 / 59, 769 85 / 80, 2049 218 / 190; 128 rows: 16 of
+    // 514 64 / 66, 1026 120 / 110.
     // CTAs per unit (direct): the tiles of one, the cluster's barriers and its join (rows by 14 a time) against one another, in
     // us.  Clusters of more than two leave gaps: 7/8 of the slots are counted, and where 8 GPCs' SMs do not take all clusters one CTA to an
-    // SM, units of many rows slow each other.  Measured with 1 / 2 / 4 / 8 CTAs: 12 units of 2 tiles and 115 rows 7.7 / 10.5 / 9.1 / 9.2;
-    // 96 of 4 and 83 rows 11.1 / 11.9 / 17.5 / 27.3; 64 of 6 and 8 rows 10.3 / 9.9 / 8.8 / 15.9; 16 of 33 and 26 rows 29.9 / 19.3 /
-    // 12.8 / 10.8; 20 of 28 and 125 rows 28.2 / 21.1 / 15.1 / 15.4 (14.0 with 5).
+    // SM, units of many rows slow each other.  Measured with 1 / 2 / 4 / 8 CTAs: 12 units of 3 tiles and 115 rows 9.8 / 11.3 / 9.4 / 9.9;
+    // 96 of 4 and 83 rows 10.5 / 12.9 / 19.2 / 30.2; 64 of 6 and 8 rows 10.0 / 9.8 / 8.5 / 16.1; 16 of 33 and 26 rows 29.9 / 19.1 /
+    // 12.8 / 11.6; 20 of 28 and 125 rows 32.0 / 22.4 / 15.6 / 16.8 (14.4 with 5).
     int c = 1;
     double best = 1e30;
     for (int k = 1; k <= std::min<long long>(kTaCluster, tiles); ++k) {
@@ -978,16 +980,16 @@ TaPlan ta_plan(int B, int N, int H, int KV, int max_len) {
         }
     }
     // Clusters of 12 or 16 for many tiles, where the units' all run at once: such clusters leave gaps, 21 and 14 of them fit
-    // on 148 SMs (16 x 16 CTAs do not, and took 17.6 us against 10.7), so three quarters of the slots are counted.
-    // Measured (8 / 16 CTAs), 8 units of 34 tiles 11.7 / 13.4, 2 of 65 14.7 / 11.2, 8 of 129 18.7 / 14.9; (8 / 12), 16
-    // of 34 10.7 / 10.7, of 129 23.8 / 21.1.
+    // on 148 SMs (16 x 16 CTAs do not, and take 18.3 us against 11.5), so three quarters of the slots are counted.
+    // Measured (8 / 16 CTAs), 8 units of 34 tiles 9.7 / 10.2, 2 of 65 12.2 / 9.8, 8 of 129 18.7 / 16.8; (8 / 12), 16
+    // of 34 11.4 / 10.4, of 129 24.0 / 19.8.
     if (tiles > 6 * kTaCluster && c == kTaCluster)
         c = units * 16 * 4 <= slots * 3 ? 16 : units * 12 * 4 <= slots * 3 ? 12 : c;
     const double t = (double)((tiles + c - 1) / c), chain = p.rows > 32 ? 1.0 : 0.75, hbm = 1.46 / slots;
     const double flat_ctas = (double)p.W * p.mt;
     const double direct_us = 9.0 + t * std::max(chain, hbm * std::min<double>(slots, units * c));
     const double flat_us = 20.0 + units * tiles / flat_ctas * std::max(chain, hbm * flat_ctas) + 0.12 * flat_ctas / units;
-    if (direct_us < flat_us && (B == 1 || t <= kTaDirectTiles)) p.cluster = c;
+    if (direct_us < flat_us && t <= kTaDirectTiles) p.cluster = c;
     return p;
 }
 

@@ -9,7 +9,7 @@
 // that no cluster barrier follows the loads; every join is in a fixed order.
 //
 // Launch, two dependent loads (lengths, rows) and the joins' latency bound it: one row of 16 heads over 1023 cache rows takes
-// 5.6 us (the tensor-core kernel 9.4), over 300 5.2.  Tried: the next keys loaded ahead (one row 5.9 us, four rows
+// 5.0 us in a graph (the tensor-core kernel 8.8), over 300 4.5.  Tried: the next keys loaded ahead (one row 5.9 us, four rows
 // 9.1 against 8.8), a shuffle sum and an exponential of its own for every key of a lane (5.7 and 8.8; now 8.1).
 #pragma once
 

@@ -162,7 +162,7 @@ def test_refuses_misaligned_words_and_overlong_rows(call, good, bad):
 
 @pytest.mark.parametrize("sizes,path", [
     ((1, 1, 16, 16, 1023), 2), ((1, 4, 2, 2, 1000), 2), ((1, 26, 16, 16, 2047), 1), ((1, 1, 8, 1, 30000), 1),
-    ((3, 100, 4, 2, 30001), 1), ((16, 64, 16, 16, 4160), 0), ((2, 48, 32, 8, 65536), 0), ((1, 1, 8, 1, 131072), 0),
+    ((3, 100, 4, 2, 30001), 1), ((16, 64, 16, 16, 4160), 0), ((2, 48, 32, 8, 65536), 0), ((1, 1, 8, 1, 131072), 0), ((1, 64, 16, 16, 131072), 0),
     ((0, 8, 16, 16, 10), -1), ((1, 257, 16, 16, 10), -1), ((1, 8, 16, 5, 10), -1), ((1, 8, 16, 16, -1), -1)])
 def test_attn_path(sizes, path):
     """The way a call takes, by its sizes (on a machine without a GPU as for 148 SMs)."""
