@@ -10,7 +10,8 @@
  * value (cudaErrorInvalidValue for refused arguments, before anything is launched; B <= 65535, at most 1024 heads,
  * V <= 2^30), outputs that overlap no input and no other output, no allocation,
  * no synchronisation: every launcher can be captured into a CUDA graph, and the lengths, trees and slots are
- * read on the device when it runs.
+ * read on the device when it runs.  Calls launch clusters of up to 16 CTAs; a part of a GPU that cannot place them
+ * answers with the launch's error.
  *
  * The tree.  Sequence b (0 <= b < B) has nodes 0 .. tree_len[b]-1 (tree_len NULL: N each; values
  * are clamped to 0..N), N <= 256.  Node 0 is the root: the last token of the sequence, whose K/V
@@ -18,8 +19,8 @@
  * Arrays over nodes are [B][N]; what belongs to nodes at or past tree_len[b] has no
  * effect and, in the outputs of tree_rope and tree_attn, is left as it was.
  *
- * The cache.  The caller's, laid out as a batch's (llmdiy_batch.h), whose own is not handed out: row r of kv head h of slot s is at
- * (s * slot_rows + r) * stride + h * 128 elements, in K and in V; sequence b uses slot[b] (NULL: slot
+ * The cache.  The caller's, laid out as a batch's (llmdiy_batch.h), whose own is not handed out: row r of kv
+ * head h of slot s is at (s * slot_rows + r) * stride + h * 128 elements, in K and in V; sequence b uses slot[b] (NULL: slot
  * b) and has len[b] committed rows (positions 0 .. len[b]-1).  The tree's own K/V rows live in buffers
  * [B][N][num_kv_heads*128] until llmdiy_tree_commit.  A slot outside 0..num_slots-1 has no rows.
  */
@@ -85,7 +86,8 @@ int llmdiy_tree_attn_status(const float* work);
  * probs = exp((x - max) / temp[r]) / sum in fp32, temp NULL = 1.  temp <= 0 (or NaN) gives the limit: equal shares
  * of the row's largest entries (greedy; llmdiy_argmax picks one of them by a rule of its own).  Entries of -inf get 0; a
  * row with nothing above -inf gives zeros; one with a NaN or +inf is NaN throughout.  A bounded wait that expires (nothing
- * else reports it) makes NaN of its row, or of parts of it, and of those that were still to come. */
+ * else reports it) makes NaN of its row, or of parts of it, and of those that were still to come.  Rows of up to 156600
+ * entries are read once; of longer ones the rest is read three times and takes about twice as long an entry. */
 int llmdiy_softmax_rows(const uint16_t* logits, int ldl, const float* temp, int R, int V, float* probs, int ldp,
                         void* stream);
 
@@ -113,7 +115,7 @@ int llmdiy_tree_verify(const float* target, int ldt, const float* draft, int ldd
 /* Moves the root's and the accepted nodes' K/V rows into the cache, for `layers` layers: rows 0, path[b][0], ..,
  * path[b][accepted[b]-1] of TK/TV become cache rows len[b], len[b]+1, .. of slot[b].  Layer l's tree buffers are
  * tree_layer_stride elements, its caches layer_stride elements after layer 0's.  len_out (may be NULL, may not be
- * len) gets len[b] + 1 + accepted[b].  Rows past slot_rows are dropped (len_out stops at slot_rows), a path entry
+ * len) gets len[b] + 1 + accepted[b] (of which N - 1 at most count).  Rows past slot_rows are dropped (len_out stops at slot_rows), a path entry
  * outside 0..N-1 leaves its cache row as it was, and accepted < 0 or a slot or len out of range moves
  * nothing (len_out = len).  No two sequences may share a slot; TK/TV may not overlap the caches. */
 int llmdiy_tree_commit(const uint16_t* TK, const uint16_t* TV, size_t tree_layer_stride, uint16_t* K, uint16_t* V,

@@ -10,8 +10,9 @@
 // loop.  x - m is exact in fp32 for fp16 x (but for far smaller x, whose share is 0), so
 // the exponent carries two roundings (k and the product).
 //
-// Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 127.9 us, 5.5 TB/s of the 6.5 of
-// a copy.  A row is in work for about 5 us (shared-memory loads, 16 warps' exponentials, the exchange of the cluster's
+// Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 125 us, 5.6 TB/s of the 6.5 of
+// a copy.  What a cluster of nine cannot hold, entries past 156600 (9 kSmSlice) of a row, is read three times, two bytes at a
+// time: 400 rows of 151936 take 67 us (5.5 TB/s), of 200000 180 (2.7 TB/s), of 262144 230.  A row is in work for about 5 us (shared-memory loads, 16 warps' exponentials, the exchange of the cluster's
 // pairs), with 30 clusters of 9 resident.  Rejected: the whole CTA's maximum and sum by barriers and plain stores (clusters
 // of 8, 141.7 us; an SM writes 32 bytes a cycle, and the warps wait for that), plain stores without barriers (139.7), one or
 // two of a thread's pairs in plain stores for clusters of 8 (137 to 142), clusters of 10 (138.6), rows fetched into L2 two
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(kSmThreads, kSmCtasPerSm)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r0 = blockIdx.x / C, step = gridDim.x / C;
     const int v0 = min(V, rank * slice), n = min(V, v0 + slice) - v0;  // this CTA's entries of every row
-    const int held = min(n, kSmSlice);  // those past the registers (rows of more than 8 kSmSlice) are read again
+    const int held = min(n, kSmSlice);  // those past the registers (rows of more than kSmMaxCluster kSmSlice) are read again
     const uint16_t* base = reinterpret_cast<const uint16_t*>(logits);
     const uintptr_t first = reinterpret_cast<uintptr_t>(base), last = first + 2 * ((uintptr_t)(R - 1) * ldl + V);
     const uint64_t pol = l2_policy_evict_first();

@@ -42,7 +42,7 @@ LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
 
 // ---------------------------------------------------------------- bias + RoPE
 // One CTA per node, bound by the latency of its loads (1536 nodes of 48 heads' rows 7.5 us, 4.2 TB/s of the 6.5 of a copy, in
-// one wave and a half).  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
+// one wave and a third: 64 registers let 8 CTAs on an SM, 1184 of those nodes at once).  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
 // to [-pi, pi] in 64 bits (a position of 10^5 leaves fp32 angles only 2 digits after the point), its sine
 // and cosine are then taken in fp32 (absolute error < 2^-21 to angles of 2^24: 2^-23 of the reduced angle's rounding, two
 // units of the last place of sine or cosine, 2^-25 of the 64-bit product; the fp16 outputs are rounded by 2^-11).  The 64
@@ -120,9 +120,12 @@ __global__ void __launch_bounds__(kRopeThreads)
 // into blocks of 128 entries, dealt contiguously to the cluster's warps (warp k of K: blocks
 // [k U / K, (k + 1) U / K)), so the warps' totals in order are a running sum over the row.
 //
-// What bounds it is the walk: a refusal needs the sum over two rows before the next child can be tried, about 2.5 us a
-// round at a new node, 1.3 of them the rows' loads, and 1.2 (the exchange) at the same one.  V = 151936: a chain 7.6 us, 24
-// trees of 32 nodes 33.  Tried: blocks held in registers (two fit; 8.8 and 36.5 us), the root's rows fetched into L2 while
+// What bounds it is the walk: a refusal needs the sum over two rows before the next child can be tried.  V = 151936, in a
+// graph: one sequence without a refusal 6.4 us, the first refusal 2.0 more (the draft's row), each further one at the same node 2.5
+// to 3, at a new node 4.3 (its rows' loads); with 24 sequences 10.3, 6.9, 6.0 and 9 to 10.  There a round at the same
+// node is the 64-bit arithmetic and its conversions on two CTAs' shares an SM, and a fifth of the rows (what does not fit
+// kVerHeld) read again.  A chain of 4 takes 7.7 us (one round), 24 trees of 32 nodes 33 (up to five rounds at up to
+// two nodes, 29 to 39 MB read).  Tried: blocks held in registers (two fit; 8.8 and 36.5 us), the root's rows fetched into L2 while
 // the tree is read (24 trees 38.9 us against 35.5), the weights as two fp32 terms in place of fp64 (37.5 against 36.3).
 constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / 32;

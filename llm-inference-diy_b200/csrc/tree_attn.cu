@@ -28,22 +28,24 @@
 // P goes to the tensor cores as the sum of two fp16 terms, p = hi + lo, for rows of every call alike: half a step of one
 // term is 2^-11 of each probability, whose scatter in the output is as large as the output's own rounding (2.9e-4 of the
 // norm together on normal inputs, 2.1e-4 with two terms, as fp32 probabilities give), and shows as it is where values cancel.  Two terms leave
-// 2^-22 of each, or 2^-32 of the row's largest (kTaRaise); l sums the unrounded fp32 values.  They cost 1.0 us of 11.3
-// (26 nodes over 2047 rows), 9 of 72 (16 ragged trees) and 31 of 183 (2 x 48 nodes over 65536 rows, grouped), for the second
-// product and a conversion back.  With one S buffer, and P beside it, the rows wait for the last product before they can store P: 12.1,
-// 85 and 226 us for these.
+// 2^-22 of each, or 2^-32 of the row's largest (kTaRaise); l sums the unrounded fp32 values.  They cost 1.1 us of 11.3
+// per call (26 nodes over 2047 rows), 8 of 71 (16 ragged trees) and 32 of 183 (2 x 48 nodes over 65536 rows, grouped): 28 of
+// these the second product, the others its conversions.  With one S buffer, and P beside it, the rows wait for the last
+// product before they can store P: 12.1, 85 and 226 us for these.
 //
 // What a row does not see must not reach it even as NaN * 0: masked scores are replaced by -inf
 // (K may hold anything there), and V rows past the end, as well as tree rows with an Inf or NaN, are zeroed in
 // shared memory before PV; the few rows that do see such a tree row add p * v themselves at the end.
 //
-// Bounds and what was measured.  Short caches: launch, barriers, TMEM and first instructions (about 7 us) and 0.75 us a tile;
-// 26 nodes x 16 heads over 2047 rows take 10.8 us (5 tiles a CTA).  Long ones: HBM for few rows (64 nodes over 131072 rows of
-// 16 heads 198 us, 5.4 TB/s of the 6.5 of a copy), the softmax of a tile's rows for many (2 x 48 nodes, 32 heads on 8, over 65536
-// rows 153 us, 637 TFLOP/s: 128 rows x 64 exponentials, two CTAs to an SM, one tile in 1.2 us each).  Ragged batches:
-// 16 trees of 64 nodes, 16 heads, over up to 4160 rows 66.5 us, about 56 of products at 5.4 TB/s and 10 of joining.
-// Rejected: two threads a row (94 us there), unrolling the tile loop (78), fetching K and V into L2 a tile further
-// ahead (131072 rows 211 us against 182), rows repeated over the lanes of small units, other joins (4 or 8 warps a block).
+// Bounds and what was measured (in a graph, where not said otherwise).  Short caches: launch, barriers, TMEM and first
+// instructions (about 7 us) and 0.9 us a tile; 26 nodes x 16 heads over 2047 rows take 11.8 us (5 tiles a CTA), 12.4 per call.
+// Long ones: HBM for few rows (64 nodes over 131072 rows of 16 heads 188 us, 5.7 TB/s of the 6.5 of a copy), for many the
+// chain S, softmax, P, PV of a tile, with the tensor pipe at 67% (2 x 48 nodes, 32 heads on 8, over 65536 rows 176 us, 555
+// TFLOP/s of S and one P; 215 per call, where it runs for long enough to meet the power limit: 1.58 GHz and less).  Ragged
+// batches: 16 trees of 64 nodes, 16 heads, over up to 4160 rows 67 us, 79 per call, about 10 of them joining.
+// Rejected, measured with P in one fp16 term (66.5 us that batch): two threads a row (94), unrolling the tile loop (78),
+// fetching K and V into L2 a tile further ahead (131072 rows 211 us against 182), rows repeated over the lanes of small
+// units, other joins (4 or 8 warps a block).
 //
 // Every wait is bounded; on expiry the CTA records an error in *err, waits (bounded) for its copies and
 // MMAs in flight, frees its TMEM and returns.
@@ -73,7 +75,8 @@ constexpr uint32_t kTaCols = 256;                   // TMEM: two buffers of S, t
 constexpr int kTaDirectTiles = 48;  // (see ta_plan)
 constexpr int kTaMaxGroup = 128;                    // query heads per kv head at most
 constexpr int kTaCluster = 8;     // CTAs per unit (direct); long caches of few units take 12 or 16 (see ta_plan)
-constexpr int kTaUnitCost = 4;  // a unit's beginning and end in tiles (16 ragged trees: 1 70.9 us, 2 67.9, 4 67.2, 6 66.8, 10 68.4)
+// a unit's beginning and end in tiles (16 ragged trees, P in one term: 1 70.9 us, 2 67.9, 4 67.2, 6 66.8, 10 68.4)
+constexpr int kTaUnitCost = 4;
 
 // Two layouts of the same kernel: units of up to 64 rows need only 16 KB for Q and get a third V
 // stage; the MMA still reads 128 rows, so rows 64-127 of its A operand are whatever lies behind
@@ -388,8 +391,8 @@ __global__ void __launch_bounds__(kTaThreads, kTaCtasPerSm)
         ta_shape(a, c.b, c.n, c.L, c.tiles, c.units);
         if (m0 < c.n) {
             // The unit's last tiles (the cache's tail, the tree) take up to two tiles longer: the last CTAs get that many
-            // fewer where the others have as many.  16 x 17 tiles: 11.2 us with equal shares, 9.6 so; with 2 or 5
-            // tiles in all equal shares are better (7.4 and 8.2 us against 8.9 and 8.7).
+            // fewer where the others have as many.  16 x 17 tiles: 11.0 us with equal shares, 9.8 so; with 2 or 5
+            // tiles in all equal shares are better (6.9 and 8.2 us against 7.0 and 8.4).
             const int span = c.tiles + min(2, (c.tiles - 1) / C);
             const int t0 = min(span * rank / C, c.tiles), t1 = min(span * (rank + 1) / C, c.tiles);
             c.at = kTaUnitCost + t0;
