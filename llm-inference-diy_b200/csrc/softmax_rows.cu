@@ -12,7 +12,8 @@
 //
 // Reading 2 and writing 4 bytes an entry is the bound: 768 rows of 151936 entries take 125 us, 5.6 TB/s of the 6.5 of
 // a copy.  What a cluster of nine cannot hold, entries past 156600 (9 kSmSlice) of a row, is read three times, two bytes at a
-// time: 400 rows of 151936 take 67 us (5.5 TB/s), of 200000 180 (2.7 TB/s), of 262144 230.  A row is in work for about 5 us (shared-memory loads, 16 warps' exponentials, the exchange of the cluster's
+// time: 400 rows of 151936 take 67 us (5.5 TB/s), of 200000 180 (2.7 TB/s), of 262144 230.  A row is in work for about
+// 5 us (shared-memory loads, 16 warps' exponentials, the exchange of the cluster's
 // pairs), with 30 clusters of 9 resident.  Rejected: the whole CTA's maximum and sum by barriers and plain stores (clusters
 // of 8, 141.7 us; an SM writes 32 bytes a cycle, and the warps wait for that), plain stores without barriers (139.7), one or
 // two of a thread's pairs in plain stores for clusters of 8 (137 to 142), clusters of 10 (138.6), rows fetched into L2 two

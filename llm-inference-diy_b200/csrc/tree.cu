@@ -42,8 +42,8 @@ LLMDIY_DEV int nodes_of(const int* tree_len, int b, int N) {
 
 // ---------------------------------------------------------------- bias + RoPE
 // One CTA per node, bound by the latency of its loads (1536 nodes of 48 heads' rows 7.5 us, 4.2 TB/s of the 6.5 of a copy, in
-// one wave and a third: 64 registers let 8 CTAs on an SM, 1184 of those nodes at once).  (y_t, y_{t+64}) turns by a = pos * base^(-t/64): the angle is formed and reduced
-// to [-pi, pi] in 64 bits (a position of 10^5 leaves fp32 angles only 2 digits after the point), its sine
+// one wave and a third: 64 registers let 8 CTAs on an SM, 1184 of those nodes at once).  (y_t, y_{t+64}) turns by
+// a = pos * base^(-t/64): the angle is formed and reduced to [-pi, pi] in 64 bits (a position of 10^5 leaves fp32 angles only 2 digits after the point), its sine
 // and cosine are then taken in fp32 (absolute error < 2^-21 to angles of 2^24: 2^-23 of the reduced angle's rounding, two
 // units of the last place of sine or cosine, 2^-25 of the 64-bit product; the fp16 outputs are rounded by 2^-11).  The 64
 // frequencies come as a kernel argument, and the first rows' loads are under way while the angles are computed.

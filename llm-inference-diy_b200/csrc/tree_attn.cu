@@ -27,8 +27,8 @@
 //
 // P goes to the tensor cores as the sum of two fp16 terms, p = hi + lo, for rows of every call alike: half a step of one
 // term is 2^-11 of each probability, whose scatter in the output is as large as the output's own rounding (2.9e-4 of the
-// norm together on normal inputs, 2.1e-4 with two terms, as fp32 probabilities give), and shows as it is where values cancel.  Two terms leave
-// 2^-22 of each, or 2^-32 of the row's largest (kTaRaise); l sums the unrounded fp32 values.  They cost 1.1 us of 11.3
+// norm together on normal inputs, 2.1e-4 with two terms, as fp32 probabilities give), and shows as it is where values
+// cancel.  Two terms leave 2^-22 of each, or 2^-32 of the row's largest (kTaRaise); l sums the unrounded fp32 values.  They cost 1.1 us of 11.3
 // per call (26 nodes over 2047 rows), 8 of 71 (16 ragged trees) and 32 of 183 (2 x 48 nodes over 65536 rows, grouped): 28 of
 // these the second product, the others its conversions.  With one S buffer, and P beside it, the rows wait for the last
 // product before they can store P: 12.1, 85 and 226 us for these.
@@ -313,8 +313,9 @@ LLMDIY_DEV float ta_ex2v(float x) {  // as ta_ex2, issued where it stands
 constexpr float kTaScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
 // Probabilities are formed as 2^(x - m + kTaRaise), o and l alike, which divides out. A row's reference m stays within
 // 2^kTaGrow of its maximum, so they reach 2^15 at most (7 - m may round to 8 - m), and of fp16's range below 1 as much as
-// can be is left to the small ones: beside a key that takes nearly all the weight but has a small value, the output is made of those. Relative to
-// the largest the rounding is 2^-32 at least where it was 2^-25 without (keys at 2^-24.6 of it were 52% off).
+// can be is left to the small ones: beside a key that takes nearly all the weight but has a small value, the output is
+// made of those. Relative to the largest the rounding is 2^-32, where it was 2^-25 without (keys at 2^-24.6 of it were
+// 52% off).
 // The exponent is a rounded product, as m is one, and then a sum, and what m is compared by is a difference: both are exact
 // near the maximum whatever the scores' size (in one fused operation the product's rounding error is left over, which
 // passes fp16 from scores of 2^24 doublings on; a packed product and sum are made into one, a packed fma and a sum are not).
